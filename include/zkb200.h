@@ -529,6 +529,68 @@ int32_t zkb_oplist_activation(zkb_oplist* list, uint32_t op_index, uint32_t* out
 /* forward pass + all proofs */
 int32_t zkb_oplist_prove(zkb_oplist* list, const uint32_t* x, uint8_t* out, size_t cap, size_t* len);
 
+/* ---- token-by-token forward passes: a paged key-value cache, the attention that reads it, projections with adapters ----
+ * No counterpart in the reference, whose forward pass takes whole sequences or one vector.  The arithmetic is its own, though: field
+ * elements and the centred integers they stand for, so a row computed over the cache is the row that zkb_row_attention(_gqa)_forward
+ * computes and zkb_prove_row_attention(_gqa) proves, and a projection with an adapter is the product with the merged matrix W + B A.
+ * All pointers are device memory of the context's GPU; calls are enqueued on the context's stream and nothing is waited for, so
+ * they can be captured into a graph from that stream.  What only the device sees goes into the caller's status words, one per sequence:
+ * status[s] becomes the largest code that a call found, and stays until the caller clears it. */
+enum { ZKB_SERVE_PAGE = 1,        /* a length or position outside the block table, or a page number outside the pool */
+       ZKB_SERVE_ROTATION = 2,    /* a position that the rotation's table does not have */
+       ZKB_SERVE_RANGE = 3,       /* a value that a 16-bit cache cannot hold */
+       ZKB_SERVE_SCORE = 4,       /* a score that is not an input of the exp table (where attention.rs:105 panics) */
+       ZKB_SERVE_ZERO_SUM = 5 };  /* the weights of a row add up to zero (attention.rs:108) */
+enum { ZKB_KV_FIELD = 0,          /* canonical u32 */
+       ZKB_KV_I16 = 1 };          /* int16, the centred value: activations after requantisation */
+#define ZKB_KV_MAX_D_HEAD 256
+/* Pages of [num_kv_heads][page_size][d_head] elements, page i at i * page_stride elements from the base (0: dense; a larger stride lets K and
+ * V pages of one pool alternate).  page_size is a power of two.  d_head up to 256, any value; rows of whole 16-byte groups whose
+ * base and stride are 16-byte aligned take the fast path. */
+typedef struct {
+    void* k_pages_dev;
+    void* v_pages_dev;
+    uint64_t page_stride;
+    uint32_t num_pages, page_size, num_kv_heads, d_head;
+    int32_t elem;
+} zkb_kv_cache;
+/* cos_sin_dev: [positions][rot_dim / 2][2] signed integers with `shift` fractional bits.  The first rot_dim elements of a head turn: element
+ * i with i + rot_dim / 2 (pairs = 0) or 2i with 2i + 1 (pairs = 1), x' = rnd((x c - y s) / 2^shift), y' = rnd((x s + y c) / 2^shift) on centred
+ * integers, rounded half away from zero, then mod p. */
+typedef struct {
+    const int32_t* cos_sin_dev;
+    uint32_t positions, rot_dim, shift;
+    int32_t pairs;
+} zkb_kv_rotation;
+/* Keys and values of new tokens into the cache.  k, v: (num_tokens, num_kv_heads, d_head), tokens *_stride words apart (0: dense).  Sequence s
+ * brings the tokens row_start[s] .. row_start[s + 1] - 1 (num_seqs + 1 nondecreasing entries); they get the positions from start[s] on, and
+ * position p lies in row p % page_size of page block_table[s][p / page_size] (num_seqs x max_blocks entries; places that no new position needs
+ * may hold anything).  Tokens before row_start[0] and from row_start[num_seqs] on are padding: nothing is read or written for them.  With a
+ * rotation (NULL: none) K is rotated by its position, and q (num_tokens, num_heads, d_head) into q_out, which may be q itself; without one q is
+ * copied.  Two sequences that append into one page in one call must not share its rows.  A token whose page or position is refused
+ * (status) is left out; a value that does not fit a 16-bit cache is stored as its low 16 bits and reported. */
+int32_t zkb_kv_append(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint32_t* k_dev, size_t k_stride, const uint32_t* v_dev, size_t v_stride, uint32_t num_tokens,
+                      const int32_t* block_table_dev, uint32_t num_seqs, uint32_t max_blocks, const int32_t* row_start_dev, const int32_t* start_dev,
+                      const zkb_kv_rotation* rotation, const uint32_t* q_dev, size_t q_stride, uint32_t num_heads, uint32_t* q_out_dev, size_t q_out_stride,
+                      int32_t* status_dev);
+/* One new token per sequence over its first lens[s] cached positions: q (num_seqs, num_heads, d_head), q_stride words between sequences
+ * (0: dense), query head h reads key head h / (num_heads / num_kv_heads).  s_j = q . k_j as a centred integer, divided by 2^score_shift and
+ * rounded half away from zero, must be an input of the exp table (65536 or 256 entries, as for zkb_row_attention_forward);
+ * out[s][h] = (sum_j e_j v_j) / (sum_j e_j), e_j = table(s_j).  A row of length 0 is zero, and so is a row that is refused (status).
+ * workspace: zkb_paged_attention_workspace bytes of the caller's, 256-byte aligned, for this call alone until it has run; NULL: the context's
+ * scratch, which a captured call must not use (ZKB_E_ARG). */
+size_t zkb_paged_attention_workspace(zkb_ctx* ctx, const zkb_kv_cache* cache, uint32_t num_seqs, uint32_t num_heads);
+int32_t zkb_paged_attention(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint32_t* q_dev, size_t q_stride, uint32_t num_heads, const int32_t* block_table_dev,
+                            uint32_t num_seqs, uint32_t max_blocks, const int32_t* lens_dev, const uint32_t* table_out_dev, size_t n_table, uint32_t score_shift,
+                            uint32_t* out_dev, int32_t* status_dev, void* workspace_dev, size_t workspace_bytes);
+/* y[t] = W x[t] + bias + B[a] (A[a] x[t]), a = adapter_of[t]; a token whose entry is outside [0, num_adapters) has no adapter.  x: tokens rows of n
+ * words, x_stride apart; W: m x n row-major; bias (m words) may be NULL; A: (num_adapters, rank, n), B: (num_adapters, m, rank); y: tokens rows of
+ * m words, y_stride apart.  An adapter's scale is part of B.  The workspace as above. */
+size_t zkb_adapter_linear_workspace(zkb_ctx* ctx, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank);
+int32_t zkb_adapter_linear(zkb_ctx* ctx, const uint32_t* x_dev, size_t x_stride, const uint32_t* w_dev, const uint32_t* bias_dev, uint32_t tokens, uint32_t m, uint32_t n,
+                           const uint32_t* a_dev, const uint32_t* b_dev, uint32_t num_adapters, uint32_t rank, const int32_t* adapter_of_dev, uint32_t* y_dev,
+                           size_t y_stride, void* workspace_dev, size_t workspace_bytes);
+
 /* ---- allocation-free weight fold ----
  * No counterpart in the reference: it exists for callers that must not allocate device memory
  * once they are running (a serving loop with a fixed memory plan, a host that forbids cudaMalloc

@@ -7,6 +7,7 @@
 #include "attention.cuh"
 #include "verify_attention.cuh"
 #include "verify_layer.cuh"
+#include "serving.cuh"
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -445,6 +446,7 @@ int32_t zkb_sumcheck_prove(zkb_ctx* c, zkb_transcript* t, int32_t kind, const ui
 #include "abi_weights.cuh"
 #include "abi_attention.cuh"
 #include "abi_pcs_batch.cuh"
+#include "abi_serving.cuh"
 
 // =============================================================================================
 // Allocation-free weight fold
