@@ -177,6 +177,7 @@ int32_t zkb_adapter_linear(zkb_ctx* c, const uint32_t* x_dev, size_t x_stride, c
         a.num_adapters = num_adapters; a.rank = num_adapters ? rank : 0; a.adapter_of = adapter_of_dev; a.y = y_dev;
         ServeWorkspace ws(c, workspace_dev, workspace_bytes, adapter_linear_workspace(c->sm_count, tokens, m, n, num_adapters, rank));
         a.workspace = ws.p;
+        a.gave_up = c->serve_flag();
         int k = 0;
         ZKB_CUDA(adapter_linear_launch(c->stream, c->sm_count, a, &k));
         serve_launched(c, k, __FILE__, __LINE__);

@@ -168,6 +168,15 @@ struct zkb_ctx {
         if (!tr_host) ZKB_CUDA(cudaHostAlloc(&tr_host, sizeof(zkb::TrState), cudaHostAllocDefault));
         return tr_host;
     }
+    // Set by a kernel of the token-by-token operators whose bounded wait ran out; page-locked, so that a synchronised host reads it without a copy.
+    int* serve_gave_up = nullptr;
+    int* serve_flag() {
+        if (!serve_gave_up) {
+            ZKB_CUDA(cudaHostAlloc(&serve_gave_up, 64, cudaHostAllocDefault));
+            *serve_gave_up = 0;
+        }
+        return serve_gave_up;
+    }
     // Second stream for work that does not depend on the transcript (the fold / tree chain of a Basefold
     // opening), joined to `stream` through events; created on first use.
     cudaStream_t side = nullptr;

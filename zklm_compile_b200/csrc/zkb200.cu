@@ -91,6 +91,7 @@ void zkb_ctx_destroy(zkb_ctx* c) {
     if (c->side) cudaStreamDestroy(c->side);
     if (c->stage) cudaFreeHost(c->stage);
     if (c->tr_host) cudaFreeHost(c->tr_host);
+    if (c->serve_gave_up) cudaFreeHost(c->serve_gave_up);
     if (c->lifted) cudaStreamDestroy(c->lifted);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
@@ -103,7 +104,14 @@ void* zkb_ctx_stream(zkb_ctx* c) { return c ? (void*)c->stream : nullptr; }
 
 int32_t zkb_ctx_sync(zkb_ctx* c) {
     if (!c) return ZKB_E_ARG;
-    ZKB_TRY(c, { c->use(); ZKB_CUDA(cudaStreamSynchronize(c->stream)); });
+    ZKB_TRY(c, {
+        c->use();
+        ZKB_CUDA(cudaStreamSynchronize(c->stream));
+        if (c->serve_gave_up && *(volatile int*)c->serve_gave_up) {
+            *c->serve_gave_up = 0;
+            throw ArgFail{ZKB_E_TIMEOUT, "a wait inside a kernel ran out: results of this context since its last synchronisation are not valid"};
+        }
+    });
 }
 int32_t zkb_timer_start(zkb_ctx* c) {
     if (!c) return ZKB_E_ARG;
