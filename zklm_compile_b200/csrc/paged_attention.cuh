@@ -4,77 +4,514 @@
 //
 // in the field, s_j read as a centred integer and rounded half away from zero.  The table stands in for exp, so no running maximum is
 // needed: both sums are plain sums mod p, and parts of a row join by adding.
+//
+// Both sums of products run on the integer tensor cores (mma.sync, unsigned bytes), with the cache's own bytes as the left operand: a
+// product of field elements is sixteen products of bytes, w x = sum_c 2^(8c) sum_i w_i d_c(i) with d(i) the bytes of 2^(8i) x mod p, a
+// rotation of x's 31 bits (digit_words).  A query head is four columns of the right operand.  For scores the 16 rows of a tile are
+// positions and the depth runs over the bytes of a key; for the output the rows are elements of the head and the depth runs over the bytes
+// of one element at several positions - either way a register of the left operand is a 32-bit word of the cache (two half words of two
+// positions in a 16-bit cache), so nothing is transposed on the way.  16-bit elements are made unsigned by flipping their top bit, and
+// 2^15 (sum of the other operand) is taken off at the end.
+//
+// What bounds it is reading the cache.  Every lane copies with 16-byte cp.async exactly the words that it will feed to the tensor cores
+// itself, so a warp's ring of tiles needs no barrier, and the ring keeps about 100 KB per SM in flight.  The work of a call is one list
+// of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences' lengths are; a row
+// that CTAs share is added up by paged_attention_join_kernel.  Integer sums have no order, so results do not depend on the split.
 #pragma once
 #include "m31.cuh"
 #include "kv_append.cuh"
+#include "adapter_linear.cuh"
 #include "serving.cuh"
 
 namespace zkb {
 
-constexpr int PA_THREADS = 256;
-constexpr u32 PA_MAX_D = 256;
+constexpr u32 PA_FLUSH = 512;                 // blocks after which 32-bit sums move to 64 bits: 512 tiles x 16 positions x 4 x 255^2 < 2^31
 
-// One CTA: one (sequence, head).
-__global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(PagedAttnArgs A) {
-    __shared__ u32 q[PA_MAX_D], e[PA_THREADS];
-    __shared__ u32 out[PA_MAX_D];
-    const u32 seq = blockIdx.x, head = blockIdx.y, d = A.c.d, kvh = head / (A.num_heads / A.c.num_kv_heads);
-    const u32 lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mask = (1u << A.c.page_bits) - 1;
-    const int len = A.lens[seq];
-    u32* to = A.out + ((size_t)seq * A.num_heads + head) * d;
-    for (u32 i = threadIdx.x; i < d; i += PA_THREADS) { q[i] = A.q[seq * A.q_stride + (size_t)head * d + i]; out[i] = 0; }
-    __syncthreads();
-    int bad = len < 0 || (u64)len > ((u64)A.max_blocks << A.c.page_bits) ? SERVE_PAGE : 0;
-    u32 sum = 0;
-    for (int base = 0; !bad && base < len; base += PA_THREADS) {
-        const int n = len - base < PA_THREADS ? len - base : PA_THREADS;
-        int mine = 0;
-        for (int j = warp; j < n; j += PA_THREADS / 32) {
-            const u32 pos = base + j;
-            const int page = A.block_table[(size_t)seq * A.max_blocks + (pos >> A.c.page_bits)];
-            u32 ev = 0;
-            if (page < 0 || (u32)page >= A.c.num_pages) mine = max(mine, (int)SERVE_PAGE);
-            else {
-                const size_t at = (size_t)page * A.c.page_stride + (((size_t)kvh << A.c.page_bits) + (pos & mask)) * d;
-                u64 acc = 0;
-                for (u32 i = lane; i < d; i += 32) {
-                    const int z = A.c.small ? ((const int16_t*)A.c.k)[at + i] : 0;
-                    const u32 kk = A.c.small ? (z < 0 ? (u32)z + ZKB_P : (u32)z) : ((const u32*)A.c.k)[at + i];
-                    acc += mul31(kk, q[i]);
-                }
-                u32 s = red64(acc);
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) s = add31(s, __shfl_xor_sync(0xffffffffu, s, off));
-                long long x = centred32(s), a = x < 0 ? -x : x;
-                if (A.score_shift) a = (a + (1ll << (A.score_shift - 1))) >> A.score_shift;
-                x = x < 0 ? -a : a;
-                const int half = (int)(A.n_table / 2);
-                if (x < -half || x >= half) mine = max(mine, (int)SERVE_SCORE);
-                else ev = A.table[x < 0 ? x + A.n_table : x];
-            }
-            if (lane == 0) e[j] = ev;
-        }
-        bad = __syncthreads_or(mine == SERVE_PAGE) ? SERVE_PAGE : (__syncthreads_or(mine) ? SERVE_SCORE : 0);
-        if (bad) break;
-        for (u32 i = threadIdx.x; i < d; i += PA_THREADS) {
-            u64 acc = out[i];
-            for (int j = 0; j < n; j++) {
-                const u32 pos = base + j;
-                const int page = A.block_table[(size_t)seq * A.max_blocks + (pos >> A.c.page_bits)];
-                const size_t at = (size_t)page * A.c.page_stride + (((size_t)kvh << A.c.page_bits) + (pos & mask)) * d + i;
-                const int z = A.c.small ? ((const int16_t*)A.c.v)[at] : 0;
-                const u32 vv = A.c.small ? (z < 0 ? (u32)z + ZKB_P : (u32)z) : ((const u32*)A.c.v)[at];
-                acc += mul31(e[j], vv);
-            }
-            out[i] = red64(acc);
-        }
-        for (int j = 0; j < n; j++) sum = add31(sum, e[j]);
-        __syncthreads();
+// x^(p - 2) by powers 2^k - 1.
+__device__ __forceinline__ u32 inv31_chain(u32 x) {
+    auto sq = [](u32 v, int n) { for (int i = 0; i < n; i++) v = mul31(v, v); return v; };
+    const u32 t2 = mul31(sq(x, 1), x), t3 = mul31(sq(t2, 1), x), t6 = mul31(sq(t3, 3), t3), t7 = mul31(sq(t6, 1), x), t14 = mul31(sq(t7, 7), t7);
+    const u32 t28 = mul31(sq(t14, 14), t14), t29 = mul31(sq(t28, 1), x);
+    return mul31(sq(t29, 2), x);               // 4 (2^29 - 1) + 1 = 2^31 - 3
+}
+
+__device__ __forceinline__ void mma_u8_16x8x32(int (&c)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async16(u32 dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ uint4 lds16(u32 a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
+// How the kernels are built for a head of up to DP elements and a slice of 2 NT query heads: warps, and half tiles (16 keys or 16 values) in a
+// warp's ring.  192 KB of ring however long a row is.
+template <int DP, bool SMALL>
+struct PaShape {
+    static constexpr int RB = DP * (SMALL ? 2 : 4);
+    static constexpr int WARPS = RB >= 1024 ? 4 : 8;
+    static constexpr int NS = RB >= 512 ? 3 : (RB == 256 ? 6 : 8);
+    static constexpr int HALF = 16 * RB;       // bytes of a half tile
+};
+struct PaWork {                                // see paged_attention_launch
+    u32 slices, slice_heads, ctas;
+    u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
+    u32* desc;                                 // [ctas][2]: 1 + item that begins in this CTA and goes on in the next, number of CTAs it goes on in
+    int fast;                                  // rows are whole 16-byte groups on 16-byte boundaries
+};
+enum : u32 { PA_BAD_PAGE = 1, PA_BAD_SCORE = 2 };
+
+// Blocks of a sequence: 0 for one without positions and one whose length the block table cannot have.
+__device__ __forceinline__ u32 pa_blocks(const PagedAttnArgs& A, u32 seq, u32 block, u32& len) {
+    const int l = A.lens[seq];
+    len = l < 0 || (u64)l > ((u64)A.max_blocks << A.c.page_bits) ? 0u : (u32)l;
+    return (len + block - 1) / block;
+}
+// The stream of blocks that a CTA takes: sequences, in each its (key head, slice) items, in each its blocks.
+struct PaWalk {
+    u32 seq, grp, blk, nb, len, block, grps;
+    u64 left;
+    __device__ __forceinline__ void step(const PagedAttnArgs& A, u32 n) {
+        left -= n;
+        blk += n;
+        if (blk < nb || !left) return;
+        blk = 0;
+        if (++grp < grps) return;
+        grp = 0;
+        do nb = pa_blocks(A, ++seq, block, len);
+        while (nb == 0);                       // left > 0: there is one
     }
-    if (!bad && len > 0 && sum == 0) bad = SERVE_ZERO_SUM;
-    if (bad && threadIdx.x == 0) atomicMax(A.status + seq, bad);
-    const u32 inv = bad ? 0 : inv31(sum);
-    for (u32 i = threadIdx.x; i < d; i += PA_THREADS) to[i] = mul31(out[i], inv);
+};
+
+// One output row (or its part) in shared memory to where it belongs.
+__device__ __forceinline__ void pa_finish(const PagedAttnArgs& A, u32 seq, u32 head, u32 e, u32 acc, u32 inv, u32 correction) {
+    A.out[((size_t)seq * A.num_heads + head) * A.c.d + e] = mul31(sub31(acc, correction), inv);
+}
+
+template <int DP, bool SMALL, int NT>
+__global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_attention_kernel(PagedAttnArgs A, PaWork P) {
+    using S = PaShape<DP, SMALL>;
+    constexpr int WARPS = S::WARPS, NS = S::NS, RB = S::RB, J = RB / 64, VJ = RB / 128, MT = DP / 16, HEADS = 2 * NT, THREADS = WARPS * 32;
+    constexpr u32 BLOCK = WARPS * 16;
+    extern __shared__ __align__(128) unsigned char pa_smem[];
+    uint4* qd = reinterpret_cast<uint4*>(pa_smem + WARPS * NS * S::HALF);          // [J][NT][32]
+    u32* acc_lo = reinterpret_cast<u32*>(qd + J * NT * 32);                        // [HEADS][DP]
+    u32* acc_hi = acc_lo + HEADS * DP;
+    __shared__ u32 corr[HEADS], inv[HEADS], flags[HEADS], es_lo[HEADS], es_hi[HEADS], scan[32];
+    __shared__ u32 start_seq;
+    __shared__ u64 start_total;
+    const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+    const u32 grps = A.c.num_kv_heads * P.slices, hpg = A.num_heads / A.c.num_kv_heads, d = A.c.d;
+    pdl_launch_dependents();
+
+    // ---- this CTA's share of the blocks ---------------------------------------------------------
+    u64 total = 0;
+    for (u32 s = tid; s < A.num_seqs; s += THREADS) { u32 len; total += pa_blocks(A, s, BLOCK, len); }
+    {   // sum over the CTA
+        __shared__ u64 part[WARPS];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (lane == 0) part[warp] = total;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) total += part[w];
+        total *= grps;
+    }
+    const u64 per = (total + P.ctas - 1) / P.ctas, from = per * blockIdx.x, to = from + per < total ? from + per : total;
+    // rows without positions are zero
+    for (u32 s = blockIdx.x; s < A.num_seqs; s += P.ctas) {
+        u32 len;
+        if (pa_blocks(A, s, BLOCK, len)) continue;
+        for (u32 i = tid; i < A.num_heads * d; i += THREADS) A.out[(size_t)s * A.num_heads * d + i] = 0;
+        if (tid == 0 && A.lens[s] != 0) atomicMax(A.status + s, (int)SERVE_PAGE);
+    }
+    if (tid == 0) { P.desc[2 * blockIdx.x] = 0; P.desc[2 * blockIdx.x + 1] = 0; }
+    if (from >= to) return;
+    {   // the sequence in which block `from` lies
+        u64 before = 0;
+        for (u32 base = 0;; base += THREADS) {
+            u32 len, nb = base + tid < A.num_seqs ? pa_blocks(A, base + tid, BLOCK, len) : 0u, x = nb;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const u32 y = __shfl_up_sync(0xffffffffu, x, o); if ((int)lane >= o) x += y; }
+            if (lane == 31) scan[warp] = x;
+            __syncthreads();
+            u64 w = 0, all = 0;
+#pragma unroll
+            for (int i = 0; i < WARPS; i++) { if (i < (int)warp) w += scan[i]; all += scan[i]; }
+            const u64 end = (before + w + x) * grps, begin = end - (u64)nb * grps;
+            if (nb && begin <= from && from < end) { start_seq = base + tid; start_total = from - begin; }
+            before += all;
+            __syncthreads();
+            if (before * grps > from) break;
+        }
+    }
+    PaWalk cw{};
+    cw.seq = start_seq;
+    cw.block = BLOCK;
+    cw.grps = grps;
+    cw.left = to - from;
+    cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
+    cw.grp = (u32)(start_total / cw.nb);
+    cw.blk = (u32)(start_total - (u64)cw.grp * cw.nb);
+    PaWalk lw = cw;                            // the copies run ahead of the computation
+
+    // ---- copies -------------------------------------------------------------------------------------
+    const u32 ring = smem_addr(pa_smem) + warp * NS * S::HALF;
+    const u32 mask = (1u << A.c.page_bits) - 1;
+    u32 bad_pages = 0, loaded = 0;             // bit k: the tile k tiles behind the last one that was copied has a bad page
+    int page_next = 0;
+    u32 half_in = 0;                           // half tile that is copied next: its slot is half_in % NS
+    u64 off = 0;                               // lanes 0 .. 15: element offset of their position of the tile, ~0: nothing there
+    auto fetch_page = [&](const PaWalk& w) {
+        const u32 pos = w.blk * BLOCK + warp * 16 + (lane & 15);
+        page_next = w.left && pos < w.len ? A.block_table[(size_t)w.seq * A.max_blocks + (pos >> A.c.page_bits)] : 0;
+    };
+    u32 slot_in = 0;
+    auto load_half = [&](bool is_v) {
+        if (!is_v && lw.left) {
+            const u32 pos = lw.blk * BLOCK + warp * 16 + (lane & 15);
+            const bool there = pos < lw.len, fine = page_next >= 0 && (u32)page_next < A.c.num_pages;
+            off = there && fine ? (u64)page_next * A.c.page_stride + (((u64)(lw.grp / P.slices) << A.c.page_bits) + (pos & mask)) * d : ~0ull;
+            bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
+            loaded++;
+        }
+        if (lw.left) {
+            const u32 dst = ring + slot_in * S::HALF + lane * 16;
+            const char* base = (const char*)(is_v ? A.c.v : A.c.k);
+            constexpr int E = SMALL ? 2 : 4;
+            const u32 row_bytes = d * E;
+            u64 o[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) o[r] = __shfl_sync(0xffffffffu, off, is_v ? q4 + 4 * r : (r < 2 ? g + 8 * r : 0));
+            auto put = [&](int idx, u64 at, u32 byte) {
+                if (at == ~0ull || byte >= row_bytes) return;
+                const char* src = base + at * E + byte;
+                if (P.fast) { cp_async16(dst + idx * 512, src); return; }
+                u32 w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (u32 i = 0; i < 16 / E; i++)
+                    if (byte + i * E < row_bytes) {
+                        if (SMALL) w[i >> 1] |= (u32) * (const uint16_t*)(src + 2 * i) << (16 * (i & 1));
+                        else w[i & 3] = *(const u32*)(src + 4 * i);
+                    }
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + idx * 512), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            };
+            if (is_v) {
+#pragma unroll
+                for (int j = 0; j < VJ; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) put(4 * j + r, o[r], (8 * j + g) * 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) put(2 * j + r, o[r], (4 * j + q4) * 16);
+            }
+            if (is_v) { lw.step(A, 1); fetch_page(lw); }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
+        half_in++;
+    };
+    fetch_page(lw);
+#pragma unroll
+    for (int h = 0; h < NS - 1; h++) load_half(h & 1);
+
+    // ---- the stretches of items ---------------------------------------------------------------------
+    u32 slot_out = 0, computed = 0;
+    while (cw.left) {
+        const u32 seq = cw.seq, kvh = cw.grp / P.slices, head0 = kvh * hpg + (cw.grp - kvh * P.slices) * P.slice_heads;
+        const u32 rest = hpg - (cw.grp - kvh * P.slices) * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
+        const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? (u32)cw.left : nb - first;
+        const u32 item = seq * grps + cw.grp;
+        __syncthreads();                        // the row before is done with these arrays
+        for (u32 i = tid; i < J * NT * 32; i += THREADS) {
+            // 16 bytes of the right operand of a lane: steps 2j, 2j + 1 of a tile of 8 columns
+            const u32 j = i / (NT * 32), nt = i / 32 % NT, n = i % 32 / 4, qq = i & 3, head = 2 * nt + (n >> 2), c = n & 3;
+            u32 w[4];
+#pragma unroll
+            for (u32 k = 0; k < 4; k++) {
+                const u32 word = 16 * j + 4 * qq + k;
+                const u32* qrow = A.q + seq * A.q_stride + (size_t)(head0 + head) * d;
+                u32 dw[4] = {0, 0, 0, 0};
+                if (SMALL) {
+                    u32 da[4], db[4];
+                    digit_words(head < heads && 2 * word < d ? qrow[2 * word] : 0u, da);
+                    digit_words(head < heads && 2 * word + 1 < d ? qrow[2 * word + 1] : 0u, db);
+                    w[k] = __byte_perm(c == 0 ? da[0] : c == 1 ? da[1] : c == 2 ? da[2] : da[3], c == 0 ? db[0] : c == 1 ? db[1] : c == 2 ? db[2] : db[3], 0x5410);
+                } else {
+                    digit_words(head < heads && word < d ? qrow[word] : 0u, dw);
+                    w[k] = c == 0 ? dw[0] : c == 1 ? dw[1] : c == 2 ? dw[2] : dw[3];
+                }
+            }
+            qd[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        for (u32 i = tid; i < 2 * HEADS * DP; i += THREADS) acc_lo[i] = 0;
+        if (tid < HEADS) { flags[tid] = 0; es_lo[tid] = 0; es_hi[tid] = 0; }
+        if (SMALL)
+            for (u32 h = warp; h < heads; h += WARPS) {
+                u64 s = 0;
+                for (u32 e = lane; e < d; e += 32) s += A.q[seq * A.q_stride + (size_t)(head0 + h) * d + e];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (lane == 0) corr[h] = mul31(red64(s), 32768u);
+            }
+        __syncthreads();
+
+        int acc[MT][NT][4];
+        u64 esum[NT];
+        u32 bad = 0;                            // bit 0: a page, bit 1 + nt: a score of this lane's head
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            esum[n] = 0;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[m][n][i] = 0;
+        }
+        auto flush = [&]() {                    // sums of 32 bits to halves that add up in shared memory
+            const bool odd = q4 & 1;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    int(&c)[4] = acc[m][n];
+                    const u32 sh = odd ? 16 : 0;
+                    const u32 r0 = red64(((u64)(u32)c[0] + ((u64)(u32)c[1] << 8)) << sh), r1 = red64(((u64)(u32)c[2] + ((u64)(u32)c[3] << 8)) << sh);
+                    const u32 v = add31(odd ? r1 : r0, __shfl_xor_sync(0xffffffffu, odd ? r0 : r1, 1));
+                    // rows of the tile are elements (see the left operand below)
+                    const u32 e = SMALL ? 8 * (8 * (m >> 2) + g) + 2 * (m & 3) + odd : 4 * (8 * (m >> 1) + g) + 2 * (m & 1) + odd;
+                    const u32 at = (2 * n + (q4 >> 1)) * DP + e;
+                    atomicAdd(acc_lo + at, v & 0xffffu);
+                    atomicAdd(acc_hi + at, v >> 16);
+                    c[0] = c[1] = c[2] = c[3] = 0;
+                }
+        };
+        for (u32 b = 0; b < count; b++) {
+            const u32 pos0 = (first + b) * BLOCK + warp * 16;
+            // keys
+            asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+            const u32 kslot = ring + slot_out * S::HALF;
+            if (pos0 < len) {
+                if ((bad_pages >> (loaded - 1 - computed)) & 1) bad |= 1;
+                int sc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0;
+#pragma unroll
+                for (int j = 0; j < J; j++) {
+                    uint4 a = lds16(kslot + (2 * j) * 512 + lane * 16), c = lds16(kslot + (2 * j + 1) * 512 + lane * 16);
+                    if (SMALL) {
+                        a.x ^= 0x80008000u; a.y ^= 0x80008000u; a.z ^= 0x80008000u; a.w ^= 0x80008000u;
+                        c.x ^= 0x80008000u; c.y ^= 0x80008000u; c.z ^= 0x80008000u; c.w ^= 0x80008000u;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint4 bq = qd[(j * NT + n) * 32 + lane];
+                        mma_u8_16x8x32(sc[n], a.x, c.x, a.y, c.y, bq.x, bq.y);
+                        mma_u8_16x8x32(sc[n], a.z, c.z, a.w, c.w, bq.z, bq.w);
+                    }
+                }
+                // one score a lane and tile of columns: position g (+ 8 for odd lanes), head 2n + (q4 >> 1)
+                const bool odd = q4 & 1;
+                const u32 row = g + (odd ? 8 : 0), pos = pos0 + row;
+                u32 ev[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const u32 sh = odd ? 16 : 0;
+                    const u32 r0 = red64(((u64)(u32)sc[n][0] + ((u64)(u32)sc[n][1] << 8)) << sh), r1 = red64(((u64)(u32)sc[n][2] + ((u64)(u32)sc[n][3] << 8)) << sh);
+                    u32 s = add31(odd ? r1 : r0, __shfl_xor_sync(0xffffffffu, odd ? r0 : r1, 1));
+                    const u32 head = 2 * n + (q4 >> 1);
+                    if (SMALL) s = sub31(s, head < heads ? corr[head] : 0u);
+                    int x = centred32(s);
+                    const u32 m = ((u32)(x < 0 ? -x : x) + ((1u << A.score_shift) >> 1)) >> A.score_shift;
+                    x = x < 0 ? -(int)m : (int)m;
+                    const int half = (int)(A.n_table / 2);
+                    const bool in = x >= -half && x < half, seen = pos < len && head < heads;
+                    ev[n] = 0;
+                    if (seen && in) ev[n] = __ldg(A.table + (x < 0 ? x + (int)A.n_table : x));
+                    if (seen && !in) bad |= 2u << n;
+                }
+                __syncwarp();                    // every lane has its keys in registers: their slot now takes the weights' digits
+                u32* ed = reinterpret_cast<u32*>(pa_smem + (kslot - smem_addr(pa_smem)));
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    u32 dw[4];
+                    digit_words(ev[n], dw);
+                    esum[n] += ev[n];
+                    const u32 col = (q4 >> 1) * 4;
+                    if (SMALL) {                 // [NT][8 slots of depth][8 columns][2 positions]
+                        uint16_t* to = reinterpret_cast<uint16_t*>(ed) + ((n * 8 + (row & 3) + 4 * (row >> 3)) * 8 + col) * 2 + ((row >> 2) & 1);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) to[2 * c] = (uint16_t)dw[c];
+                    } else {                     // [NT][16 positions][8 columns]
+                        *reinterpret_cast<uint4*>(ed + (n * 16 + row) * 8 + col) = make_uint4(dw[0], dw[1], dw[2], dw[3]);
+                    }
+                }
+                __syncwarp();
+            }
+            load_half((NS - 1) & 1);
+            slot_out = slot_out + 1 == NS ? 0 : slot_out + 1;
+            // values
+            asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
+            if (pos0 < len) {
+                const u32 vslot = ring + slot_out * S::HALF;
+                const u32* ed = reinterpret_cast<const u32*>(pa_smem + (kslot - smem_addr(pa_smem)));
+                constexpr int KS = SMALL ? 1 : 2;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    u32 b0[NT], b1[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const u32* e8 = ed + (SMALL ? n * 64 : (n * 16 + 8 * ks) * 8);
+                        b0[n] = e8[q4 * 8 + g];
+                        b1[n] = e8[(q4 + 4) * 8 + g];
+                    }
+#pragma unroll
+                    for (int j = 0; j < VJ; j++) {
+                        if (SMALL) {
+                            uint4 v[4];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) v[r] = lds16(vslot + (4 * j + r) * 512 + lane * 16);
+                            const u32* p0 = reinterpret_cast<const u32*>(&v[0]);
+                            const u32* p1 = reinterpret_cast<const u32*>(&v[1]);
+                            const u32* p2 = reinterpret_cast<const u32*>(&v[2]);
+                            const u32* p3 = reinterpret_cast<const u32*>(&v[3]);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const u32 a0 = __byte_perm(p0[i], p1[i], 0x5410) ^ 0x80008000u, a1 = __byte_perm(p0[i], p1[i], 0x7632) ^ 0x80008000u;
+                                const u32 a2 = __byte_perm(p2[i], p3[i], 0x5410) ^ 0x80008000u, a3 = __byte_perm(p2[i], p3[i], 0x7632) ^ 0x80008000u;
+#pragma unroll
+                                for (int n = 0; n < NT; n++) mma_u8_16x8x32(acc[4 * j + i][n], a0, a1, a2, a3, b0[n], b1[n]);
+                            }
+                        } else {
+                            const uint4 v = lds16(vslot + (4 * j + 2 * ks) * 512 + lane * 16), u = lds16(vslot + (4 * j + 2 * ks + 1) * 512 + lane * 16);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                mma_u8_16x8x32(acc[2 * j][n], v.x, v.y, u.x, u.y, b0[n], b1[n]);
+                                mma_u8_16x8x32(acc[2 * j + 1][n], v.z, v.w, u.z, u.w, b0[n], b1[n]);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();                        // the slot of the keys may be written again
+            load_half(NS & 1);
+            slot_out = slot_out + 1 == NS ? 0 : slot_out + 1;
+            computed++;
+            if ((b + 1) % PA_FLUSH == 0) flush();
+        }
+        flush();
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            u32 s = red64(esum[n]);
+            u32 f = (bad & 1 ? PA_BAD_PAGE : 0u) | (bad & (2u << n) ? PA_BAD_SCORE : 0u);
+#pragma unroll
+            for (int o = 1; o < 32; o = o == 1 ? 4 : o * 2) {                       // all lanes but the other head's
+                s = add31(s, __shfl_xor_sync(0xffffffffu, s, o));
+                f |= __shfl_xor_sync(0xffffffffu, f, o);
+            }
+            if (g == 0 && !(q4 & 1)) {
+                const u32 h = 2 * n + (q4 >> 1);
+                atomicAdd(es_lo + h, s & 0xffffu);
+                atomicAdd(es_hi + h, s >> 16);
+                if (f) atomicOr(flags + h, f);
+            }
+        }
+        __syncthreads();
+        const bool begins = first == 0, ends = first + count == nb;
+        if (begins && ends) {
+            if (tid < heads) {
+                const u32 s = red64(es_lo[tid] + ((u64)es_hi[tid] << 16)), f = flags[tid];
+                const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : s == 0 ? SERVE_ZERO_SUM : 0;
+                if (code) atomicMax(A.status + seq, code);
+                inv[tid] = code ? 0u : inv31_chain(s);
+                corr[tid] = SMALL ? mul31(s, 32768u) : 0u;
+            }
+            __syncthreads();
+            for (u32 i = tid; i < heads * DP; i += THREADS) {
+                const u32 h = i / DP, e = i % DP;
+                if (e < d) pa_finish(A, seq, head0 + h, e, red64(acc_lo[i] + ((u64)acc_hi[i] << 16)), inv[h], corr[h]);
+            }
+        } else {
+            u32* slot = P.slots + (size_t)(2 * blockIdx.x + (begins ? 1 : 0)) * HEADS * (DP + 4);
+            for (u32 i = tid; i < heads * DP; i += THREADS) slot[i / DP * (DP + 4) + i % DP] = red64(acc_lo[i] + ((u64)acc_hi[i] << 16));
+            if (tid < heads) {
+                slot[tid * (DP + 4) + DP] = red64(es_lo[tid] + ((u64)es_hi[tid] << 16));
+                slot[tid * (DP + 4) + DP + 1] = flags[tid];
+            }
+            if (begins && tid == 0) {
+                P.desc[2 * blockIdx.x + 1] = (u32)((nb - first - count + per - 1) / per);
+                P.desc[2 * blockIdx.x] = item + 1;
+            }
+        }
+        cw.step(A, count);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// A row that several CTAs share, added up by the CTA of the same number as the one in which it begins; blockIdx.y: a head of the slice.
+template <int DP, bool SMALL, int NT>
+__global__ void __launch_bounds__(DP) paged_attention_join_kernel(PagedAttnArgs A, PaWork P) {
+    constexpr int HEADS = 2 * NT;
+    pdl_wait();
+    const u32 c = blockIdx.x, h = blockIdx.y, item = P.desc[2 * c];
+    if (!item) return;
+    const u32 more = P.desc[2 * c + 1], grps = A.c.num_kv_heads * P.slices, seq = (item - 1) / grps, grp = (item - 1) - seq * grps;
+    const u32 kvh = grp / P.slices, hpg = A.num_heads / A.c.num_kv_heads, in = (grp - kvh * P.slices) * P.slice_heads + h;
+    if (in >= hpg || h >= P.slice_heads) return;
+    const u32* at = P.slots + ((size_t)(2 * c + 1) * HEADS + h) * (DP + 4);
+    const u32 e = threadIdx.x;
+    u64 acc = at[e], es = at[DP];
+    u32 f = at[DP + 1];
+    for (u32 k = 1; k <= more; k++) {
+        const u32* s = P.slots + ((size_t)(2 * (c + k)) * HEADS + h) * (DP + 4);
+        acc += s[e];
+        es += s[DP];
+        f |= s[DP + 1];
+    }
+    const u32 s = red64(es);
+    const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : s == 0 ? SERVE_ZERO_SUM : 0;
+    if (code && e == 0) atomicMax(A.status + seq, code);
+    if (e < A.c.d) pa_finish(A, seq, kvh * hpg + in, e, red64(acc), code ? 0u : inv31_chain(s), SMALL ? mul31(s, 32768u) : 0u);
+}
+
+// ---- launch ---------------------------------------------------------------------------------------------
+struct PaChoice { u32 dp, nt, slices, slice_heads; };
+// 2 nt query heads of a key head share a pass over it: as many as the sums fit into registers with (dp / 16 x nt x 4 of them a lane).
+inline PaChoice pa_choice(u32 d, u32 hpg) {
+    PaChoice c{};
+    c.dp = d <= 64 ? 64 : (d <= 128 ? 128 : 256);
+    const u32 most = c.dp == 256 ? 4 : 8;
+    c.slices = (hpg + most - 1) / most;
+    c.slice_heads = (hpg + c.slices - 1) / c.slices;
+    c.nt = c.slice_heads <= 2 ? 1 : (c.slice_heads <= 4 ? 2 : 4);
+    return c;
+}
+template <int DP, bool SMALL, int NT>
+inline cudaError_t pa_launch(cudaStream_t stream, const PagedAttnArgs& a, PaWork w, int* launches) {
+    using S = PaShape<DP, SMALL>;
+    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)4 * NT * DP * 4;
+    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<DP, SMALL, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    const u64 most = (u64)a.num_seqs * a.c.num_kv_heads * w.slices * ((((u64)a.max_blocks << a.c.page_bits) + S::WARPS * 16 - 1) / (S::WARPS * 16));
+    if (most < w.ctas) w.ctas = (u32)most;
+    paged_attention_kernel<DP, SMALL, NT><<<w.ctas, S::WARPS * 32, smem, stream>>>(a, w);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(w.ctas, w.slice_heads);
+    cfg.blockDim = DP;
+    cfg.stream = stream;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<DP, SMALL, NT>, a, w);
+    *launches += 2;
+    return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace zkb

@@ -13,11 +13,30 @@ cudaError_t kv_append_launch(cudaStream_t stream, int sm_count, const AppendArgs
     return cudaGetLastError();
 }
 
-size_t paged_attention_workspace(int, uint32_t, uint32_t, uint32_t, uint32_t) { return 256; }
+size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs) {
+    if (!num_seqs) return 0;
+    const PaChoice c = pa_choice(d, num_heads / num_kv_heads);
+    return ((size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4) + (size_t)sm_count * 2) * 4;
+}
 cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const PagedAttnArgs& a, int* launches) {
-    paged_attention_kernel<<<dim3(a.num_seqs, a.num_heads), PA_THREADS, 0, stream>>>(a);
-    ++*launches;
-    return cudaGetLastError();
+    const PaChoice c = pa_choice(a.c.d, a.num_heads / a.c.num_kv_heads);
+    const u32 size = a.c.small ? 2 : 4;
+    PaWork w{};
+    w.slices = c.slices;
+    w.slice_heads = c.slice_heads;
+    w.ctas = (u32)sm_count;
+    w.slots = (u32*)a.workspace;
+    w.desc = w.slots + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4);
+    w.fast = a.c.d * size % 16 == 0 && a.c.page_stride * size % 16 == 0 && !((uintptr_t)a.c.k & 15) && !((uintptr_t)a.c.v & 15);
+    const u32 which = c.dp | c.nt << 16 | (a.c.small ? 1u << 24 : 0u);
+    switch (which) {
+#define ZKB_PA(DP, NT)                                                                              \
+    case DP | NT << 16: return pa_launch<DP, false, NT>(stream, a, w, launches);                     \
+    case DP | NT << 16 | 1u << 24: return pa_launch<DP, true, NT>(stream, a, w, launches);
+        ZKB_PA(64, 1) ZKB_PA(64, 2) ZKB_PA(64, 4) ZKB_PA(128, 1) ZKB_PA(128, 2) ZKB_PA(128, 4) ZKB_PA(256, 1) ZKB_PA(256, 2)
+#undef ZKB_PA
+    }
+    return cudaErrorInvalidValue;
 }
 
 // cuTensorMapEncodeTiled, without linking the driver library.
