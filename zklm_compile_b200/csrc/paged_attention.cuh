@@ -18,6 +18,7 @@
 // of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences' lengths are; a row
 // that CTAs share is added up by paged_attention_join_kernel.  Integer sums have no order, so results do not depend on the split.
 #pragma once
+#include <type_traits>
 #include "m31.cuh"
 #include "kv_append.cuh"
 #include "adapter_linear.cuh"
@@ -36,15 +37,25 @@ __device__ __forceinline__ u32 inv31_chain(u32 x) {
 }
 
 __device__ __forceinline__ void mma_u8_16x8x32(int (&c)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void cp_async16(u32 dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ uint4 lds16(u32 a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-    return v;
+// The four columns of a head are digits c of weight 2^(8c); a lane with an even q4 holds digits 0 and 1 of rows g and g + 8, the odd one beside it
+// digits 2 and 3.  Even lanes finish row g, odd ones row g + 8: the value mod p.  2^8 x and 2^16 x mod p are rotations.
+__device__ __forceinline__ u32 pa_pair(int c0, int c1) {                  // sums below 2^31, of weights 1 and 2^8
+    const u32 hi = (u32)c1, r = ((hi << 8) & ZKB_P) + (hi >> 23);
+    const u32 lo = (u32)c0, t = lo + r;                                   // below 2^32
+    return (t & ZKB_P) + (t >> 31);                                       // at most p
+}
+__device__ __forceinline__ u32 pa_value(const int (&c)[4], bool odd) {
+    const u32 t0 = pa_pair(c[0], c[1]), t1 = pa_pair(c[2], c[3]);
+    const u32 mine = odd ? t1 : t0, theirs = __shfl_xor_sync(0xffffffffu, odd ? t0 : t1, 1);
+    const u32 lo = odd ? theirs : mine, hi = odd ? mine : theirs;
+    const u32 s = lo + (((hi << 16) & ZKB_P) + (hi >> 15));               // at most 2p
+    const u32 f = (s & ZKB_P) + (s >> 31);
+    return umin32(f, f - ZKB_P);
 }
 
 // How the kernels are built for a head of up to DP elements and a slice of 2 NT query heads: warps, and half tiles (16 keys or 16 values) in a
@@ -100,7 +111,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     uint4* qd = reinterpret_cast<uint4*>(pa_smem + WARPS * NS * S::HALF);          // [J][NT][32]
     u32* acc_lo = reinterpret_cast<u32*>(qd + J * NT * 32);                        // [HEADS][DP]
     u32* acc_hi = acc_lo + HEADS * DP;
-    __shared__ u32 corr[HEADS], inv[HEADS], flags[HEADS], es_lo[HEADS], es_hi[HEADS], scan[32];
+    __shared__ u32 off_q[HEADS][2], corr[HEADS], inv[HEADS], flags[HEADS], es_lo[HEADS], es_hi[HEADS], scan[32];
     __shared__ u32 start_seq;
     __shared__ u64 start_total;
     const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
@@ -160,62 +171,64 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     PaWalk lw = cw;                            // the copies run ahead of the computation
 
     // ---- copies -------------------------------------------------------------------------------------
-    const u32 ring = smem_addr(pa_smem) + warp * NS * S::HALF;
+    const u32 ring_at = warp * NS * S::HALF, ring = smem_addr(pa_smem) + ring_at + lane * 16;
     const u32 mask = (1u << A.c.page_bits) - 1;
+    constexpr u32 E = SMALL ? 2 : 4;
+    const u32 row_bytes = d * E, chunks = (row_bytes + 15) / 16;
+    const u64 page_bytes = A.c.page_stride * E;
+    const int k_copies = (int)((chunks + 3 - q4) / 4), v_copies = (int)((chunks + 7 - g) / 8);      // 16-byte groups of a row that are this lane's
     u32 bad_pages = 0, loaded = 0;             // bit k: the tile k tiles behind the last one that was copied has a bad page
-    int page_next = 0;
-    u32 half_in = 0;                           // half tile that is copied next: its slot is half_in % NS
-    u64 off = 0;                               // lanes 0 .. 15: element offset of their position of the tile, ~0: nothing there
+    int page_next = 0, page = -1;              // lanes 0 .. 15 (and again 16 .. 31): the page of their position in the next tile and in this one, -1: none
     auto fetch_page = [&](const PaWalk& w) {
         const u32 pos = w.blk * BLOCK + warp * 16 + (lane & 15);
         page_next = w.left && pos < w.len ? A.block_table[(size_t)w.seq * A.max_blocks + (pos >> A.c.page_bits)] : 0;
     };
     u32 slot_in = 0;
-    auto load_half = [&](bool is_v) {
-        if (!is_v && lw.left) {
-            const u32 pos = lw.blk * BLOCK + warp * 16 + (lane & 15);
-            const bool there = pos < lw.len, fine = page_next >= 0 && (u32)page_next < A.c.num_pages;
-            off = there && fine ? (u64)page_next * A.c.page_stride + (((u64)(lw.grp / P.slices) << A.c.page_bits) + (pos & mask)) * d : ~0ull;
-            bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
-            loaded++;
+    // A lane's groups of one row: `n` of them, STEP bytes apart, to every second / fourth place of its part of the slot.
+    auto copy_row = [&](u32 dst, const char* src, int n, u32 first_byte, auto count, auto step, auto place) {
+        if (P.fast) {
+#pragma unroll
+            for (int j = 0; j < decltype(count)::value; j++)
+                if (j < n) cp_async16(dst + j * decltype(place)::value * 512, src + j * decltype(step)::value);
+            return;
         }
+        for (int j = 0; j < n; j++) {
+            u32 w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (u32 i = 0; i < 16 / E; i++)
+                if (first_byte + j * decltype(step)::value + i * E < row_bytes) {
+                    const char* at = src + j * decltype(step)::value + i * E;
+                    if (SMALL) w[i >> 1] |= (u32) * (const uint16_t*)at << (16 * (i & 1));
+                    else w[i & 3] = *(const u32*)at;
+                }
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + j * decltype(place)::value * 512), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+    };
+    auto load_half = [&](bool is_v) {
         if (lw.left) {
-            const u32 dst = ring + slot_in * S::HALF + lane * 16;
+            const u32 pos0 = lw.blk * BLOCK + warp * 16;
+            if (!is_v) {
+                const bool there = pos0 + (lane & 15) < lw.len, fine = page_next >= 0 && (u32)page_next < A.c.num_pages;
+                page = there && fine ? page_next : -1;
+                bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
+                loaded++;
+            }
+            const u32 dst = ring + slot_in * S::HALF;
+            const u32 kv_row = (lw.grp / P.slices) << A.c.page_bits;
             const char* base = (const char*)(is_v ? A.c.v : A.c.k);
-            constexpr int E = SMALL ? 2 : 4;
-            const u32 row_bytes = d * E;
-            u64 o[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) o[r] = __shfl_sync(0xffffffffu, off, is_v ? q4 + 4 * r : (r < 2 ? g + 8 * r : 0));
-            auto put = [&](int idx, u64 at, u32 byte) {
-                if (at == ~0ull || byte >= row_bytes) return;
-                const char* src = base + at * E + byte;
-                if (P.fast) { cp_async16(dst + idx * 512, src); return; }
-                u32 w[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (u32 i = 0; i < 16 / E; i++)
-                    if (byte + i * E < row_bytes) {
-                        if (SMALL) w[i >> 1] |= (u32) * (const uint16_t*)(src + 2 * i) << (16 * (i & 1));
-                        else w[i & 3] = *(const u32*)(src + 4 * i);
-                    }
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + idx * 512), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-            };
-            if (is_v) {
-#pragma unroll
-                for (int j = 0; j < VJ; j++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) put(4 * j + r, o[r], (8 * j + g) * 16);
-            } else {
-#pragma unroll
-                for (int j = 0; j < J; j++)
-#pragma unroll
-                    for (int r = 0; r < 2; r++) put(2 * j + r, o[r], (4 * j + q4) * 16);
+            for (int r = 0; r < (is_v ? 4 : 2); r++) {
+                const u32 row = is_v ? q4 + 4 * r : g + 8 * r, byte = (is_v ? g : q4) * 16;
+                const int pg = __shfl_sync(0xffffffffu, page, row);
+                const char* src = base + (u64)(u32)pg * page_bytes + (u64)(kv_row + ((pos0 + row) & mask)) * row_bytes + byte;
+                const int n = pg < 0 ? 0 : (is_v ? v_copies : k_copies);
+                if (is_v) copy_row(dst + r * 512, src, n, byte, std::integral_constant<int, VJ>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+                else copy_row(dst + r * 512, src, n, byte, std::integral_constant<int, J>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
             }
             if (is_v) { lw.step(A, 1); fetch_page(lw); }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
-        half_in++;
     };
     fetch_page(lw);
 #pragma unroll
@@ -253,12 +266,16 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         for (u32 i = tid; i < 2 * HEADS * DP; i += THREADS) acc_lo[i] = 0;
         if (tid < HEADS) { flags[tid] = 0; es_lo[tid] = 0; es_hi[tid] = 0; }
         if (SMALL)
-            for (u32 h = warp; h < heads; h += WARPS) {
+            for (u32 h = warp; h < HEADS; h += WARPS) {
                 u64 s = 0;
-                for (u32 e = lane; e < d; e += 32) s += A.q[seq * A.q_stride + (size_t)(head0 + h) * d + e];
+                for (u32 e = lane; e < (h < heads ? d : 0u); e += 32) s += A.q[seq * A.q_stride + (size_t)(head0 + h) * d + e];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (lane == 0) corr[h] = mul31(red64(s), 32768u);
+                if (lane == 0) {                    // what flipped top bits add to a score is taken off its digits 0 and 2 at the start
+                    const u32 less = neg31(mul31(red64(s), 32768u));
+                    off_q[h][0] = less & 0xffffu;
+                    off_q[h][1] = less >> 16;
+                }
             }
         __syncthreads();
 
@@ -280,9 +297,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     int(&c)[4] = acc[m][n];
-                    const u32 sh = odd ? 16 : 0;
-                    const u32 r0 = red64(((u64)(u32)c[0] + ((u64)(u32)c[1] << 8)) << sh), r1 = red64(((u64)(u32)c[2] + ((u64)(u32)c[3] << 8)) << sh);
-                    const u32 v = add31(odd ? r1 : r0, __shfl_xor_sync(0xffffffffu, odd ? r0 : r1, 1));
+                    const u32 v = pa_value(c, odd);
                     // rows of the tile are elements (see the left operand below)
                     const u32 e = SMALL ? 8 * (8 * (m >> 2) + g) + 2 * (m & 3) + odd : 4 * (8 * (m >> 1) + g) + 2 * (m & 1) + odd;
                     const u32 at = (2 * n + (q4 >> 1)) * DP + e;
@@ -295,15 +310,19 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             const u32 pos0 = (first + b) * BLOCK + warp * 16;
             // keys
             asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
-            const u32 kslot = ring + slot_out * S::HALF;
+            const u32 kslot = ring_at + slot_out * S::HALF;
             if (pos0 < len) {
                 if ((bad_pages >> (loaded - 1 - computed)) & 1) bad |= 1;
+                const uint4* kt = reinterpret_cast<const uint4*>(pa_smem + kslot) + lane;
                 int sc[NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0;
+                for (int n = 0; n < NT; n++) {
+                    sc[n][1] = sc[n][3] = 0;
+                    sc[n][0] = sc[n][2] = SMALL ? (int)off_q[2 * n + (q4 >> 1)][q4 & 1] : 0;
+                }
 #pragma unroll
                 for (int j = 0; j < J; j++) {
-                    uint4 a = lds16(kslot + (2 * j) * 512 + lane * 16), c = lds16(kslot + (2 * j + 1) * 512 + lane * 16);
+                    uint4 a = kt[2 * j * 32], c = kt[(2 * j + 1) * 32];
                     if (SMALL) {
                         a.x ^= 0x80008000u; a.y ^= 0x80008000u; a.z ^= 0x80008000u; a.w ^= 0x80008000u;
                         c.x ^= 0x80008000u; c.y ^= 0x80008000u; c.z ^= 0x80008000u; c.w ^= 0x80008000u;
@@ -321,11 +340,8 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 u32 ev[NT];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const u32 sh = odd ? 16 : 0;
-                    const u32 r0 = red64(((u64)(u32)sc[n][0] + ((u64)(u32)sc[n][1] << 8)) << sh), r1 = red64(((u64)(u32)sc[n][2] + ((u64)(u32)sc[n][3] << 8)) << sh);
-                    u32 s = add31(odd ? r1 : r0, __shfl_xor_sync(0xffffffffu, odd ? r0 : r1, 1));
+                    const u32 s = pa_value(sc[n], odd);
                     const u32 head = 2 * n + (q4 >> 1);
-                    if (SMALL) s = sub31(s, head < heads ? corr[head] : 0u);
                     int x = centred32(s);
                     const u32 m = ((u32)(x < 0 ? -x : x) + ((1u << A.score_shift) >> 1)) >> A.score_shift;
                     x = x < 0 ? -(int)m : (int)m;
@@ -336,18 +352,22 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                     if (seen && !in) bad |= 2u << n;
                 }
                 __syncwarp();                    // every lane has its keys in registers: their slot now takes the weights' digits
-                u32* ed = reinterpret_cast<u32*>(pa_smem + (kslot - smem_addr(pa_smem)));
+                u32* ed = reinterpret_cast<u32*>(pa_smem + kslot);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    u32 dw[4];
-                    digit_words(ev[n], dw);
                     esum[n] += ev[n];
                     const u32 col = (q4 >> 1) * 4;
-                    if (SMALL) {                 // [NT][8 slots of depth][8 columns][2 positions]
-                        uint16_t* to = reinterpret_cast<uint16_t*>(ed) + ((n * 8 + (row & 3) + 4 * (row >> 3)) * 8 + col) * 2 + ((row >> 2) & 1);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) to[2 * c] = (uint16_t)dw[c];
+                    if (SMALL) {
+                        // [NT][8 slots of depth][8 columns], a word for positions p and p + 4: the lane of p writes columns 0 and 1, that of p + 4 columns 2 and 3
+                        const u32 other = __shfl_xor_sync(0xffffffffu, ev[n], 16);
+                        const bool high = g & 4;
+                        const u32 a = high ? other : ev[n], b = high ? ev[n] : other, sel = high ? 0x7362 : 0x5140;
+                        const u32 x = __byte_perm(a, rotl31(a, 8), sel), y = __byte_perm(b, rotl31(b, 8), sel);
+                        *reinterpret_cast<uint2*>(ed + (n * 8 + (row & 3) + 4 * (row >> 3)) * 8 + col + (high ? 2 : 0)) =
+                            make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
                     } else {                     // [NT][16 positions][8 columns]
+                        u32 dw[4];
+                        digit_words(ev[n], dw);
                         *reinterpret_cast<uint4*>(ed + (n * 16 + row) * 8 + col) = make_uint4(dw[0], dw[1], dw[2], dw[3]);
                     }
                 }
@@ -358,8 +378,8 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             // values
             asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
             if (pos0 < len) {
-                const u32 vslot = ring + slot_out * S::HALF;
-                const u32* ed = reinterpret_cast<const u32*>(pa_smem + (kslot - smem_addr(pa_smem)));
+                const uint4* vt = reinterpret_cast<const uint4*>(pa_smem + ring_at + slot_out * S::HALF) + lane;
+                const u32* ed = reinterpret_cast<const u32*>(pa_smem + kslot);
                 constexpr int KS = SMALL ? 1 : 2;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
@@ -375,7 +395,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                         if (SMALL) {
                             uint4 v[4];
 #pragma unroll
-                            for (int r = 0; r < 4; r++) v[r] = lds16(vslot + (4 * j + r) * 512 + lane * 16);
+                            for (int r = 0; r < 4; r++) v[r] = vt[(4 * j + r) * 32];
                             const u32* p0 = reinterpret_cast<const u32*>(&v[0]);
                             const u32* p1 = reinterpret_cast<const u32*>(&v[1]);
                             const u32* p2 = reinterpret_cast<const u32*>(&v[2]);
@@ -388,7 +408,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                                 for (int n = 0; n < NT; n++) mma_u8_16x8x32(acc[4 * j + i][n], a0, a1, a2, a3, b0[n], b1[n]);
                             }
                         } else {
-                            const uint4 v = lds16(vslot + (4 * j + 2 * ks) * 512 + lane * 16), u = lds16(vslot + (4 * j + 2 * ks + 1) * 512 + lane * 16);
+                            const uint4 v = vt[(4 * j + 2 * ks) * 32], u = vt[(4 * j + 2 * ks + 1) * 32];
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
                                 mma_u8_16x8x32(acc[2 * j][n], v.x, v.y, u.x, u.y, b0[n], b1[n]);
