@@ -22,16 +22,13 @@ constexpr u32 LIN_TOKENS = 64;                 // tokens per tile at most: 256 c
 constexpr u32 LIN_MAX_STAGES = 8;
 constexpr u32 LIN_THREADS = 192;               // warp 0 copies, warp 1 issues, warps 2 to 5 empty the accumulators
 
-__device__ __forceinline__ u32 rotl31(u32 x, u32 s) { return ((x << s) & ZKB_P) | (x >> (31 - s)); }
-// Byte c of the four rotations of x, for c = 0 .. 3: a 4 x 4 transpose of bytes.
+// Byte c of the four rotations of x by 8i, i = 0 .. 3, for c = 0 .. 3.  All of them are bytes of x, of x >> 7, or of x without the top bits of its bytes.
 __device__ __forceinline__ void digit_words(u32 x, u32 (&w)[4]) {
-    const u32 r0 = x, r1 = rotl31(x, 8), r2 = rotl31(x, 16), r3 = rotl31(x, 24);
-    const u32 a = __byte_perm(r0, r1, 0x5140), b = __byte_perm(r2, r3, 0x5140);    // bytes 0, 0', 1, 1'
-    const u32 c = __byte_perm(r0, r1, 0x7362), d = __byte_perm(r2, r3, 0x7362);    // bytes 2, 2', 3, 3'
-    w[0] = __byte_perm(a, b, 0x5410);
-    w[1] = __byte_perm(a, b, 0x7632);
-    w[2] = __byte_perm(c, d, 0x5410);
-    w[3] = __byte_perm(c, d, 0x7632);
+    const u32 t = x >> 7, m = x & 0x007f7f7fu;
+    w[0] = __byte_perm(x, t, 0x4560);
+    w[1] = __byte_perm(x, t, 0x5601);
+    w[2] = __byte_perm(x, t, 0x6012);
+    w[3] = __byte_perm(x, m, 0x4563);
 }
 
 // How a product is cut: `tiles` of LIN_ROWS rows x `tt` tokens, each `steps` deep in `segs` segments.  Tiles' steps lie one behind the other and every CTA takes `per`

@@ -13,10 +13,11 @@
 // positions in a 16-bit cache), so nothing is transposed on the way.  16-bit elements are made unsigned by flipping their top bit, and
 // 2^15 (sum of the other operand) is taken off at the end.
 //
-// What bounds it is reading the cache.  Every lane copies with 16-byte cp.async exactly the words that it will feed to the tensor cores
-// itself, so a warp's ring of tiles needs no barrier, and the ring keeps about 100 KB per SM in flight.  The work of a call is one list
-// of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences' lengths are; a row
-// that CTAs share is added up by paged_attention_join_kernel.  Integer sums have no order, so results do not depend on the split.
+// What bounds it is reading the cache.  Every warp has a ring of half tiles of its own, filled row by row with bulk copies (one instruction
+// for 16 rows, which may lie in different pages) that an mbarrier a slot counts, so warps never wait for one another within a row.  The work
+// of a call is one list of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences'
+// lengths are; a row that CTAs share is added up by paged_attention_join_kernel.  Integer sums have no order, so results do not depend on
+// the split.
 #pragma once
 #include <type_traits>
 #include "m31.cuh"
@@ -41,37 +42,35 @@ __device__ __forceinline__ void mma_u8_16x8x32(int (&c)[4], u32 a0, u32 a1, u32 
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void cp_async16(u32 dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
-// The four columns of a head are digits c of weight 2^(8c); a lane with an even q4 holds digits 0 and 1 of rows g and g + 8, the odd one beside it
-// digits 2 and 3.  Even lanes finish row g, odd ones row g + 8: the value mod p.  2^8 x and 2^16 x mod p are rotations.
-__device__ __forceinline__ u32 pa_pair(int c0, int c1) {                  // sums below 2^31, of weights 1 and 2^8
-    const u32 hi = (u32)c1, r = ((hi << 8) & ZKB_P) + (hi >> 23);
-    const u32 lo = (u32)c0, t = lo + r;                                   // below 2^32
-    return (t & ZKB_P) + (t >> 31);                                       // at most p
-}
-__device__ __forceinline__ u32 pa_value(const int (&c)[4], bool odd) {
-    const u32 t0 = pa_pair(c[0], c[1]), t1 = pa_pair(c[2], c[3]);
-    const u32 mine = odd ? t1 : t0, theirs = __shfl_xor_sync(0xffffffffu, odd ? t0 : t1, 1);
-    const u32 lo = odd ? theirs : mine, hi = odd ? mine : theirs;
-    const u32 s = lo + (((hi << 16) & ZKB_P) + (hi >> 15));               // at most 2p
-    const u32 f = (s & ZKB_P) + (s >> 31);
-    return umin32(f, f - ZKB_P);
+// The four columns of a head are digits c of weight 2^(8c), sums below 2^31; a lane with an even q4 holds digits 0 and 1 of rows g and g + 8, the odd
+// one beside it digits 2 and 3.  Even lanes finish row g, odd ones row g + 8: the value mod p.  `weight`: of the lane's own two digits and of
+// its neighbour's.
+struct PaWeights { u32 own0, own1, other0, other1; };
+__device__ __forceinline__ u32 pa_value(const int (&c)[4], bool odd, const PaWeights& w) {
+    const u32 o0 = __shfl_xor_sync(0xffffffffu, (u32)(odd ? c[0] : c[2]), 1), o1 = __shfl_xor_sync(0xffffffffu, (u32)(odd ? c[1] : c[3]), 1);
+    const u64 v = (u64)(u32)(odd ? c[2] : c[0]) * w.own0 + (u64)(u32)(odd ? c[3] : c[1]) * w.own1 + (u64)o0 * w.other0 + (u64)o1 * w.other1;   // below 2^56
+    const u32 s = ((u32)v & ZKB_P) + (u32)(v >> 31);                                  // below 2^31 + 2^25
+    return umin32(s, s - ZKB_P);
 }
 
-// How the kernels are built for a head of up to DP elements and a slice of 2 NT query heads: warps, and half tiles (16 keys or 16 values) in a
-// warp's ring.  192 KB of ring however long a row is.
+// How the kernels are built for a head of up to DP elements: warps, half tiles (16 keys or 16 values) in a warp's ring, and the distance of rows in
+// shared memory - 64 bytes over a multiple of 128 for keys, which lanes read as two rows by 64 bytes a phase, 32 over for values, read as four
+// rows by 32 bytes - so that no two lanes of a phase meet in a bank.
 template <int DP, bool SMALL>
 struct PaShape {
     static constexpr int RB = DP * (SMALL ? 2 : 4);
-    static constexpr int WARPS = RB >= 1024 ? 4 : 8;
-    static constexpr int NS = RB >= 512 ? 3 : (RB == 256 ? 6 : 8);
-    static constexpr int HALF = 16 * RB;       // bytes of a half tile
+    static constexpr int WARPS = RB >= 1024 ? 5 : 8;
+    static constexpr int NS = RB >= 512 ? 2 : (RB == 256 ? 4 : 6);
+    static constexpr int KP = RB + 64, VP = RB + 32;
+    static constexpr int HALF = 16 * KP;       // bytes of a slot
+    static constexpr int ED = SMALL ? 256 : 512;   // bytes of a tile's weights, as digits, per tile of columns
 };
 struct PaWork {                                // see paged_attention_launch
     u32 slices, slice_heads, ctas;
     u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
     u32* desc;                                 // [ctas][2]: 1 + item that begins in this CTA and goes on in the next, number of CTAs it goes on in
     int fast;                                  // rows are whole 16-byte groups on 16-byte boundaries
+    int* gave_up;
 };
 enum : u32 { PA_BAD_PAGE = 1, PA_BAD_SCORE = 2 };
 
@@ -111,11 +110,15 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     uint4* qd = reinterpret_cast<uint4*>(pa_smem + WARPS * NS * S::HALF);          // [J][NT][32]
     u32* acc_lo = reinterpret_cast<u32*>(qd + J * NT * 32);                        // [HEADS][DP]
     u32* acc_hi = acc_lo + HEADS * DP;
+    unsigned char* digits = reinterpret_cast<unsigned char*>(acc_hi + HEADS * DP); // [WARPS][NT][ED]
+    __shared__ __align__(8) u64 bars[WARPS * NS];
+    __shared__ volatile int gave_up;
     __shared__ u32 off_q[HEADS][2], corr[HEADS], inv[HEADS], flags[HEADS], es_lo[HEADS], es_hi[HEADS], scan[32];
     __shared__ u32 start_seq;
     __shared__ u64 start_total;
     const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
     const u32 grps = A.c.num_kv_heads * P.slices, hpg = A.num_heads / A.c.num_kv_heads, d = A.c.d;
+    if (tid == 0) gave_up = 0;
     pdl_launch_dependents();
 
     // ---- this CTA's share of the blocks ---------------------------------------------------------
@@ -171,71 +174,67 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     PaWalk lw = cw;                            // the copies run ahead of the computation
 
     // ---- copies -------------------------------------------------------------------------------------
-    const u32 ring_at = warp * NS * S::HALF, ring = smem_addr(pa_smem) + ring_at + lane * 16;
+    const u32 ring_at = warp * NS * S::HALF, ring = smem_addr(pa_smem) + ring_at, bar0 = smem_addr(bars + warp * NS);
     const u32 mask = (1u << A.c.page_bits) - 1;
     constexpr u32 E = SMALL ? 2 : 4;
-    const u32 row_bytes = d * E, chunks = (row_bytes + 15) / 16;
+    const u32 row_bytes = d * E;
     const u64 page_bytes = A.c.page_stride * E;
-    const int k_copies = (int)((chunks + 3 - q4) / 4), v_copies = (int)((chunks + 7 - g) / 8);      // 16-byte groups of a row that are this lane's
+    if (lane == 0) {
+        for (int i = 0; i < NS; i++) mbar_init(bar0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    __syncwarp();
     u32 bad_pages = 0, loaded = 0;             // bit k: the tile k tiles behind the last one that was copied has a bad page
-    int page_next = 0, page = -1;              // lanes 0 .. 15 (and again 16 .. 31): the page of their position in the next tile and in this one, -1: none
+    int page_next = 0, page = -1;              // lanes 0 .. 15: the page of their position in the next tile and in this one, -1: none
     auto fetch_page = [&](const PaWalk& w) {
-        const u32 pos = w.blk * BLOCK + warp * 16 + (lane & 15);
-        page_next = w.left && pos < w.len ? A.block_table[(size_t)w.seq * A.max_blocks + (pos >> A.c.page_bits)] : 0;
+        const u32 pos = w.blk * BLOCK + warp * 16 + lane;
+        page_next = lane < 16 && w.left && pos < w.len ? A.block_table[(size_t)w.seq * A.max_blocks + (pos >> A.c.page_bits)] : 0;
     };
     u32 slot_in = 0;
-    // A lane's groups of one row: `n` of them, STEP bytes apart, to every second / fourth place of its part of the slot.
-    auto copy_row = [&](u32 dst, const char* src, int n, u32 first_byte, auto count, auto step, auto place) {
+    auto load_half = [&](bool is_v) {          // the next half tile into the next slot, a row by each of the lanes 0 .. 15
+        if (!lw.left) return;
+        const u32 pos = lw.blk * BLOCK + warp * 16 + lane;
+        if (!is_v) {
+            const bool there = lane < 16 && pos < lw.len, fine = page_next >= 0 && (u32)page_next < A.c.num_pages;
+            page = there && fine ? page_next : -1;
+            bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
+            loaded++;
+        }
+        const u32 bar = bar0 + 8 * slot_in, dst = ring + slot_in * S::HALF;
+        const char* src = (const char*)(is_v ? A.c.v : A.c.k) + (u64)(u32)page * page_bytes + (u64)(((lw.grp / P.slices) << A.c.page_bits) + (pos & mask)) * row_bytes;
+        const u32 rows = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (P.fast) {
-#pragma unroll
-            for (int j = 0; j < decltype(count)::value; j++)
-                if (j < n) cp_async16(dst + j * decltype(place)::value * 512, src + j * decltype(step)::value);
-            return;
-        }
-        for (int j = 0; j < n; j++) {
-            u32 w[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (u32 i = 0; i < 16 / E; i++)
-                if (first_byte + j * decltype(step)::value + i * E < row_bytes) {
-                    const char* at = src + j * decltype(step)::value + i * E;
-                    if (SMALL) w[i >> 1] |= (u32) * (const uint16_t*)at << (16 * (i & 1));
-                    else w[i & 3] = *(const u32*)at;
+            if (lane == 0) mbar_expect(bar, rows * row_bytes);
+            if (page >= 0) bulk_load(dst + lane * (is_v ? S::VP : S::KP), src, row_bytes, bar);
+        } else {
+            for (int r = 0; r < 16; r++) {
+                const char* from_row = (const char*)__shfl_sync(0xffffffffu, (u64)src, r);
+                if (__shfl_sync(0xffffffffu, page, r) < 0) continue;
+                unsigned char* to_row = pa_smem + ring_at + slot_in * S::HALF + r * (is_v ? S::VP : S::KP);
+                for (u32 i = lane; i < d; i += 32) {
+                    if (SMALL) reinterpret_cast<uint16_t*>(to_row)[i] = reinterpret_cast<const uint16_t*>(from_row)[i];
+                    else reinterpret_cast<u32*>(to_row)[i] = reinterpret_cast<const u32*>(from_row)[i];
                 }
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + j * decltype(place)::value * 512), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-        }
-    };
-    auto load_half = [&](bool is_v) {
-        if (lw.left) {
-            const u32 pos0 = lw.blk * BLOCK + warp * 16;
-            if (!is_v) {
-                const bool there = pos0 + (lane & 15) < lw.len, fine = page_next >= 0 && (u32)page_next < A.c.num_pages;
-                page = there && fine ? page_next : -1;
-                bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
-                loaded++;
             }
-            const u32 dst = ring + slot_in * S::HALF;
-            const u32 kv_row = (lw.grp / P.slices) << A.c.page_bits;
-            const char* base = (const char*)(is_v ? A.c.v : A.c.k);
-#pragma unroll
-            for (int r = 0; r < (is_v ? 4 : 2); r++) {
-                const u32 row = is_v ? q4 + 4 * r : g + 8 * r, byte = (is_v ? g : q4) * 16;
-                const int pg = __shfl_sync(0xffffffffu, page, row);
-                const char* src = base + (u64)(u32)pg * page_bytes + (u64)(kv_row + ((pos0 + row) & mask)) * row_bytes + byte;
-                const int n = pg < 0 ? 0 : (is_v ? v_copies : k_copies);
-                if (is_v) copy_row(dst + r * 512, src, n, byte, std::integral_constant<int, VJ>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
-                else copy_row(dst + r * 512, src, n, byte, std::integral_constant<int, J>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-            }
-            if (is_v) { lw.step(A, 1); fetch_page(lw); }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (is_v) { lw.step(A, 1); fetch_page(lw); }
         slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
     };
     fetch_page(lw);
 #pragma unroll
-    for (int h = 0; h < NS - 1; h++) load_half(h & 1);
+    for (int h = 0; h < NS; h++) load_half(h & 1);
+
+    const bool odd = q4 & 1;
+    const PaWeights weights = odd ? PaWeights{1u << 16, 1u << 24, 1u, 1u << 8} : PaWeights{1u, 1u << 8, 1u << 16, 1u << 24};
+    u32 slot_out = 0, phase = 0;
+    auto wait_half = [&] { mbar_wait(bar0 + 8 * slot_out, phase, &gave_up); };
+    auto next_slot = [&] { if (++slot_out == NS) { slot_out = 0; phase ^= 1; } };
 
     // ---- the stretches of items ---------------------------------------------------------------------
-    u32 slot_out = 0, computed = 0;
+    u32 computed = 0;
     while (cw.left) {
         const u32 seq = cw.seq, kvh = cw.grp / P.slices, head0 = kvh * hpg + (cw.grp - kvh * P.slices) * P.slice_heads;
         const u32 rest = hpg - (cw.grp - kvh * P.slices) * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
@@ -291,13 +290,12 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 for (int i = 0; i < 4; i++) acc[m][n][i] = 0;
         }
         auto flush = [&]() {                    // sums of 32 bits to halves that add up in shared memory
-            const bool odd = q4 & 1;
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     int(&c)[4] = acc[m][n];
-                    const u32 v = pa_value(c, odd);
+                    const u32 v = pa_value(c, odd, weights);
                     // rows of the tile are elements (see the left operand below)
                     const u32 e = SMALL ? 8 * (8 * (m >> 2) + g) + 2 * (m & 3) + odd : 4 * (8 * (m >> 1) + g) + 2 * (m & 1) + odd;
                     const u32 at = (2 * n + (q4 >> 1)) * DP + e;
@@ -306,23 +304,25 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                     c[0] = c[1] = c[2] = c[3] = 0;
                 }
         };
+        u32* ed = reinterpret_cast<u32*>(digits + warp * NT * S::ED);
+        const u32 round_up = (1u << A.score_shift) >> 1;
         for (u32 b = 0; b < count; b++) {
             const u32 pos0 = (first + b) * BLOCK + warp * 16;
+            const bool active = pos0 < len;
             // keys
-            asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
-            const u32 kslot = ring_at + slot_out * S::HALF;
-            if (pos0 < len) {
+            wait_half();
+            int sc[NT][4];
+            if (active) {
                 if ((bad_pages >> (loaded - 1 - computed)) & 1) bad |= 1;
-                const uint4* kt = reinterpret_cast<const uint4*>(pa_smem + kslot) + lane;
-                int sc[NT][4];
+                const unsigned char* kt = pa_smem + ring_at + slot_out * S::HALF + g * S::KP + q4 * 16;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     sc[n][1] = sc[n][3] = 0;
-                    sc[n][0] = sc[n][2] = SMALL ? (int)off_q[2 * n + (q4 >> 1)][q4 & 1] : 0;
+                    sc[n][0] = sc[n][2] = SMALL ? (int)off_q[2 * n + (q4 >> 1)][odd] : 0;
                 }
 #pragma unroll
                 for (int j = 0; j < J; j++) {
-                    uint4 a = kt[2 * j * 32], c = kt[(2 * j + 1) * 32];
+                    uint4 a = *reinterpret_cast<const uint4*>(kt + j * 64), c = *reinterpret_cast<const uint4*>(kt + 8 * S::KP + j * 64);
                     if (SMALL) {
                         a.x ^= 0x80008000u; a.y ^= 0x80008000u; a.z ^= 0x80008000u; a.w ^= 0x80008000u;
                         c.x ^= 0x80008000u; c.y ^= 0x80008000u; c.z ^= 0x80008000u; c.w ^= 0x80008000u;
@@ -334,36 +334,38 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                         mma_u8_16x8x32(sc[n], a.z, c.z, a.w, c.w, bq.z, bq.w);
                     }
                 }
-                // one score a lane and tile of columns: position g (+ 8 for odd lanes), head 2n + (q4 >> 1)
-                const bool odd = q4 & 1;
-                const u32 row = g + (odd ? 8 : 0), pos = pos0 + row;
+            }
+            __syncwarp();                        // every lane has read its keys
+            load_half(NS & 1);
+            next_slot();
+            if (active) {
+                // one score a lane and tile of columns: position g (+ 8 for odd lanes), head 2n + (q4 >> 1).  Columns of a head behind the last one are zero and
+                // so are their scores; nobody reads what becomes of them.
+                const u32 row = g + (odd ? 8 : 0);
+                const bool seen = pos0 + row < len;
                 u32 ev[NT];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const u32 s = pa_value(sc[n], odd);
-                    const u32 head = 2 * n + (q4 >> 1);
-                    int x = centred32(s);
-                    const u32 m = ((u32)(x < 0 ? -x : x) + ((1u << A.score_shift) >> 1)) >> A.score_shift;
-                    x = x < 0 ? -(int)m : (int)m;
-                    const int half = (int)(A.n_table / 2);
-                    const bool in = x >= -half && x < half, seen = pos < len && head < heads;
-                    ev[n] = 0;
-                    if (seen && in) ev[n] = __ldg(A.table + (x < 0 ? x + (int)A.n_table : x));
+                    const u32 s = pa_value(sc[n], odd, weights), minus = ZKB_P - s;
+                    const bool neg = minus < s;
+                    const u32 m = (umin32(s, minus) + round_up) >> A.score_shift;
+                    const u32 index = neg ? 0u - m : m;
+                    const bool in = index + A.n_table / 2 < A.n_table;
+                    ev[n] = seen && in ? __ldg(A.table + (index & (A.n_table - 1))) : 0u;
                     if (seen && !in) bad |= 2u << n;
                 }
-                __syncwarp();                    // every lane has its keys in registers: their slot now takes the weights' digits
-                u32* ed = reinterpret_cast<u32*>(pa_smem + kslot);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     esum[n] += ev[n];
                     const u32 col = (q4 >> 1) * 4;
                     if (SMALL) {
                         // [NT][8 slots of depth][8 columns], a word for positions p and p + 4: the lane of p writes columns 0 and 1, that of p + 4 columns 2 and 3
+                        // (bytes 0 and 1 of digit_words, c = 0, 1 or 2, 3)
                         const u32 other = __shfl_xor_sync(0xffffffffu, ev[n], 16);
                         const bool high = g & 4;
-                        const u32 a = high ? other : ev[n], b = high ? ev[n] : other, sel = high ? 0x7362 : 0x5140;
-                        const u32 x = __byte_perm(a, rotl31(a, 8), sel), y = __byte_perm(b, rotl31(b, 8), sel);
-                        *reinterpret_cast<uint2*>(ed + (n * 8 + (row & 3) + 4 * (row >> 3)) * 8 + col + (high ? 2 : 0)) =
+                        const u32 a = high ? other : ev[n], b = high ? ev[n] : other, sel = high ? 0x4312 : 0x0140;
+                        const u32 x = __byte_perm(a, (a << (high ? 9 : 0)) >> (high ? 25 : 23), sel), y = __byte_perm(b, (b << (high ? 9 : 0)) >> (high ? 25 : 23), sel);
+                        *reinterpret_cast<uint2*>(ed + ((n * 8 + (row & 3) + 4 * (row >> 3)) * 8 + col + (high ? 2 : 0))) =
                             make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
                     } else {                     // [NT][16 positions][8 columns]
                         u32 dw[4];
@@ -373,13 +375,10 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 }
                 __syncwarp();
             }
-            load_half((NS - 1) & 1);
-            slot_out = slot_out + 1 == NS ? 0 : slot_out + 1;
             // values
-            asm volatile("cp.async.wait_group %0;" ::"n"(NS - 2) : "memory");
-            if (pos0 < len) {
-                const uint4* vt = reinterpret_cast<const uint4*>(pa_smem + ring_at + slot_out * S::HALF) + lane;
-                const u32* ed = reinterpret_cast<const u32*>(pa_smem + kslot);
+            wait_half();
+            if (active) {
+                const unsigned char* vt = pa_smem + ring_at + slot_out * S::HALF + q4 * S::VP + g * 16;
                 constexpr int KS = SMALL ? 1 : 2;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
@@ -393,22 +392,21 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
                     for (int j = 0; j < VJ; j++) {
                         if (SMALL) {
-                            uint4 v[4];
+                            u32 v[4][4];
 #pragma unroll
-                            for (int r = 0; r < 4; r++) v[r] = vt[(4 * j + r) * 32];
-                            const u32* p0 = reinterpret_cast<const u32*>(&v[0]);
-                            const u32* p1 = reinterpret_cast<const u32*>(&v[1]);
-                            const u32* p2 = reinterpret_cast<const u32*>(&v[2]);
-                            const u32* p3 = reinterpret_cast<const u32*>(&v[3]);
+                            for (int r = 0; r < 4; r++) {
+                                const uint4 t = *reinterpret_cast<const uint4*>(vt + r * 4 * S::VP + j * 128);
+                                v[r][0] = t.x; v[r][1] = t.y; v[r][2] = t.z; v[r][3] = t.w;
+                            }
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                const u32 a0 = __byte_perm(p0[i], p1[i], 0x5410) ^ 0x80008000u, a1 = __byte_perm(p0[i], p1[i], 0x7632) ^ 0x80008000u;
-                                const u32 a2 = __byte_perm(p2[i], p3[i], 0x5410) ^ 0x80008000u, a3 = __byte_perm(p2[i], p3[i], 0x7632) ^ 0x80008000u;
+                                const u32 a0 = __byte_perm(v[0][i], v[1][i], 0x5410) ^ 0x80008000u, a1 = __byte_perm(v[0][i], v[1][i], 0x7632) ^ 0x80008000u;
+                                const u32 a2 = __byte_perm(v[2][i], v[3][i], 0x5410) ^ 0x80008000u, a3 = __byte_perm(v[2][i], v[3][i], 0x7632) ^ 0x80008000u;
 #pragma unroll
                                 for (int n = 0; n < NT; n++) mma_u8_16x8x32(acc[4 * j + i][n], a0, a1, a2, a3, b0[n], b1[n]);
                             }
                         } else {
-                            const uint4 v = vt[(4 * j + 2 * ks) * 32], u = vt[(4 * j + 2 * ks + 1) * 32];
+                            const uint4 v = *reinterpret_cast<const uint4*>(vt + 2 * ks * 4 * S::VP + j * 128), u = *reinterpret_cast<const uint4*>(vt + (2 * ks + 1) * 4 * S::VP + j * 128);
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
                                 mma_u8_16x8x32(acc[2 * j][n], v.x, v.y, u.x, u.y, b0[n], b1[n]);
@@ -418,9 +416,9 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                     }
                 }
             }
-            __syncwarp();                        // the slot of the keys may be written again
-            load_half(NS & 1);
-            slot_out = slot_out + 1 == NS ? 0 : slot_out + 1;
+            __syncwarp();                        // every lane has read its values and the digits
+            load_half((NS + 1) & 1);
+            next_slot();
             computed++;
             if ((b + 1) % PA_FLUSH == 0) flush();
         }
@@ -470,7 +468,14 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         }
         cw.step(A, count);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (gave_up) {                              // nothing of this warp may still be in flight when it ends
+        for (u32 h = 0; h < NS; h++) {
+            const u32 last = 2 * loaded - 1 - h, use = last / NS;
+            if (h < 2 * loaded)
+                for (u32 n = 0; n < (1u << 16) && !mbar_try(bar0 + 8 * (last % NS), use & 1); n++) {}
+        }
+        if (lane == 0) *P.gave_up = 1;
+    }
 }
 
 // A row that several CTAs share, added up by the CTA of the same number as the one in which it begins; blockIdx.y: a head of the slice.
@@ -514,7 +519,8 @@ inline PaChoice pa_choice(u32 d, u32 hpg) {
 template <int DP, bool SMALL, int NT>
 inline cudaError_t pa_launch(cudaStream_t stream, const PagedAttnArgs& a, PaWork w, int* launches) {
     using S = PaShape<DP, SMALL>;
-    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)4 * NT * DP * 4;
+    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)4 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED;
+    static_assert(smem <= 226 * 1024, "with the kernel's own arrays below the 227 KB of a CTA");
     cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<DP, SMALL, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const u64 most = (u64)a.num_seqs * a.c.num_kv_heads * w.slices * ((((u64)a.max_blocks << a.c.page_bits) + S::WARPS * 16 - 1) / (S::WARPS * 16));

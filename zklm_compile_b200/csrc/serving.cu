@@ -25,6 +25,7 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
     w.slices = c.slices;
     w.slice_heads = c.slice_heads;
     w.ctas = (u32)sm_count;
+    w.gave_up = a.gave_up;
     w.slots = (u32*)a.workspace;
     w.desc = w.slots + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4);
     w.fast = a.c.d * size % 16 == 0 && a.c.page_stride * size % 16 == 0 && !((uintptr_t)a.c.k & 15) && !((uintptr_t)a.c.v & 15);

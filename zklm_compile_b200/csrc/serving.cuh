@@ -45,6 +45,7 @@ struct PagedAttnArgs {
     uint32_t* out;                                           // [num_seqs][num_heads][d]
     int32_t* status;
     void* workspace;
+    int* gave_up;                                            // set when a wait inside a kernel ran out
 };
 size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs);
 cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const PagedAttnArgs& a, int* launches);
@@ -58,7 +59,7 @@ struct LinearArgs {
     const int32_t* adapter_of;                               // per token; outside [0, num_adapters): none
     uint32_t* y;
     void* workspace;
-    int* gave_up;                                            // set when a wait inside a kernel ran out
+    int* gave_up;                                            // as above
 };
 size_t adapter_linear_workspace(int sm_count, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank);
 cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const LinearArgs& a, int* launches);
