@@ -13,8 +13,9 @@
 // positions in a 16-bit cache), so nothing is transposed on the way.  16-bit elements are made unsigned by flipping their top bit, and
 // 2^15 (sum of the other operand) is taken off at the end.
 //
-// What bounds it is reading the cache.  Every warp has a ring of half tiles of its own, filled row by row with bulk copies (one instruction
-// for 16 rows, which may lie in different pages) that an mbarrier a slot counts, so warps never wait for one another within a row.  The work
+// What bounds it is reading the cache.  Every warp has a ring of half tiles of its own, filled by tensor copies (16 rows by 128 bytes each) that
+// an mbarrier a slot counts, so warps never wait for one another within a row.  (A bulk copy a row instead of a box held the 16-bit cache to
+// 3.4 TB/s.)  The work
 // of a call is one list of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences'
 // lengths are; a row that CTAs share is added up by paged_attention_join_kernel.  Integer sums have no order, so results do not depend on
 // the split.
@@ -53,23 +54,22 @@ __device__ __forceinline__ u32 pa_value(const int (&c)[4], bool odd, const PaWei
     return umin32(s, s - ZKB_P);
 }
 
-// How the kernels are built for a head of up to DP elements: warps, half tiles (16 keys or 16 values) in a warp's ring, and the distance of rows in
-// shared memory - 64 bytes over a multiple of 128 for keys, which lanes read as two rows by 64 bytes a phase, 32 over for values, read as four
-// rows by 32 bytes - so that no two lanes of a phase meet in a bank.
+// How the kernels are built for a head of up to DP elements: warps, and half tiles (16 keys or 16 values) in a warp's ring.  A half tile lies as the
+// tensor copies leave it: columns of 128 bytes, 16 rows of one behind the other, the 16-byte groups of a row swizzled by the row's low bits.
+// Which position becomes which row of an operand is free, and is chosen so that no two lanes of a phase meet in a bank.
 template <int DP, bool SMALL>
 struct PaShape {
     static constexpr int RB = DP * (SMALL ? 2 : 4);
     static constexpr int WARPS = RB >= 1024 ? 5 : 8;
     static constexpr int NS = RB >= 512 ? 2 : (RB == 256 ? 4 : 6);
-    static constexpr int KP = RB + 64, VP = RB + 32;
-    static constexpr int HALF = 16 * KP;       // bytes of a slot
+    static constexpr int HALF = 16 * RB;       // bytes of a slot
     static constexpr int ED = SMALL ? 256 : 512;   // bytes of a tile's weights, as digits, per tile of columns
 };
 struct PaWork {                                // see paged_attention_launch
     u32 slices, slice_heads, ctas;
     u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
     u32* desc;                                 // [ctas][2]: 1 + item that begins in this CTA and goes on in the next, number of CTAs it goes on in
-    int fast;                                  // rows are whole 16-byte groups on 16-byte boundaries
+    int fast;                                  // tensor copies: rows are whole 16-byte groups on 16-byte boundaries, pages have 8 rows or more
     int* gave_up;
 };
 enum : u32 { PA_BAD_PAGE = 1, PA_BAD_SCORE = 2 };
@@ -102,11 +102,13 @@ __device__ __forceinline__ void pa_finish(const PagedAttnArgs& A, u32 seq, u32 h
 }
 
 template <int DP, bool SMALL, int NT>
-__global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_attention_kernel(PagedAttnArgs A, PaWork P) {
+__global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                                                   PagedAttnArgs A, PaWork P) {
     using S = PaShape<DP, SMALL>;
     constexpr int WARPS = S::WARPS, NS = S::NS, RB = S::RB, J = RB / 64, VJ = RB / 128, MT = DP / 16, HEADS = 2 * NT, THREADS = WARPS * 32;
     constexpr u32 BLOCK = WARPS * 16;
-    extern __shared__ __align__(128) unsigned char pa_smem[];
+    extern __shared__ __align__(16) unsigned char pa_raw[];
+    unsigned char* const pa_smem = pa_raw + ((0u - smem_addr(pa_raw)) & 1023u);    // the swizzle goes by addresses
     uint4* qd = reinterpret_cast<uint4*>(pa_smem + WARPS * NS * S::HALF);          // [J][NT][32]
     u32* acc_lo = reinterpret_cast<u32*>(qd + J * NT * 32);                        // [HEADS][DP]
     u32* acc_hi = acc_lo + HEADS * DP;
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         page_next = lane < 16 && w.left && pos < w.len ? A.block_table[(size_t)w.seq * A.max_blocks + (pos >> A.c.page_bits)] : 0;
     };
     u32 slot_in = 0;
-    auto load_half = [&](bool is_v) {          // the next half tile into the next slot, a row by each of the lanes 0 .. 15
+    auto load_half = [&](bool is_v) {          // the next half tile into the next slot
         if (!lw.left) return;
         const u32 pos = lw.blk * BLOCK + warp * 16 + lane;
         if (!is_v) {
@@ -201,20 +203,27 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
             loaded++;
         }
-        const u32 bar = bar0 + 8 * slot_in, dst = ring + slot_in * S::HALF;
-        const char* src = (const char*)(is_v ? A.c.v : A.c.k) + (u64)(u32)page * page_bytes + (u64)(((lw.grp / P.slices) << A.c.page_bits) + (pos & mask)) * row_bytes;
-        const u32 rows = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        const u32 bar = bar0 + 8 * slot_in, y0 = ((lw.grp / P.slices) << A.c.page_bits) + (pos & mask);
         if (P.fast) {
-            if (lane == 0) mbar_expect(bar, rows * row_bytes);
-            if (page >= 0) bulk_load(dst + lane * (is_v ? S::VP : S::KP), src, row_bytes, bar);
+            // boxes of 16 rows (8 where a page has no more) by 128 bytes; the lane of a box's first row has its page
+            const u32 rows = P.fast, at = lane & 15;
+            const bool mine = lane < 16 && page >= 0 && at % rows == 0;
+            const u32 boxes = __popc(__ballot_sync(0xffffffffu, mine));
+            const u32 columns = (row_bytes + 127) / 128, dst = ring + slot_in * S::HALF + at * 128;
+            if (lane == 0) mbar_expect(bar, boxes * columns * rows * 128);
+            if (mine)
+                for (u32 c = 0; c < columns; c++) tensor_load_3d(dst + c * 2048, is_v ? &map_v : &map_k, (int)(c * (128 / E)), (int)y0, page, bar);
         } else {
+            const char* src = (const char*)(is_v ? A.c.v : A.c.k) + (u64)(u32)page * page_bytes + (u64)y0 * row_bytes;
             for (int r = 0; r < 16; r++) {
                 const char* from_row = (const char*)__shfl_sync(0xffffffffu, (u64)src, r);
                 if (__shfl_sync(0xffffffffu, page, r) < 0) continue;
-                unsigned char* to_row = pa_smem + ring_at + slot_in * S::HALF + r * (is_v ? S::VP : S::KP);
+                unsigned char* to = pa_smem + ring_at + slot_in * S::HALF + r * 128;
                 for (u32 i = lane; i < d; i += 32) {
-                    if (SMALL) reinterpret_cast<uint16_t*>(to_row)[i] = reinterpret_cast<const uint16_t*>(from_row)[i];
-                    else reinterpret_cast<u32*>(to_row)[i] = reinterpret_cast<const u32*>(from_row)[i];
+                    const u32 byte = i * E;
+                    unsigned char* w = to + (byte >> 7) * 2048 + ((byte & 127) ^ ((r & 7) << 4));
+                    if (SMALL) *reinterpret_cast<uint16_t*>(w) = reinterpret_cast<const uint16_t*>(from_row)[i];
+                    else *reinterpret_cast<u32*>(w) = reinterpret_cast<const u32*>(from_row)[i];
                 }
             }
             __syncwarp();
@@ -227,6 +236,9 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
     for (int h = 0; h < NS; h++) load_half(h & 1);
 
+    // keys: lane (g, q4) reads rows k_row and k_row + 8, so that a phase has two rows four apart; values: rows 2 q4 and 2 q4 + 1 (and those + 8), two apart
+    const u32 k_row = (g >> 1) + 4 * (g & 1), k_at = k_row * 128 + ((q4 ^ k_row) << 4);
+    const u32 v_at0 = 2 * q4 * 128 + ((g ^ (2 * q4)) << 4), v_at1 = (2 * q4 + 1) * 128 + ((g ^ (2 * q4 + 1)) << 4);
     const bool odd = q4 & 1;
     const PaWeights weights = odd ? PaWeights{1u << 16, 1u << 24, 1u, 1u << 8} : PaWeights{1u, 1u << 8, 1u << 16, 1u << 24};
     u32 slot_out = 0, phase = 0;
@@ -314,7 +326,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             int sc[NT][4];
             if (active) {
                 if ((bad_pages >> (loaded - 1 - computed)) & 1) bad |= 1;
-                const unsigned char* kt = pa_smem + ring_at + slot_out * S::HALF + g * S::KP + q4 * 16;
+                const unsigned char* kt = pa_smem + ring_at + slot_out * S::HALF;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     sc[n][1] = sc[n][3] = 0;
@@ -322,7 +334,8 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 }
 #pragma unroll
                 for (int j = 0; j < J; j++) {
-                    uint4 a = *reinterpret_cast<const uint4*>(kt + j * 64), c = *reinterpret_cast<const uint4*>(kt + 8 * S::KP + j * 64);
+                    const unsigned char* at = kt + (j >> 1) * 2048 + (j & 1 ? k_at ^ 64 : k_at);
+                    uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 1024);
                     if (SMALL) {
                         a.x ^= 0x80008000u; a.y ^= 0x80008000u; a.z ^= 0x80008000u; a.w ^= 0x80008000u;
                         c.x ^= 0x80008000u; c.y ^= 0x80008000u; c.z ^= 0x80008000u; c.w ^= 0x80008000u;
@@ -339,9 +352,9 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             load_half(NS & 1);
             next_slot();
             if (active) {
-                // one score a lane and tile of columns: position g (+ 8 for odd lanes), head 2n + (q4 >> 1).  Columns of a head behind the last one are zero and
+                // one score a lane and tile of columns: position k_row (+ 8 for odd lanes), head 2n + (q4 >> 1).  Columns of a head behind the last one are zero and
                 // so are their scores; nobody reads what becomes of them.
-                const u32 row = g + (odd ? 8 : 0);
+                const u32 row = k_row + (odd ? 8 : 0);
                 const bool seen = pos0 + row < len;
                 u32 ev[NT];
 #pragma unroll
@@ -359,18 +372,18 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                     esum[n] += ev[n];
                     const u32 col = (q4 >> 1) * 4;
                     if (SMALL) {
-                        // [NT][8 slots of depth][8 columns], a word for positions p and p + 4: the lane of p writes columns 0 and 1, that of p + 4 columns 2 and 3
+                        // [NT][8 slots of depth][8 columns], a word for positions p and p + 1: the lane of p writes columns 0 and 1, that of p + 1 columns 2 and 3
                         // (bytes 0 and 1 of digit_words, c = 0, 1 or 2, 3)
-                        const u32 other = __shfl_xor_sync(0xffffffffu, ev[n], 16);
-                        const bool high = g & 4;
+                        const u32 other = __shfl_xor_sync(0xffffffffu, ev[n], 8);
+                        const bool high = row & 1;
                         const u32 a = high ? other : ev[n], b = high ? ev[n] : other, sel = high ? 0x4312 : 0x0140;
                         const u32 x = __byte_perm(a, (a << (high ? 9 : 0)) >> (high ? 25 : 23), sel), y = __byte_perm(b, (b << (high ? 9 : 0)) >> (high ? 25 : 23), sel);
-                        *reinterpret_cast<uint2*>(ed + ((n * 8 + (row & 3) + 4 * (row >> 3)) * 8 + col + (high ? 2 : 0))) =
+                        *reinterpret_cast<uint2*>(ed + ((n * 8 + ((row & 7) >> 1) + 4 * (row >> 3)) * 8 + col + (high ? 2 : 0))) =
                             make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
-                    } else {                     // [NT][16 positions][8 columns]
+                    } else {                     // [NT][16 slots of depth][8 columns]
                         u32 dw[4];
                         digit_words(ev[n], dw);
-                        *reinterpret_cast<uint4*>(ed + (n * 16 + row) * 8 + col) = make_uint4(dw[0], dw[1], dw[2], dw[3]);
+                        *reinterpret_cast<uint4*>(ed + (n * 16 + (row & 8) + (row & 1) * 4 + ((row & 7) >> 1)) * 8 + col) = make_uint4(dw[0], dw[1], dw[2], dw[3]);
                     }
                 }
                 __syncwarp();
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             // values
             wait_half();
             if (active) {
-                const unsigned char* vt = pa_smem + ring_at + slot_out * S::HALF + q4 * S::VP + g * 16;
+                const unsigned char* vt = pa_smem + ring_at + slot_out * S::HALF;
                 constexpr int KS = SMALL ? 1 : 2;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
@@ -395,7 +408,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                             u32 v[4][4];
 #pragma unroll
                             for (int r = 0; r < 4; r++) {
-                                const uint4 t = *reinterpret_cast<const uint4*>(vt + r * 4 * S::VP + j * 128);
+                                const uint4 t = *reinterpret_cast<const uint4*>(vt + (r & 1 ? v_at1 : v_at0) + (r >> 1) * 1024 + j * 2048);
                                 v[r][0] = t.x; v[r][1] = t.y; v[r][2] = t.z; v[r][3] = t.w;
                             }
 #pragma unroll
@@ -406,7 +419,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                                 for (int n = 0; n < NT; n++) mma_u8_16x8x32(acc[4 * j + i][n], a0, a1, a2, a3, b0[n], b1[n]);
                             }
                         } else {
-                            const uint4 v = *reinterpret_cast<const uint4*>(vt + 2 * ks * 4 * S::VP + j * 128), u = *reinterpret_cast<const uint4*>(vt + (2 * ks + 1) * 4 * S::VP + j * 128);
+                            const uint4 v = *reinterpret_cast<const uint4*>(vt + v_at0 + ks * 1024 + j * 2048), u = *reinterpret_cast<const uint4*>(vt + v_at1 + ks * 1024 + j * 2048);
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
                                 mma_u8_16x8x32(acc[2 * j][n], v.x, v.y, u.x, u.y, b0[n], b1[n]);
@@ -517,15 +530,15 @@ inline PaChoice pa_choice(u32 d, u32 hpg) {
     return c;
 }
 template <int DP, bool SMALL, int NT>
-inline cudaError_t pa_launch(cudaStream_t stream, const PagedAttnArgs& a, PaWork w, int* launches) {
+inline cudaError_t pa_launch(cudaStream_t stream, const CUtensorMap (&maps)[2], const PagedAttnArgs& a, PaWork w, int* launches) {
     using S = PaShape<DP, SMALL>;
-    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)4 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED;
+    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)4 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED + 1024;
     static_assert(smem <= 226 * 1024, "with the kernel's own arrays below the 227 KB of a CTA");
     cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<DP, SMALL, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const u64 most = (u64)a.num_seqs * a.c.num_kv_heads * w.slices * ((((u64)a.max_blocks << a.c.page_bits) + S::WARPS * 16 - 1) / (S::WARPS * 16));
     if (most < w.ctas) w.ctas = (u32)most;
-    paged_attention_kernel<DP, SMALL, NT><<<w.ctas, S::WARPS * 32, smem, stream>>>(a, w);
+    paged_attention_kernel<DP, SMALL, NT><<<w.ctas, S::WARPS * 32, smem, stream>>>(maps[0], maps[1], a, w);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -13,33 +13,6 @@ cudaError_t kv_append_launch(cudaStream_t stream, int sm_count, const AppendArgs
     return cudaGetLastError();
 }
 
-size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs) {
-    if (!num_seqs) return 0;
-    const PaChoice c = pa_choice(d, num_heads / num_kv_heads);
-    return ((size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4) + (size_t)sm_count * 2) * 4;
-}
-cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const PagedAttnArgs& a, int* launches) {
-    const PaChoice c = pa_choice(a.c.d, a.num_heads / a.c.num_kv_heads);
-    const u32 size = a.c.small ? 2 : 4;
-    PaWork w{};
-    w.slices = c.slices;
-    w.slice_heads = c.slice_heads;
-    w.ctas = (u32)sm_count;
-    w.gave_up = a.gave_up;
-    w.slots = (u32*)a.workspace;
-    w.desc = w.slots + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4);
-    w.fast = a.c.d * size % 16 == 0 && a.c.page_stride * size % 16 == 0 && !((uintptr_t)a.c.k & 15) && !((uintptr_t)a.c.v & 15);
-    const u32 which = c.dp | c.nt << 16 | (a.c.small ? 1u << 24 : 0u);
-    switch (which) {
-#define ZKB_PA(DP, NT)                                                                              \
-    case DP | NT << 16: return pa_launch<DP, false, NT>(stream, a, w, launches);                     \
-    case DP | NT << 16 | 1u << 24: return pa_launch<DP, true, NT>(stream, a, w, launches);
-        ZKB_PA(64, 1) ZKB_PA(64, 2) ZKB_PA(64, 4) ZKB_PA(128, 1) ZKB_PA(128, 2) ZKB_PA(128, 4) ZKB_PA(256, 1) ZKB_PA(256, 2)
-#undef ZKB_PA
-    }
-    return cudaErrorInvalidValue;
-}
-
 // cuTensorMapEncodeTiled, without linking the driver library.
 static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 f = [] {
@@ -59,6 +32,46 @@ static cudaError_t rows_tensor_map(CUtensorMap* map, const u32* w, u32 rows, u32
     const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, (void*)w, dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs) {
+    if (!num_seqs) return 0;
+    const PaChoice c = pa_choice(d, num_heads / num_kv_heads);
+    return ((size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4) + (size_t)sm_count * 2) * 4;
+}
+cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const PagedAttnArgs& a, int* launches) {
+    const PaChoice c = pa_choice(a.c.d, a.num_heads / a.c.num_kv_heads);
+    const u32 size = a.c.small ? 2 : 4;
+    PaWork w{};
+    w.slices = c.slices;
+    w.slice_heads = c.slice_heads;
+    w.ctas = (u32)sm_count;
+    w.gave_up = a.gave_up;
+    w.slots = (u32*)a.workspace;
+    w.desc = w.slots + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4);
+    // Tensor copies want 16-byte boundaries; a box of less than the 8 rows of the swizzle's pattern is left to plain loads.
+    CUtensorMap maps[2] = {};
+    const uint64_t row_bytes = (uint64_t)a.c.d * size, page_bytes = a.c.page_stride * size;
+    if (a.c.page_bits >= 3 && ((u64)a.c.num_kv_heads << a.c.page_bits) < (1ull << 31) && row_bytes % 16 == 0 && page_bytes % 16 == 0 && page_bytes < (1ull << 40) && !((uintptr_t)a.c.k & 15) && !((uintptr_t)a.c.v & 15)) {
+        auto encode = tensor_map_encoder();
+        if (!encode) return cudaErrorNotSupported;
+        w.fast = a.c.page_bits >= 4 ? 16 : 8;
+        const cuuint64_t dims[3] = {a.c.d, (cuuint64_t)a.c.num_kv_heads << a.c.page_bits, a.c.num_pages}, strides[2] = {row_bytes, page_bytes};
+        const cuuint32_t box[3] = {128 / size, (cuuint32_t)w.fast, 1}, unit[3] = {1, 1, 1};
+        for (int i = 0; i < 2; i++)
+            if (encode(&maps[i], a.c.small ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, i ? a.c.v : a.c.k, dims, strides, box, unit,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+                return cudaErrorInvalidValue;
+    }
+    const u32 which = c.dp | c.nt << 16 | (a.c.small ? 1u << 24 : 0u);
+    switch (which) {
+#define ZKB_PA(DP, NT)                                                                              \
+    case DP | NT << 16: return pa_launch<DP, false, NT>(stream, maps, a, w, launches);                     \
+    case DP | NT << 16 | 1u << 24: return pa_launch<DP, true, NT>(stream, maps, a, w, launches);
+        ZKB_PA(64, 1) ZKB_PA(64, 2) ZKB_PA(64, 4) ZKB_PA(128, 1) ZKB_PA(128, 2) ZKB_PA(128, 4) ZKB_PA(256, 1) ZKB_PA(256, 2)
+#undef ZKB_PA
+    }
+    return cudaErrorInvalidValue;
 }
 
 static size_t round256(size_t b) { return (b + 255) & ~size_t(255); }

@@ -39,6 +39,12 @@ __device__ __forceinline__ void tensor_load_2d(u32 dst, const CUtensorMap* map, 
                  : "memory");
 }
 
+__device__ __forceinline__ void tensor_load_3d(u32 dst, const CUtensorMap* map, int x, int y, int z, u32 bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(bar)
+                 : "memory");
+}
+
 // One warp; `columns` a power of two from 32 to 512.
 __device__ __forceinline__ void tmem_alloc(u32 dst_smem, u32 columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(columns) : "memory");
