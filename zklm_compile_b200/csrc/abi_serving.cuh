@@ -134,6 +134,8 @@ int32_t zkb_paged_attention(zkb_ctx* c, const zkb_kv_cache* cache, const uint32_
         a.q_stride = serve_stride(q_stride, (uint64_t)num_heads * a.c.d, "q_stride");
         if (!num_seqs) return ZKB_OK;
         if (!max_blocks) throw ArgFail{ZKB_E_ARG, "paged_attention: a block table without places"};
+        // the work is counted in tiles of 16 positions and up, in 32 bits a CTA
+        if ((double)num_seqs * max_blocks * cache->page_size * num_heads >= (double)(1ull << 42)) throw ArgFail{ZKB_E_TOO_LARGE, "paged_attention: more than 2^42 scores"};
         need_words(q_dev, "q"); need_words(block_table_dev, "block_table"); need_words(lens_dev, "lens"); need_words(table_out_dev, "the exp table");
         need_words(out_dev, "out"); need_words(status_dev, "status");
         a.q = q_dev; a.num_heads = num_heads; a.num_seqs = num_seqs; a.max_blocks = max_blocks;

@@ -82,8 +82,7 @@ __device__ __forceinline__ u32 pa_blocks(const PagedAttnArgs& A, u32 seq, u32 bl
 }
 // The stream of blocks that a CTA takes: sequences, in each its (key head, slice) items, in each its blocks.
 struct PaWalk {
-    u32 seq, grp, blk, nb, len, block, grps;
-    u64 left;
+    u32 seq, grp, blk, nb, len, block, grps, left;
     __device__ __forceinline__ void step(const PagedAttnArgs& A, u32 n) {
         left -= n;
         blk += n;
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     cw.seq = start_seq;
     cw.block = BLOCK;
     cw.grps = grps;
-    cw.left = to - from;
+    cw.left = (u32)(to - from);
     cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
     cw.grp = (u32)(start_total / cw.nb);
     cw.blk = (u32)(start_total - (u64)cw.grp * cw.nb);
@@ -181,6 +180,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     constexpr u32 E = SMALL ? 2 : 4;
     const u32 row_bytes = d * E;
     const u64 page_bytes = A.c.page_stride * E;
+    const u32 columns = (row_bytes + 127) / 128;
     if (lane == 0) {
         for (int i = 0; i < NS; i++) mbar_init(bar0 + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -188,40 +188,56 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     }
     __syncwarp();
     u32 bad_pages = 0, loaded = 0;             // bit k: the tile k tiles behind the last one that was copied has a bad page
-    int page_next = 0, page = -1;              // lanes 0 .. 15: the page of their position in the next tile and in this one, -1: none
-    auto fetch_page = [&](const PaWalk& w) {
-        const u32 pos = w.blk * BLOCK + warp * 16 + lane;
-        page_next = lane < 16 && w.left && pos < w.len ? A.block_table[(size_t)w.seq * A.max_blocks + (pos >> A.c.page_bits)] : 0;
+    // With tensor copies a tile lies in one page (two of 8 rows), the same for all lanes, fetched a tile ahead; without, lanes 0 .. 15 look up their rows'.
+    int next0 = 0, next1 = 0, page0 = -1, page1 = -1;
+    auto page_of = [&](u32 pos) { return A.block_table[(size_t)lw.seq * A.max_blocks + (pos >> A.c.page_bits)]; };
+    auto fetch_page = [&] {
+        const u32 pos0 = lw.blk * BLOCK + warp * 16;
+        if (!P.fast || !lw.left) return;
+        next0 = pos0 < lw.len ? page_of(pos0) : 0;
+        if (P.fast == 8) next1 = pos0 + 8 < lw.len ? page_of(pos0 + 8) : 0;
     };
     u32 slot_in = 0;
     auto load_half = [&](bool is_v) {          // the next half tile into the next slot
         if (!lw.left) return;
-        const u32 pos = lw.blk * BLOCK + warp * 16 + lane;
-        if (!is_v) {
-            const bool there = lane < 16 && pos < lw.len, fine = page_next >= 0 && (u32)page_next < A.c.num_pages;
-            page = there && fine ? page_next : -1;
-            bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, there && !fine) ? 1u : 0u);
-            loaded++;
-        }
-        const u32 bar = bar0 + 8 * slot_in, y0 = ((lw.grp / P.slices) << A.c.page_bits) + (pos & mask);
+        const u32 pos0 = lw.blk * BLOCK + warp * 16, bar = bar0 + 8 * slot_in, kv_row = (lw.grp / P.slices) << A.c.page_bits;
         if (P.fast) {
-            // boxes of 16 rows (8 where a page has no more) by 128 bytes; the lane of a box's first row has its page
-            const u32 rows = P.fast, at = lane & 15;
-            const bool mine = lane < 16 && page >= 0 && at % rows == 0;
-            const u32 boxes = __popc(__ballot_sync(0xffffffffu, mine));
-            const u32 columns = (row_bytes + 127) / 128, dst = ring + slot_in * S::HALF + at * 128;
-            if (lane == 0) mbar_expect(bar, boxes * columns * rows * 128);
-            if (mine)
-                for (u32 c = 0; c < columns; c++) tensor_load_3d(dst + c * 2048, is_v ? &map_v : &map_k, (int)(c * (128 / E)), (int)y0, page, bar);
+            // boxes of 16 rows (8 where a page has no more) by 128 bytes
+            if (!is_v) {
+                const bool fine0 = (u32)next0 < A.c.num_pages, fine1 = (u32)next1 < A.c.num_pages;
+                page0 = fine0 && pos0 < lw.len ? next0 : -1;
+                page1 = fine1 && P.fast == 8 && pos0 + 8 < lw.len ? next1 : -1;
+                bad_pages = bad_pages << 1 | (u32)(!fine0 || !fine1);
+                loaded++;
+            }
+            if (lane == 0) {
+                const u32 bytes = columns * 128 * P.fast, dst = ring + slot_in * S::HALF;
+                mbar_expect(bar, (page0 >= 0 ? bytes : 0u) + (page1 >= 0 ? bytes : 0u));
+                const CUtensorMap* map = is_v ? &map_v : &map_k;
+#pragma unroll
+                for (u32 c = 0; c < RB / 128; c++) {
+                    if (c >= columns) break;
+                    if (page0 >= 0) tensor_load_3d(dst + c * 2048, map, (int)(c * (128 / E)), (int)(kv_row + (pos0 & mask)), page0, bar);
+                    if (page1 >= 0) tensor_load_3d(dst + c * 2048 + 1024, map, (int)(c * (128 / E)), (int)(kv_row + ((pos0 + 8) & mask)), page1, bar);
+                }
+            }
         } else {
-            const char* src = (const char*)(is_v ? A.c.v : A.c.k) + (u64)(u32)page * page_bytes + (u64)y0 * row_bytes;
+            const u32 pos = pos0 + lane;
+            const bool there = lane < 16 && pos < lw.len;
+            const int page = there ? page_of(pos) : 0;
+            const bool fine = (u32)page < A.c.num_pages;
+            if (!is_v) {
+                bad_pages = bad_pages << 1 | (__any_sync(0xffffffffu, !fine) ? 1u : 0u);
+                loaded++;
+            }
+            const char* src = (const char*)(is_v ? A.c.v : A.c.k) + (u64)(u32)page * page_bytes + (u64)(kv_row + (pos & mask)) * row_bytes;
             for (int r = 0; r < 16; r++) {
                 const char* from_row = (const char*)__shfl_sync(0xffffffffu, (u64)src, r);
-                if (__shfl_sync(0xffffffffu, page, r) < 0) continue;
-                unsigned char* to = pa_smem + ring_at + slot_in * S::HALF + r * 128;
+                if (!__shfl_sync(0xffffffffu, (int)(there && fine), r)) continue;
+                unsigned char* to_row = pa_smem + ring_at + slot_in * S::HALF + r * 128;
                 for (u32 i = lane; i < d; i += 32) {
                     const u32 byte = i * E;
-                    unsigned char* w = to + (byte >> 7) * 2048 + ((byte & 127) ^ ((r & 7) << 4));
+                    unsigned char* w = to_row + (byte >> 7) * 2048 + ((byte & 127) ^ ((r & 7) << 4));
                     if (SMALL) *reinterpret_cast<uint16_t*>(w) = reinterpret_cast<const uint16_t*>(from_row)[i];
                     else *reinterpret_cast<u32*>(w) = reinterpret_cast<const u32*>(from_row)[i];
                 }
@@ -229,10 +245,10 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         }
-        if (is_v) { lw.step(A, 1); fetch_page(lw); }
+        if (is_v) { lw.step(A, 1); fetch_page(); }
         slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
     };
-    fetch_page(lw);
+    fetch_page();
 #pragma unroll
     for (int h = 0; h < NS; h++) load_half(h & 1);
 
@@ -250,7 +266,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     while (cw.left) {
         const u32 seq = cw.seq, kvh = cw.grp / P.slices, head0 = kvh * hpg + (cw.grp - kvh * P.slices) * P.slice_heads;
         const u32 rest = hpg - (cw.grp - kvh * P.slices) * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
-        const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? (u32)cw.left : nb - first;
+        const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? cw.left : nb - first;
         const u32 item = seq * grps + cw.grp;
         __syncthreads();                        // the row before is done with these arrays
         for (u32 i = tid; i < J * NT * 32; i += THREADS) {
@@ -320,11 +336,10 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         const u32 round_up = (1u << A.score_shift) >> 1;
         for (u32 b = 0; b < count; b++) {
             const u32 pos0 = (first + b) * BLOCK + warp * 16;
-            const bool active = pos0 < len;
-            // keys
+            // keys.  A warp behind the last position goes along with what its slot holds: none of its positions is seen, so all its weights are zero.
             wait_half();
             int sc[NT][4];
-            if (active) {
+            {
                 if ((bad_pages >> (loaded - 1 - computed)) & 1) bad |= 1;
                 const unsigned char* kt = pa_smem + ring_at + slot_out * S::HALF;
 #pragma unroll
@@ -351,7 +366,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             __syncwarp();                        // every lane has read its keys
             load_half(NS & 1);
             next_slot();
-            if (active) {
+            {
                 // one score a lane and tile of columns: position k_row (+ 8 for odd lanes), head 2n + (q4 >> 1).  Columns of a head behind the last one are zero and
                 // so are their scores; nobody reads what becomes of them.
                 const u32 row = k_row + (odd ? 8 : 0);
@@ -390,7 +405,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             }
             // values
             wait_half();
-            if (active) {
+            {
                 const unsigned char* vt = pa_smem + ring_at + slot_out * S::HALF;
                 constexpr int KS = SMALL ? 1 : 2;
 #pragma unroll
