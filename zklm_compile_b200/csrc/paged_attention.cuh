@@ -70,6 +70,7 @@ struct PaWork {                                // see paged_attention_launch
     u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
     u32* desc;                                 // [ctas][2]: 1 + item that begins in this CTA and goes on in the next, number of CTAs it goes on in
     int fast;                                  // tensor copies: rows are whole 16-byte groups on 16-byte boundaries, pages have 8 rows or more
+    int whole;                                 // a box has all the columns of its rows
     int* gave_up;
 };
 enum : u32 { PA_BAD_PAGE = 1, PA_BAD_SCORE = 2 };
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         if (!lw.left) return;
         const u32 pos0 = lw.blk * BLOCK + warp * 16, bar = bar0 + 8 * slot_in, kv_row = (lw.grp / P.slices) << A.c.page_bits;
         if (P.fast) {
-            // boxes of 16 rows (8 where a page has no more) by 128 bytes
+            // boxes of 16 rows (8 where a page has no more), all of a row where it is whole columns of 128 bytes, else a column each
             if (!is_v) {
                 const bool fine0 = (u32)next0 < A.c.num_pages, fine1 = (u32)next1 < A.c.num_pages;
                 page0 = fine0 && pos0 < lw.len ? next0 : -1;
@@ -210,16 +211,12 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 bad_pages = bad_pages << 1 | (u32)(!fine0 || !fine1);
                 loaded++;
             }
-            if (lane == 0) {
-                const u32 bytes = columns * 128 * P.fast, dst = ring + slot_in * S::HALF;
-                mbar_expect(bar, (page0 >= 0 ? bytes : 0u) + (page1 >= 0 ? bytes : 0u));
-                const CUtensorMap* map = is_v ? &map_v : &map_k;
-#pragma unroll
-                for (u32 c = 0; c < RB / 128; c++) {
-                    if (c >= columns) break;
-                    if (page0 >= 0) tensor_load_3d(dst + c * 2048, map, (int)(c * (128 / E)), (int)(kv_row + (pos0 & mask)), page0, bar);
-                    if (page1 >= 0) tensor_load_3d(dst + c * 2048 + 1024, map, (int)(c * (128 / E)), (int)(kv_row + ((pos0 + 8) & mask)), page1, bar);
-                }
+            const u32 bytes = columns * 128 * P.fast, dst = ring + slot_in * S::HALF, step = P.whole ? columns : 1u;
+            mbar_expect_one(bar, (page0 >= 0 ? bytes : 0u) + (page1 >= 0 ? bytes : 0u));
+            const CUtensorMap* map = is_v ? &map_v : &map_k;
+            for (u32 c = 0; c < columns; c += step) {
+                if (page0 >= 0) tensor_load_4d_one(dst + c * 2048, map, (int)(c * (128 / E)), (int)(kv_row + (pos0 & mask)), 0, page0, bar);
+                if (page1 >= 0) tensor_load_4d_one(dst + c * 2048 + 1024, map, (int)(c * (128 / E)), (int)(kv_row + ((pos0 + 8) & mask)), 0, page1, bar);
             }
         } else {
             const u32 pos = pos0 + lane;

@@ -56,10 +56,13 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
         auto encode = tensor_map_encoder();
         if (!encode) return cudaErrorNotSupported;
         w.fast = a.c.page_bits >= 4 ? 16 : 8;
-        const cuuint64_t dims[3] = {a.c.d, (cuuint64_t)a.c.num_kv_heads << a.c.page_bits, a.c.num_pages}, strides[2] = {row_bytes, page_bytes};
-        const cuuint32_t box[3] = {128 / size, (cuuint32_t)w.fast, 1}, unit[3] = {1, 1, 1};
+        w.whole = w.fast == 16 && row_bytes % 128 == 0;
+        const u32 columns = w.whole ? (u32)(row_bytes / 128) : 1u;
+        const cuuint64_t dims[4] = {w.whole ? 128 / size : a.c.d, (cuuint64_t)a.c.num_kv_heads << a.c.page_bits, columns, a.c.num_pages};
+        const cuuint64_t strides[3] = {row_bytes, w.whole ? 128 : row_bytes, page_bytes};
+        const cuuint32_t box[4] = {128 / size, (cuuint32_t)w.fast, columns, 1}, unit[4] = {1, 1, 1, 1};
         for (int i = 0; i < 2; i++)
-            if (encode(&maps[i], a.c.small ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, i ? a.c.v : a.c.k, dims, strides, box, unit,
+            if (encode(&maps[i], a.c.small ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, i ? a.c.v : a.c.k, dims, strides, box, unit,
                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
                 return cudaErrorInvalidValue;
     }

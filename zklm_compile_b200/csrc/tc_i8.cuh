@@ -39,9 +39,15 @@ __device__ __forceinline__ void tensor_load_2d(u32 dst, const CUtensorMap* map, 
                  : "memory");
 }
 
-__device__ __forceinline__ void tensor_load_3d(u32 dst, const CUtensorMap* map, int x, int y, int z, u32 bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
-                 "r"(z), "r"(bar)
+// By one lane of a converged warp, all of whose lanes have the same operands: chosen inside the instruction's own statement, so that the compiler need not
+// provide for several lanes with operands of their own (a branch on the lane cost fifty instructions a copy).
+__device__ __forceinline__ void mbar_expect_one(u32 bar, u32 bytes) {
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; @p mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tensor_load_4d_one(u32 dst, const CUtensorMap* map, int x, int y, int z, int w, u32 bar) {
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff;\n"
+                 "@p cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6]; }" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(w), "r"(bar)
                  : "memory");
 }
 
