@@ -83,14 +83,16 @@ __device__ __forceinline__ u32 pa_blocks(const PagedAttnArgs& A, u32 seq, u32 bl
 }
 // The stream of blocks that a CTA takes: sequences, in each its (key head, slice) items, in each its blocks.
 struct PaWalk {
-    u32 seq, grp, blk, nb, len, block, grps, left;
+    u32 seq, kvh, slice, blk, nb, len, block, slices, left;
     __device__ __forceinline__ void step(const PagedAttnArgs& A, u32 n) {
         left -= n;
         blk += n;
         if (blk < nb || !left) return;
         blk = 0;
-        if (++grp < grps) return;
-        grp = 0;
+        if (++slice < slices) return;
+        slice = 0;
+        if (++kvh < A.c.num_kv_heads) return;
+        kvh = 0;
         do nb = pa_blocks(A, ++seq, block, len);
         while (nb == 0);                       // left > 0: there is one
     }
@@ -168,11 +170,13 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     PaWalk cw{};
     cw.seq = start_seq;
     cw.block = BLOCK;
-    cw.grps = grps;
+    cw.slices = P.slices;
     cw.left = (u32)(to - from);
     cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
-    cw.grp = (u32)(start_total / cw.nb);
-    cw.blk = (u32)(start_total - (u64)cw.grp * cw.nb);
+    const u32 start_grp = (u32)(start_total / cw.nb);
+    cw.kvh = start_grp / P.slices;
+    cw.slice = start_grp - cw.kvh * P.slices;
+    cw.blk = (u32)(start_total - (u64)start_grp * cw.nb);
     PaWalk lw = cw;                            // the copies run ahead of the computation
 
     // ---- copies -------------------------------------------------------------------------------------
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     u32 slot_in = 0;
     auto load_half = [&](bool is_v) {          // the next half tile into the next slot
         if (!lw.left) return;
-        const u32 pos0 = lw.blk * BLOCK + warp * 16, bar = bar0 + 8 * slot_in, kv_row = (lw.grp / P.slices) << A.c.page_bits;
+        const u32 pos0 = lw.blk * BLOCK + warp * 16, bar = bar0 + 8 * slot_in, kv_row = lw.kvh << A.c.page_bits;
         if (P.fast) {
             // boxes of 16 rows (8 where a page has no more), all of a row where it is whole columns of 128 bytes, else a column each
             if (!is_v) {
@@ -261,10 +265,9 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     // ---- the stretches of items ---------------------------------------------------------------------
     u32 computed = 0;
     while (cw.left) {
-        const u32 seq = cw.seq, kvh = cw.grp / P.slices, head0 = kvh * hpg + (cw.grp - kvh * P.slices) * P.slice_heads;
-        const u32 rest = hpg - (cw.grp - kvh * P.slices) * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
+        const u32 seq = cw.seq, head0 = cw.kvh * hpg + cw.slice * P.slice_heads, rest = hpg - cw.slice * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
         const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? cw.left : nb - first;
-        const u32 item = seq * grps + cw.grp;
+        const u32 item = seq * grps + cw.kvh * P.slices + cw.slice;
         __syncthreads();                        // the row before is done with these arrays
         for (u32 i = tid; i < J * NT * 32; i += THREADS) {
             // 16 bytes of the right operand of a lane: steps 2j, 2j + 1 of a tile of 8 columns
