@@ -20,7 +20,8 @@ constexpr u32 LIN_STEP = 32;                   // columns of W per step: 128 byt
 constexpr u32 LIN_SEG = 256;                   // steps after which the accumulators are emptied (8192 columns)
 constexpr u32 LIN_TOKENS = 64;                 // tokens per tile at most: 256 columns of an accumulator
 constexpr u32 LIN_MAX_STAGES = 8;
-constexpr u32 LIN_THREADS = 192;               // warp 0 copies, warp 1 issues, warps 2 to 5 empty the accumulators
+constexpr u32 LIN_FILL = 128;                  // threads that fill operands by plain stores, where a kernel has such
+constexpr u32 LIN_JOIN_TOKENS = 8;
 
 // Byte c of the four rotations of x by 8i, i = 0 .. 3, for c = 0 .. 3.  All of them are bytes of x, of x >> 7, or of x without the top bits of its bytes.
 __device__ __forceinline__ void digit_words(u32 x, u32 (&w)[4]) {
@@ -34,27 +35,34 @@ __device__ __forceinline__ void digit_words(u32 x, u32 (&w)[4]) {
 // How a product is cut: `tiles` of LIN_ROWS rows x `tt` tokens, each `steps` deep in `segs` segments.  Tiles' steps lie one behind the other and every CTA takes `per`
 // of them, so all CTAs finish together; a CTA leaves its sum over each stretch of one tile's segment in slot (CTA + tile * segs + segment), which are all different.
 struct LinPlan {
-    u32 tokens, m, n, tt, ntiles, mtiles, steps, segs, per, ctas, stages, stage_bytes, tmem_cols;
+    u32 tokens, m, n, a_rows, tt, ntiles, mtiles, wtiles, steps, segs, per, ctas, stages, stage_bytes, tmem_cols;   // tiles: wtiles of W, then those of the adapters' A
     u64 total;
     size_t slot_words;
 };
-inline LinPlan lin_plan(int sm_count, u32 tokens, u32 m, u32 n) {
+inline LinPlan lin_plan(int sm_count, u32 tokens, u32 m, u32 n, u32 a_rows) {
     LinPlan p{};
-    p.tokens = tokens; p.m = m; p.n = n;
+    p.tokens = tokens; p.m = m; p.n = n; p.a_rows = a_rows;
     p.ntiles = (tokens + LIN_TOKENS - 1) / LIN_TOKENS;
     p.tt = ((tokens + p.ntiles - 1) / p.ntiles + 3) / 4 * 4;
-    p.mtiles = (m + LIN_ROWS - 1) / LIN_ROWS;
+    p.wtiles = (m + LIN_ROWS - 1) / LIN_ROWS;
+    p.mtiles = p.wtiles + (a_rows + LIN_ROWS - 1) / LIN_ROWS;
     p.steps = (n + LIN_STEP - 1) / LIN_STEP;
     p.segs = (p.steps + LIN_SEG - 1) / LIN_SEG;
     p.total = (u64)p.mtiles * p.ntiles * p.steps;
     p.per = (u32)((p.total + sm_count - 1) / sm_count);
     p.ctas = (u32)((p.total + p.per - 1) / p.per);
-    p.stage_bytes = LIN_ROWS * 128 + 4 * p.tt * 128;
+    p.stage_bytes = LIN_ROWS * 128 + (4 * p.tt * 128 + 1023) / 1024 * 1024;
     p.stages = 200 * 1024 / p.stage_bytes < LIN_MAX_STAGES ? 200 * 1024 / p.stage_bytes : LIN_MAX_STAGES;
     p.tmem_cols = 32;
     while (p.tmem_cols < 8 * p.tt) p.tmem_cols *= 2;
     p.slot_words = (size_t)p.tt * LIN_ROWS;
     return p;
+}
+// Rows of A that the product takes along with W's (all adapters for all tokens), or 0: then each token's own rank products are made apart.
+// Along, an adapter's rows are read once however many tokens use it and no launch is added; apart, no adapter that no token has is read.
+inline u32 lin_a_rows(u32 tokens, u32 m, u32 num_adapters, u32 rank) {
+    const u64 rows = (u64)num_adapters * rank, tiles = (rows + LIN_ROWS - 1) / LIN_ROWS, wtiles = (m + LIN_ROWS - 1) / LIN_ROWS;
+    return rows && (tiles <= (wtiles < 8 ? 1 : wtiles / 8) || tiles * LIN_ROWS <= (u64)tokens * rank / 2) && rows < (1u << 30) ? (u32)rows : 0u;
 }
 // Tokens of one pass: their operand (16 bytes a value) is read by every row of tiles and should stay in L2.
 inline u32 lin_chunk(u32 tokens, u32 n) {
@@ -62,11 +70,14 @@ inline u32 lin_chunk(u32 tokens, u32 n) {
     const u32 most = fit < LIN_TOKENS ? LIN_TOKENS : (fit > 2048 ? 2048u : (u32)fit);
     return tokens < most ? tokens : most;
 }
-inline size_t lin_digit_bytes(const LinPlan& p) { return (size_t)p.ntiles * p.steps * p.tt * 512; }
-inline size_t lin_slot_bytes(const LinPlan& p) { return ((size_t)p.ctas + (size_t)p.mtiles * p.ntiles * p.segs) * p.slot_words * 4; }
+inline bool lin_fused(const LinPlan& p) { return p.ntiles == 1; }
+inline size_t lin_digit_bytes(const LinPlan& p) { return lin_fused(p) ? 0 : (size_t)p.ntiles * p.steps * p.tt * 512; }
+// For any number of tokens up to the plan's: fewer of them may be shared by more CTAs.
+inline size_t lin_slot_bytes(int sm_count, const LinPlan& p) { return ((size_t)sm_count + (size_t)p.mtiles * p.ntiles * p.segs) * p.slot_words * 4; }
 
 // The tokens' operand, in the order in which the tiles are copied: per (tile of tokens, step) 4 tt rows of 128 bytes, swizzled.
 __global__ void __launch_bounds__(512) linear_digits_kernel(const u32* __restrict__ x, u64 x_stride, LinPlan p, unsigned char* __restrict__ out) {
+    pdl_launch_dependents();
     const u32 step = blockIdx.x, nt = blockIdx.y, tok = threadIdx.x >> 3, q = threadIdx.x & 7;
     const u32 t = nt * p.tt + tok, j = step * LIN_STEP + 4 * q;
     unsigned char* tile = out + ((size_t)nt * p.steps + step) * p.tt * 512;
@@ -105,17 +116,24 @@ struct LinWalk {                               // a CTA's stretches, the same fo
     }
 };
 
-__global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_constant__ CUtensorMap map_w, LinPlan p, const unsigned char* __restrict__ digits,
-                                                                   u32* __restrict__ slots, int* gave_up_out) {
-    extern __shared__ __align__(16) unsigned char lin_smem[];
+// Warp 0 copies, warp 1 issues, warps 2 to 5 empty the accumulators, and where W or the tokens' operand is filled by plain stores warps 6 to 9 do that.
+// W_COPY: W by tensor copies; otherwise (rows that start on no 16-byte boundary) word by word.  X_FILL: the tokens' operand is made here from x,
+// which for one tile of tokens costs less than copying its 16 bytes a value; otherwise it is copied from where linear_digits_kernel left it.
+template <bool W_COPY, bool X_FILL>
+__global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) linear_bytes_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
+                                                                                              LinPlan p, LinearArgs A, int x_vec, const unsigned char* __restrict__ digits,
+                                                                                              u32* __restrict__ slots) {
+    constexpr bool FILL = !W_COPY || X_FILL;
+    extern __shared__ __align__(16) unsigned char lin_raw[];
     __shared__ __align__(8) u64 bars[2 * LIN_MAX_STAGES + 2];
     __shared__ u32 tmem_base;
     __shared__ volatile int gave_up;
     const u32 warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const u32 base = (smem_addr(lin_smem) + 1023) & ~1023u;
+    unsigned char* const smem = lin_raw + ((0u - smem_addr(lin_raw)) & 1023u);         // the swizzle goes by addresses
+    const u32 base = smem_addr(smem);
     const u32 full = smem_addr(bars), empty = full + 8 * LIN_MAX_STAGES, acc_full = empty + 8 * LIN_MAX_STAGES, acc_empty = acc_full + 8;
     if (threadIdx.x == 0) {
-        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, FILL ? 1 + LIN_FILL / 32 : 1); mbar_init(empty + 8 * s, 1); }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 4);
         gave_up = 0;
@@ -125,21 +143,28 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const u32 tmem = tmem_base, b_bytes = p.tt * 512;
     LinWalk walk(p);
     if (warp == 0) {
         if (lane == 0) {
             u32 it = 0;
             bool ok = true;
+            if (!X_FILL) pdl_wait();             // the digits come from the kernel before this one
             while (ok && walk.next()) {
+                const bool of_w = walk.mt < p.wtiles;
+                const int row = (int)((of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS);
                 for (u32 k = 0; k < walk.count; k++, it++) {
                     const u32 s = it % p.stages, round = it / p.stages, st = base + s * p.stage_bytes;
                     if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
-                    mbar_expect(full + 8 * s, p.stage_bytes);
-                    tensor_load_2d(st, &map_w, (int)((walk.first + k) * LIN_STEP), (int)(walk.mt * LIN_ROWS), full + 8 * s);
-                    bulk_load(st + LIN_ROWS * 128, digits + ((size_t)walk.nt * p.steps + walk.first + k) * b_bytes, b_bytes, full + 8 * s);
+                    mbar_expect(full + 8 * s, (W_COPY ? LIN_ROWS * 128 : 0u) + (X_FILL ? 0u : b_bytes));
+                    if (W_COPY) tensor_load_2d(st, of_w ? &map_w : &map_a, (int)((walk.first + k) * LIN_STEP), row, full + 8 * s);
+                    if (!X_FILL) bulk_load(st + LIN_ROWS * 128, digits + ((size_t)walk.nt * p.steps + walk.first + k) * b_bytes, b_bytes, full + 8 * s);
                 }
             }
+            // Where x is read directly, the kernel before this one (if it is one of the same call) makes what the join reads: the join, which waits for this
+            // kernel, must find it done.
+            if (X_FILL) pdl_wait();
             if (!ok)                             // given up: nothing of this CTA may still be in flight when it ends
                 for (u32 i = it > p.stages ? it - p.stages : 0; i < it; i++)
                     for (u32 n = 0; n < (1u << 16) && !mbar_try(full + 8 * (i % p.stages), (i / p.stages) & 1); n++) {}
@@ -152,7 +177,7 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
             while (ok && walk.next()) {
                 if (n && !(ok = mbar_wait(acc_empty, (n - 1) & 1, &gave_up))) { mma_commit(acc_full); n++; break; }
                 tc_fence_after();
-                const bool two = walk.mt * LIN_ROWS + 128 < p.m;
+                const bool two = walk.mt < p.wtiles ? walk.mt * LIN_ROWS + 128 < p.m : (walk.mt - p.wtiles) * LIN_ROWS + 128 < p.a_rows;
                 for (u32 k = 0; k < walk.count; k++, it++) {
                     const u32 s = it % p.stages, st = base + s * p.stage_bytes;
                     if (!(ok = mbar_wait(full + 8 * s, (it / p.stages) & 1, &gave_up))) break;
@@ -172,16 +197,17 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
             if (!ok)
                 for (u32 i = 0; i < (1u << 16) && !mbar_try(acc_full, (n - 1) & 1); i++) {}
         }
-    } else {
+    } else if (warp < 6) {
         const u32 quarter = warp & 3;            // the lanes of TMEM that this warp may read
         u32 n = 0;
         while (walk.next()) {
             if (!mbar_wait(acc_full, n & 1, &gave_up)) break;
             tc_fence_after();
             u32* slot = slots + (size_t)walk.slot * p.slot_words;
+            const u32 rows = walk.mt < p.wtiles ? p.m - walk.mt * LIN_ROWS : p.a_rows - (walk.mt - p.wtiles) * LIN_ROWS;
             for (u32 half = 0; half < 2; half++) {
                 const u32 row = half * 128 + quarter * 32 + lane;
-                if (walk.mt * LIN_ROWS + half * 128 >= p.m) break;
+                if (half * 128 >= rows) break;
                 for (u32 t0 = 0; t0 < p.tt; t0 += 16) {
                     u32 v[4][16];
 #pragma unroll
@@ -203,80 +229,204 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
             if (lane == 0) mbar_arrive(acc_empty);
             n++;
         }
+    } else if (FILL) {
+        const u32 tid = threadIdx.x - 192;
+        u32 it = 0, late = 0;                    // late: a step whose words of W are still on their way
+        bool ok = true;
+        u32 x[4][4];
+        // the thread's groups of four values of x: token (tid + 128 i) / 8, columns 4 (tid & 7) .. of the step
+        auto fetch = [&](u32 step) {
+#pragma unroll
+            for (u32 i = 0; i < 4; i++) {
+                const u32 t = (tid >> 3) + 16 * i, j = step * LIN_STEP + 4 * (tid & 7);
+                const u32* at = A.x + t * A.x_stride + j;
+                if (x_vec && t < p.tokens && j + 4 <= p.n) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(at);
+                    x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+                } else {
+#pragma unroll
+                    for (u32 e = 0; e < 4; e++) x[i][e] = t < p.tokens && j + e < p.n ? at[e] : 0u;
+                }
+            }
+        };
+        auto signal = [&](u32 step_it) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * (step_it % p.stages));
+        };
+        bool more = walk.next();
+        u32 k = 0;
+        if (X_FILL && more) fetch(walk.first);
+        while (more && ok) {
+            const u32 s = it % p.stages, round = it / p.stages, step = walk.first + k;
+            const bool of_w = walk.mt < p.wtiles;
+            const u32 row0 = (of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS, rows = (of_w ? p.m : p.a_rows) - row0;
+            unsigned char* st = smem + s * p.stage_bytes;
+            if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
+            if (!W_COPY) {
+                const u32 j = step * LIN_STEP + lane, most = rows < LIN_ROWS ? rows : LIN_ROWS;
+                const u32* src = (of_w ? A.w : A.a) + (size_t)row0 * p.n + j;
+                for (u32 r = warp - 6; r < most; r += LIN_FILL / 32) {
+                    const u32 to = smem_addr(st) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+                    // past the end of a row nothing is read and zero is stored
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(j < p.n ? src + (size_t)r * p.n : A.w), "r"(j < p.n ? 4 : 0) : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            if (X_FILL) {
+#pragma unroll
+                for (u32 i = 0; i < 4; i++) {
+                    const u32 tok = (tid >> 3) + 16 * i, q = tid & 7;
+                    if (tok >= p.tt) break;
+                    u32 w[4][4];
+#pragma unroll
+                    for (u32 e = 0; e < 4; e++) {
+                        u32 d[4];
+                        digit_words(x[i][e], d);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) w[c][e] = d[c];
+                    }
+#pragma unroll
+                    for (u32 c = 0; c < 4; c++) {
+                        const u32 r = 4 * tok + c;
+                        *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+                    }
+                }
+            }
+            if (++k == walk.count) { more = walk.next(); k = 0; }
+            if (X_FILL && more) fetch(walk.first + k);
+            if (W_COPY) {
+                signal(it);
+            } else {
+                if (late) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    signal(it - 1);
+                }
+                late = 1;
+            }
+            it++;
+        }
+        if (!W_COPY) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (late && ok) signal(it - 1);
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, p.tmem_cols);
-    if (threadIdx.x == 0 && gave_up) *gave_up_out = 1;
+    if (threadIdx.x == 0 && gave_up) *A.gave_up = 1;
 }
 
-// Sum of one output's slots (see LinPlan).
-__device__ __forceinline__ u64 lin_sum(const LinPlan& p, const u32* __restrict__ slots, u32 t, u32 i) {
-    const u32 nt = t / p.tt, mt = i / LIN_ROWS, tile = mt * p.ntiles + nt;
-    const size_t in = (size_t)(t - nt * p.tt) * LIN_ROWS + (i - mt * LIN_ROWS);
+// Sum of one output's slots (see LinPlan): row i of tile mt, token t.
+__device__ __forceinline__ u64 lin_sum(const LinPlan& p, const u32* __restrict__ slots, u32 mt, u32 t, u32 row) {
+    const u32 nt = t / p.tt, tile = mt * p.ntiles + nt;
+    const size_t in = (size_t)(t - nt * p.tt) * LIN_ROWS + row;
     const u64 begin = (u64)tile * p.steps;
     u64 s = 0;
     for (u32 seg = 0; seg < p.segs; seg++) {
         const u64 b = begin + seg * LIN_SEG, e = begin + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps);
-        for (u32 c = (u32)(b / p.per); c <= (u32)((e - 1) / p.per); c++) s += slots[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words + in];
+        const u32 last = (u32)((e - 1) / p.per);
+        for (u32 c = (u32)(b / p.per); c <= last; c++) s += slots[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words + in];
     }
     return s;
 }
-__global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan p, const u32* __restrict__ slots, const u32* __restrict__ u) {
-    const u32 i = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+// Four products of field elements fit 64 bits.
+__device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
+    const u64 s = (u64)a[0] * b[0] + (u64)a[1] * b[1] + (u64)a[2] * b[2] + (u64)a[3] * b[3];
+    return (s & ZKB_P) + (s >> 31);
+}
+// One CTA: a tile's 256 rows, LIN_JOIN_TOKENS tokens.  The rows of B that a thread needs stay in registers, 16 values at a time, while tokens beside each
+// other have the same adapter.
+__global__ void __launch_bounds__(LIN_ROWS) linear_join_kernel(LinearArgs A, LinPlan p, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
+    extern __shared__ __align__(16) u32 lin_u[];         // [LIN_JOIN_TOKENS][rank rounded up to 16]
+    __shared__ int of[LIN_JOIN_TOKENS];
+    const u32 mt = blockIdx.x, t0 = blockIdx.y * LIN_JOIN_TOKENS, i = mt * LIN_ROWS + threadIdx.x, rank = A.rank, pad = (rank + 15) / 16 * 16;
+    const u32 count = A.tokens - t0 < LIN_JOIN_TOKENS ? A.tokens - t0 : LIN_JOIN_TOKENS;
+    if (threadIdx.x < LIN_JOIN_TOKENS && rank) {
+        const int a = threadIdx.x < count ? A.adapter_of[t0 + threadIdx.x] : -1;
+        of[threadIdx.x] = a >= 0 && (u32)a < A.num_adapters ? a : -1;
+    }
+    const u64 bias = A.bias && i < A.m ? A.bias[i] : 0u;
+    pdl_wait();
+    __syncthreads();
+    if (rank) {
+        for (u32 k = threadIdx.x; k < count * pad; k += LIN_ROWS) {
+            const u32 t = k / pad, r = k - t * pad;
+            u32 v = 0;
+            if (of[t] >= 0 && r < rank) {
+                const u32 row = (u32)of[t] * rank + r;
+                v = p.a_rows ? red64(lin_sum(p, slots, p.wtiles + row / LIN_ROWS, t0 + t, row % LIN_ROWS)) : u_own[(size_t)(t0 + t) * rank + r];
+            }
+            lin_u[k] = v;
+        }
+        __syncthreads();
+    }
     if (i >= A.m) return;
-    u64 y = lin_sum(p, slots, t, i) + (A.bias ? A.bias[i] : 0);
-    const int of = u ? A.adapter_of[t] : -1;
-    if (of >= 0 && (u32)of < A.num_adapters)
-        for (u32 r = 0; r < A.rank; r++) y += mul31(A.b[((size_t)of * A.m + i) * A.rank + r], u[(size_t)t * A.rank + r]);
-    A.y[t * A.y_stride + i] = red64(y);
+    u64 y[LIN_JOIN_TOKENS];
+#pragma unroll
+    for (u32 t = 0; t < LIN_JOIN_TOKENS; t++) y[t] = t < count ? lin_sum(p, slots, mt, t0 + t, threadIdx.x) + bias : 0u;
+    for (u32 r0 = 0; r0 < rank; r0 += 16) {
+        u32 b[16];
+        int have = -1;
+#pragma unroll
+        for (u32 t = 0; t < LIN_JOIN_TOKENS; t++) {
+            if (t >= count || of[t] < 0) continue;
+            if (of[t] != have) {
+                have = of[t];
+                const u32* at = A.b + ((size_t)have * A.m + i) * rank + r0;
+                if (rank % 4 == 0 && !((uintptr_t)A.b & 15)) {
+#pragma unroll
+                    for (u32 k = 0; k < 4; k++) {
+                        const uint4 v = r0 + 4 * k < rank ? *reinterpret_cast<const uint4*>(at + 4 * k) : make_uint4(0, 0, 0, 0);
+                        b[4 * k] = v.x; b[4 * k + 1] = v.y; b[4 * k + 2] = v.z; b[4 * k + 3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (u32 k = 0; k < 16; k++) b[k] = r0 + k < rank ? at[k] : 0u;
+                }
+            }
+            const uint4* uv = reinterpret_cast<const uint4*>(lin_u + t * pad + r0);
+#pragma unroll
+            for (u32 k = 0; k < 4; k++) {
+                const uint4 v = uv[k];
+                const u32 w[4] = {v.x, v.y, v.z, v.w};
+                y[t] += lin_dot4(b + 4 * k, w);
+            }
+        }
+    }
+#pragma unroll
+    for (u32 t = 0; t < LIN_JOIN_TOKENS; t++)
+        if (t < count) A.y[(t0 + t) * A.y_stride + i] = red64(y[t]);
 }
 
-// u[t][r] = A[of[t]][r] . x[t]; a warp per (token, r).
-__global__ void __launch_bounds__(256) adapter_shrink_kernel(LinearArgs A, u32* __restrict__ u) {
-    const u32 w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (w >= A.tokens * A.rank) return;
-    const u32 t = w / A.rank, r = w - t * A.rank;
+// u[t][r] = A[of[t]][r] . x[t]; a CTA per (r, t).
+__global__ void __launch_bounds__(128) adapter_shrink_kernel(LinearArgs A, int vec, u32* __restrict__ u) {
+    __shared__ u32 part[4];
+    pdl_launch_dependents();
+    const u32 r = blockIdx.x, t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int of = A.adapter_of[t];
+    if (of < 0 || (u32)of >= A.num_adapters) return;      // nobody reads this token's
+    const u32* a = A.a + ((size_t)of * A.rank + r) * A.n;
+    const u32* x = A.x + t * A.x_stride;
     u64 acc = 0;
-    if (of >= 0 && (u32)of < A.num_adapters) {
-        const u32* a = A.a + ((size_t)of * A.rank + r) * A.n;
-        const u32* x = A.x + t * A.x_stride;
-        for (u32 j = lane; j < A.n; j += 32) acc += mul31(a[j], x[j]);
+    if (vec) {
+#pragma unroll 4
+        for (u32 j = threadIdx.x; j < A.n / 4; j += 128) {
+            const uint4 v = reinterpret_cast<const uint4*>(a)[j], w = reinterpret_cast<const uint4*>(x)[j];
+            const u32 p[4] = {v.x, v.y, v.z, v.w}, q[4] = {w.x, w.y, w.z, w.w};
+            acc += lin_dot4(p, q);
+        }
+    } else {
+#pragma unroll 4
+        for (u32 j = threadIdx.x; j < A.n; j += 128) acc += mul31(a[j], x[j]);
     }
     u32 s = red64(acc);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) s = add31(s, __shfl_xor_sync(0xffffffffu, s, off));
-    if (lane == 0) u[w] = s;
-}
-
-// A 32 x 32 tile of Y per CTA.
-__global__ void __launch_bounds__(256) adapter_linear_kernel(LinearArgs A, const u32* __restrict__ u) {
-    __shared__ u32 ws[32][33], xs[32][33];
-    const u32 i0 = blockIdx.x * 32, t0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    u64 acc[4] = {0, 0, 0, 0};
-    for (u32 j0 = 0; j0 < A.n; j0 += 32) {
-        for (u32 r = ty; r < 32; r += 8) {
-            ws[r][tx] = i0 + r < A.m && j0 + tx < A.n ? A.w[(size_t)(i0 + r) * A.n + j0 + tx] : 0;
-            xs[r][tx] = t0 + r < A.tokens && j0 + tx < A.n ? A.x[(t0 + r) * A.x_stride + j0 + tx] : 0;
-        }
-        __syncthreads();
-        for (u32 j = 0; j < 32; j++)
-            for (int k = 0; k < 4; k++) acc[k] += mul31(ws[tx][j], xs[ty + 8 * k][j]);
-        __syncthreads();
-    }
-    const u32 i = i0 + tx;
-    if (i >= A.m) return;
-    for (int k = 0; k < 4; k++) {
-        const u32 t = t0 + ty + 8 * k;
-        if (t >= A.tokens) continue;
-        u64 y = acc[k] + (A.bias ? A.bias[i] : 0);
-        const int of = u ? A.adapter_of[t] : -1;
-        if (of >= 0 && (u32)of < A.num_adapters)
-            for (u32 r = 0; r < A.rank; r++) y += mul31(A.b[((size_t)of * A.m + i) * A.rank + r], u[(size_t)t * A.rank + r]);
-        A.y[t * A.y_stride + i] = red64(y);
-    }
+    if (lane == 0) part[warp] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) u[(size_t)t * A.rank + r] = add31(add31(part[0], part[1]), add31(part[2], part[3]));
 }
 
 }  // namespace zkb

@@ -78,41 +78,79 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
 }
 
 static size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
+// Launch that, if `early`, may begin while the kernel before it is still running (see pdl_wait in m31.cuh): only behind a kernel of the same call, whose own
+// launch waited for all that came before.
+template <class... KArgs, class... Args>
+static cudaError_t launch_after(bool early, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = stream; cfg.attrs = at; cfg.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+// Where the parts of a call's workspace begin.
+struct LinSpace { size_t digits, slots, end; u32 chunk, a_rows; };
+static LinSpace lin_space(int sm_count, u32 tokens, u32 m, u32 n, u32 num_adapters, u32 rank) {
+    LinSpace w{};
+    w.chunk = lin_chunk(tokens, n);
+    w.a_rows = lin_a_rows(w.chunk, m, num_adapters, rank);
+    const LinPlan p = lin_plan(sm_count, w.chunk, m, n, w.a_rows);
+    w.digits = num_adapters && !w.a_rows ? round256((size_t)w.chunk * rank * 4) : 0;
+    w.slots = w.digits + round256(lin_digit_bytes(p));
+    w.end = w.slots + lin_slot_bytes(sm_count, p);
+    return w;
+}
 size_t adapter_linear_workspace(int sm_count, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank) {
-    if (!tokens) return 0;
-    const LinPlan p = lin_plan(sm_count, lin_chunk(tokens, n), m, n);
-    return round256((num_adapters ? (size_t)tokens * rank * 4 : 0)) + round256(lin_digit_bytes(p)) + lin_slot_bytes(p);
+    return tokens ? lin_space(sm_count, tokens, m, n, num_adapters, rank).end : 0;
+}
+template <bool W_COPY, bool X_FILL>
+static cudaError_t lin_product(cudaStream_t stream, bool early, const CUtensorMap& map_w, const CUtensorMap& map_a, const LinPlan& p, const LinearArgs& a, const unsigned char* digits,
+                               u32* slots) {
+    cudaError_t e = cudaFuncSetAttribute(linear_bytes_kernel<W_COPY, X_FILL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 201 * 1024);
+    if (e != cudaSuccess) return e;
+    const int x_vec = a.n % 4 == 0 && a.x_stride % 4 == 0 && !((uintptr_t)a.x & 15);
+    const dim3 block(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL));
+    const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+    return launch_after(early, linear_bytes_kernel<W_COPY, X_FILL>, dim3(p.ctas), block, smem, stream, map_w, map_a, p, a, x_vec, digits, slots);
 }
 cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const LinearArgs& a, int* launches) {
-    u32* u = a.num_adapters ? (u32*)a.workspace : nullptr;
-    if (u) {
-        adapter_shrink_kernel<<<(a.tokens * a.rank + 7) / 8, 256, 0, stream>>>(a, u);
-        ++*launches;
+    const LinSpace space = lin_space(sm_count, a.tokens, a.m, a.n, a.num_adapters, a.rank);
+    u32* u = (u32*)a.workspace;
+    unsigned char* digits = (unsigned char*)a.workspace + space.digits;
+    u32* slots = (u32*)((unsigned char*)a.workspace + space.slots);
+    const bool copies = a.n % 4 == 0 && !((uintptr_t)a.w & 15) && !(space.a_rows && ((uintptr_t)a.a & 15));
+    CUtensorMap map_w = {}, map_a = {};
+    cudaError_t e = cudaSuccess;
+    if (copies) {
+        if ((e = rows_tensor_map(&map_w, a.w, a.m, a.n)) != cudaSuccess) return e;
+        if (space.a_rows && (e = rows_tensor_map(&map_a, a.a, space.a_rows, a.n)) != cudaSuccess) return e;
     }
-    if (a.n % 4 || ((uintptr_t)a.w & 15) || a.tokens < 5) {
-        adapter_linear_kernel<<<dim3((a.m + 31) / 32, (a.tokens + 31) / 32), 256, 0, stream>>>(a, u);
-        ++*launches;
-        return cudaGetLastError();
-    }
-    CUtensorMap map;
-    cudaError_t e = rows_tensor_map(&map, a.w, a.m, a.n);
-    if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(linear_bytes_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 201 * 1024);
-    if (e != cudaSuccess) return e;
-    const u32 chunk = lin_chunk(a.tokens, a.n);
-    unsigned char* digits = (unsigned char*)a.workspace + round256(u ? (size_t)a.tokens * a.rank * 4 : 0);
-    u32* slots = (u32*)(digits + round256(lin_digit_bytes(lin_plan(sm_count, chunk, a.m, a.n))));
-    for (u32 t0 = 0; t0 < a.tokens; t0 += chunk) {
+    for (u32 t0 = 0; t0 < a.tokens; t0 += space.chunk) {
         LinearArgs c = a;
-        c.tokens = a.tokens - t0 < chunk ? a.tokens - t0 : chunk;
+        c.tokens = a.tokens - t0 < space.chunk ? a.tokens - t0 : space.chunk;
         c.x += t0 * a.x_stride;
         c.y += t0 * a.y_stride;
-        if (u) c.adapter_of += t0;
-        const LinPlan p = lin_plan(sm_count, c.tokens, a.m, a.n);
-        linear_digits_kernel<<<dim3(p.steps, p.ntiles), 8 * p.tt, 0, stream>>>(c.x, c.x_stride, p, digits);
-        linear_bytes_kernel<<<p.ctas, LIN_THREADS, (size_t)p.stages * p.stage_bytes + 1024, stream>>>(map, p, digits, slots, a.gave_up);
-        linear_join_kernel<<<dim3((a.m + 255) / 256, c.tokens), 256, 0, stream>>>(c, p, slots, u ? u + (size_t)t0 * a.rank : nullptr);
-        *launches += 3;
+        if (a.rank) c.adapter_of += t0;
+        const LinPlan p = lin_plan(sm_count, c.tokens, a.m, a.n, space.a_rows);
+        if (a.rank && !space.a_rows) {
+            const int vec = a.n % 4 == 0 && a.x_stride % 4 == 0 && !((uintptr_t)a.x & 15) && !((uintptr_t)a.a & 15);
+            adapter_shrink_kernel<<<dim3(a.rank, c.tokens), 128, 0, stream>>>(c, vec, u);
+            ++*launches;
+        }
+        const bool fused = lin_fused(p), early = !fused || (a.rank && !space.a_rows);
+        if (!fused) {
+            linear_digits_kernel<<<dim3(p.steps, p.ntiles), 8 * p.tt, 0, stream>>>(c.x, c.x_stride, p, digits);
+            ++*launches;
+        }
+        if (copies) e = fused ? lin_product<true, true>(stream, early, map_w, map_a, p, c, digits, slots) : lin_product<true, false>(stream, early, map_w, map_a, p, c, digits, slots);
+        else e = fused ? lin_product<false, true>(stream, early, map_w, map_a, p, c, digits, slots) : lin_product<false, false>(stream, early, map_w, map_a, p, c, digits, slots);
+        if (e != cudaSuccess) return e;
+        e = launch_after(true, linear_join_kernel, dim3(p.wtiles, (c.tokens + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS), dim3(LIN_ROWS),
+                         (size_t)LIN_JOIN_TOKENS * ((a.rank + 15) / 16 * 16) * 4, stream, c, p, slots, u);
+        if (e != cudaSuccess) return e;
+        *launches += 2;
     }
     return cudaGetLastError();
 }
