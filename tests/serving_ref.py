@@ -100,3 +100,10 @@ def linear(x, w, bias=None, a=None, b=None, of=None):
             u = (a[of[t]].astype(np.int64) * x[t] % P).sum(1) % P
             y[t] += (b[of[t]].astype(np.int64) * u % P).sum(1)
     return y % P
+
+
+def linear_wide(x, w):
+    """The same product by halves of 16 bits, whose sums of products are exact in 64-bit floats (below 2^53 for less than 2^20 columns)."""
+    x0, x1, w0, w1 = ((v & 0xffff).astype(np.float64) if low else (v >> 16).astype(np.float64) for v in (x, w) for low in (True, False))
+    part = lambda a, b: (a @ b.T).astype(np.int64) % P
+    return (part(x0, w0) + (part(x0, w1) + part(x1, w0)) * 65536 + part(x1, w1) * 2) % P

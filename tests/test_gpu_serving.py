@@ -386,6 +386,21 @@ def test_linear_every_value_at_its_largest(ctx, t):
         check_linear(ctx, x, w)
 
 
+@pytest.mark.parametrize("t", [1, 12, 30, 36, 48, 61, 64, 100])
+@pytest.mark.parametrize("m,n", [(6000, 2048), (5000, 2051), (300, 20000)])
+def test_linear_many_steps(ctx, t, m, n):
+    """Matrices of many more steps than a ring has stages, whose stretches end inside tiles; called again and again without waiting in between."""
+    rng = np.random.default_rng(t)
+    x, w = field(rng, t, n), field(rng, m, n)
+    x_dev, w_dev, outs = ctx.upload(x), ctx.upload(w), [ctx.upload(np.zeros(t * m, np.uint32)) for _ in range(4)]
+    for out in outs:
+        zs.adapter_linear(ctx, x_dev, w_dev, t, m, n, out)
+    want = R.linear_wide(x, w)
+    for out in outs:
+        assert np.array_equal(out.download().reshape(t, m), want)
+    ctx.sync()                                              # raises if a wait inside a kernel ran out
+
+
 @pytest.mark.parametrize("t", [1, 20, 150])
 def test_linear_strided_rows(ctx, t):
     rng = np.random.default_rng(t)

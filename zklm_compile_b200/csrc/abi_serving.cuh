@@ -154,6 +154,7 @@ static void adapter_linear_dims(uint32_t tokens, uint32_t m, uint32_t n, uint32_
     if (!m || !n) throw ArgFail{ZKB_E_ARG, "adapter_linear: empty dimension"};
     if (num_adapters && !rank) throw ArgFail{ZKB_E_ARG, "adapter_linear: adapters of rank 0"};
     if (m > (1u << 24) || n > (1u << 24) || tokens > (1u << 20) || rank > 1024) throw ArgFail{ZKB_E_TOO_LARGE, "adapter_linear: more than 2^24 rows or columns, 2^20 tokens or rank 1024"};
+    if (!adapter_linear_fits(tokens, m, n, num_adapters, rank)) throw ArgFail{ZKB_E_TOO_LARGE, "adapter_linear: W has more than 2^40 elements"};
 }
 size_t zkb_adapter_linear_workspace(zkb_ctx* c, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank) {
     if (!c) return 0;

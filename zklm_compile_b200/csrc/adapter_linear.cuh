@@ -21,7 +21,6 @@ constexpr u32 LIN_SEG = 256;                   // steps after which the accumula
 constexpr u32 LIN_TOKENS = 64;                 // tokens per tile at most: 256 columns of an accumulator
 constexpr u32 LIN_MAX_STAGES = 8;
 constexpr u32 LIN_FILL = 128;                  // threads that fill operands by plain stores, where a kernel has such
-constexpr u32 LIN_JOIN_TOKENS = 8;
 
 // Byte c of the four rotations of x by 8i, i = 0 .. 3, for c = 0 .. 3.  All of them are bytes of x, of x >> 7, or of x without the top bits of its bytes.
 __device__ __forceinline__ void digit_words(u32 x, u32 (&w)[4]) {
@@ -35,8 +34,7 @@ __device__ __forceinline__ void digit_words(u32 x, u32 (&w)[4]) {
 // How a product is cut: `tiles` of LIN_ROWS rows x `tt` tokens, each `steps` deep in `segs` segments.  Tiles' steps lie one behind the other and every CTA takes `per`
 // of them, so all CTAs finish together; a CTA leaves its sum over each stretch of one tile's segment in slot (CTA + tile * segs + segment), which are all different.
 struct LinPlan {
-    u32 tokens, m, n, a_rows, tt, ntiles, mtiles, wtiles, steps, segs, per, ctas, stages, stage_bytes, tmem_cols;   // tiles: wtiles of W, then those of the adapters' A
-    u64 total;
+    u32 tokens, m, n, a_rows, tt, ntiles, mtiles, wtiles, steps, segs, per, ctas, stages, stage_bytes, tmem_cols, total;   // tiles: wtiles of W, then those of the adapters' A
     size_t slot_words;
 };
 inline LinPlan lin_plan(int sm_count, u32 tokens, u32 m, u32 n, u32 a_rows) {
@@ -48,15 +46,19 @@ inline LinPlan lin_plan(int sm_count, u32 tokens, u32 m, u32 n, u32 a_rows) {
     p.mtiles = p.wtiles + (a_rows + LIN_ROWS - 1) / LIN_ROWS;
     p.steps = (n + LIN_STEP - 1) / LIN_STEP;
     p.segs = (p.steps + LIN_SEG - 1) / LIN_SEG;
-    p.total = (u64)p.mtiles * p.ntiles * p.steps;
-    p.per = (u32)((p.total + sm_count - 1) / sm_count);
-    p.ctas = (u32)((p.total + p.per - 1) / p.per);
+    p.total = p.mtiles * p.ntiles * p.steps;                  // below 2^32: lin_fits
+    p.per = (p.total + sm_count - 1) / sm_count;
+    p.ctas = (p.total + p.per - 1) / p.per;
     p.stage_bytes = LIN_ROWS * 128 + (4 * p.tt * 128 + 1023) / 1024 * 1024;
     p.stages = 200 * 1024 / p.stage_bytes < LIN_MAX_STAGES ? 200 * 1024 / p.stage_bytes : LIN_MAX_STAGES;
     p.tmem_cols = 32;
     while (p.tmem_cols < 8 * p.tt) p.tmem_cols *= 2;
     p.slot_words = (size_t)p.tt * LIN_ROWS;
     return p;
+}
+// Whether the steps of one pass can be counted in 31 bits (2^40 products of W's elements and tokens would not).
+inline bool lin_fits(u32 tokens, u32 m, u32 n, u32 a_rows) {
+    return ((u64)((m + LIN_ROWS - 1) / LIN_ROWS) + (a_rows + LIN_ROWS - 1) / LIN_ROWS) * ((tokens + LIN_TOKENS - 1) / LIN_TOKENS) * ((n + LIN_STEP - 1) / LIN_STEP) < (1ull << 31);
 }
 // Rows of A that the product takes along with W's (all adapters for all tokens), or 0: then each token's own rank products are made apart.
 // Along, an adapter's rows are read once however many tokens use it and no launch is added; apart, no adapter that no token has is read.
@@ -99,15 +101,15 @@ __global__ void __launch_bounds__(512) linear_digits_kernel(const u32* __restric
 
 struct LinWalk {                               // a CTA's stretches, the same for every role
     const LinPlan& p;
-    u64 at, end;
-    __device__ LinWalk(const LinPlan& plan) : p(plan), at((u64)blockIdx.x * plan.per), end(at + plan.per < plan.total ? at + plan.per : plan.total) {}
+    u32 at, end;
+    __device__ LinWalk(const LinPlan& plan) : p(plan), at(blockIdx.x * plan.per), end(plan.total - at > plan.per ? at + plan.per : plan.total) {}
     u32 mt, nt, first, count, slot;
     __device__ bool next() {
         if (at >= end) return false;
-        const u32 tile = (u32)(at / p.steps);
-        first = (u32)(at - (u64)tile * p.steps);
+        const u32 tile = at / p.steps;
+        first = at - tile * p.steps;
         const u32 seg = first / LIN_SEG, seg_end = (seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps;
-        count = end - at < seg_end - first ? (u32)(end - at) : seg_end - first;
+        count = end - at < seg_end - first ? end - at : seg_end - first;
         mt = tile / p.ntiles;
         nt = tile - mt * p.ntiles;
         slot = blockIdx.x + tile * p.segs + seg;
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
     const u32 base = smem_addr(smem);
     const u32 full = smem_addr(bars), empty = full + 8 * LIN_MAX_STAGES, acc_full = empty + 8 * LIN_MAX_STAGES, acc_empty = acc_full + 8;
     if (threadIdx.x == 0) {
-        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, FILL ? 1 + LIN_FILL / 32 : 1); mbar_init(empty + 8 * s, 1); }
+        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, FILL ? 2 : 1); mbar_init(empty + 8 * s, 1); }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 4);
         gave_up = 0;
@@ -230,86 +232,73 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
             n++;
         }
     } else if (FILL) {
-        const u32 tid = threadIdx.x - 192;
-        u32 it = 0, late = 0;                    // late: a step whose words of W are still on their way
+        // Each warp takes every fourth step, so that four steps' loads are under way - but no more warps than stages: a warp knows that the stage of its last
+        // step was empty, and from that that its next one's was emptied the time before last; with fewer stages than warps it could be two phases ahead, where
+        // a wait by parity sees the wrong one.
+        const u32 fillers = p.stages < LIN_FILL / 32 ? p.stages : LIN_FILL / 32;
+        u32 it = 0;
         bool ok = true;
-        u32 x[4][4];
-        // the thread's groups of four values of x: token (tid + 128 i) / 8, columns 4 (tid & 7) .. of the step
-        auto fetch = [&](u32 step) {
-#pragma unroll
-            for (u32 i = 0; i < 4; i++) {
-                const u32 t = (tid >> 3) + 16 * i, j = step * LIN_STEP + 4 * (tid & 7);
-                const u32* at = A.x + t * A.x_stride + j;
-                if (x_vec && t < p.tokens && j + 4 <= p.n) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at);
-                    x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
-                } else {
-#pragma unroll
-                    for (u32 e = 0; e < 4; e++) x[i][e] = t < p.tokens && j + e < p.n ? at[e] : 0u;
-                }
-            }
-        };
-        auto signal = [&](u32 step_it) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * (step_it % p.stages));
-        };
-        bool more = walk.next();
-        u32 k = 0;
-        if (X_FILL && more) fetch(walk.first);
-        while (more && ok) {
-            const u32 s = it % p.stages, round = it / p.stages, step = walk.first + k;
+        while (ok && walk.next()) {
             const bool of_w = walk.mt < p.wtiles;
-            const u32 row0 = (of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS, rows = (of_w ? p.m : p.a_rows) - row0;
-            unsigned char* st = smem + s * p.stage_bytes;
-            if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
-            if (!W_COPY) {
-                const u32 j = step * LIN_STEP + lane, most = rows < LIN_ROWS ? rows : LIN_ROWS;
-                const u32* src = (of_w ? A.w : A.a) + (size_t)row0 * p.n + j;
-                for (u32 r = warp - 6; r < most; r += LIN_FILL / 32) {
-                    const u32 to = smem_addr(st) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
-                    // past the end of a row nothing is read and zero is stored
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(j < p.n ? src + (size_t)r * p.n : A.w), "r"(j < p.n ? 4 : 0) : "memory");
+            const u32 row0 = (of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS, rows = (of_w ? p.m : p.a_rows) - row0, most = rows < LIN_ROWS ? rows : LIN_ROWS;
+            for (u32 k = 0; k < walk.count; k++, it++) {
+                if (it % fillers != warp - 6) continue;
+                const u32 s = it % p.stages, round = it / p.stages, step = walk.first + k;
+                unsigned char* st = smem + s * p.stage_bytes;
+                if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
+                if (!W_COPY) {
+                    const u32 j = step * LIN_STEP + lane, bytes = j < p.n ? 4 : 0;      // past the end of a row nothing is read and zero is stored
+                    const u32* src = bytes ? (of_w ? A.w : A.a) + (size_t)row0 * p.n + j : A.w;
+                    const size_t next = bytes ? p.n : 0;
+                    const u32 to = smem_addr(st) + (lane & 3) * 4;
+#pragma unroll 8
+                    for (u32 r = 0; r < most; r++, src += next)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-            if (X_FILL) {
+                if (X_FILL) {
+                    // groups of four values of x: token (lane + 32 i) / 8, columns 4 (lane & 7) .. of the step
+                    const u32 q = lane & 7, j = step * LIN_STEP + 4 * q;
+                    for (u32 tok0 = 0; tok0 < p.tt; tok0 += 16) {
+                        u32 x[4][4];
 #pragma unroll
-                for (u32 i = 0; i < 4; i++) {
-                    const u32 tok = (tid >> 3) + 16 * i, q = tid & 7;
-                    if (tok >= p.tt) break;
-                    u32 w[4][4];
+                        for (u32 i = 0; i < 4; i++) {
+                            const u32 t = tok0 + 4 * i + (lane >> 3);
+                            const u32* at = A.x + t * A.x_stride + j;
+                            if (x_vec && t < p.tokens && j + 4 <= p.n) {
+                                const uint4 v = *reinterpret_cast<const uint4*>(at);
+                                x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+                            } else {
 #pragma unroll
-                    for (u32 e = 0; e < 4; e++) {
-                        u32 d[4];
-                        digit_words(x[i][e], d);
+                                for (u32 e = 0; e < 4; e++) x[i][e] = t < p.tokens && j + e < p.n ? at[e] : 0u;
+                            }
+                        }
 #pragma unroll
-                        for (int c = 0; c < 4; c++) w[c][e] = d[c];
+                        for (u32 i = 0; i < 4; i++) {
+                            const u32 t = tok0 + 4 * i + (lane >> 3);
+                            if (t >= p.tt) break;
+                            u32 w[4][4];
+#pragma unroll
+                            for (u32 e = 0; e < 4; e++) {
+                                u32 d[4];
+                                digit_words(x[i][e], d);
+#pragma unroll
+                                for (int c = 0; c < 4; c++) w[c][e] = d[c];
+                            }
+#pragma unroll
+                            for (u32 c = 0; c < 4; c++) {
+                                const u32 r = 4 * t + c;
+                                *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+                            }
+                        }
                     }
-#pragma unroll
-                    for (u32 c = 0; c < 4; c++) {
-                        const u32 r = 4 * tok + c;
-                        *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
-                    }
                 }
+                if (!W_COPY) asm volatile("cp.async.wait_all;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + 8 * s);
             }
-            if (++k == walk.count) { more = walk.next(); k = 0; }
-            if (X_FILL && more) fetch(walk.first + k);
-            if (W_COPY) {
-                signal(it);
-            } else {
-                if (late) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    signal(it - 1);
-                }
-                late = 1;
-            }
-            it++;
         }
-        if (!W_COPY) {
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            if (late && ok) signal(it - 1);
-        }
+        if (!W_COPY) asm volatile("cp.async.wait_all;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -318,86 +307,86 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
     if (threadIdx.x == 0 && gave_up) *A.gave_up = 1;
 }
 
-// Sum of one output's slots (see LinPlan): row i of tile mt, token t.
-__device__ __forceinline__ u64 lin_sum(const LinPlan& p, const u32* __restrict__ slots, u32 mt, u32 t, u32 row) {
-    const u32 nt = t / p.tt, tile = mt * p.ntiles + nt;
-    const size_t in = (size_t)(t - nt * p.tt) * LIN_ROWS + row;
-    const u64 begin = (u64)tile * p.steps;
-    u64 s = 0;
+// Sums of slots (see LinPlan): row `row` of tile mt, tokens t, t + step, ... of one tile of tokens; those from `end` on are left out.
+template <int N>
+__device__ __forceinline__ void lin_sums(const LinPlan& p, const u32* __restrict__ slots, u32 mt, u32 nt, u32 row, u32 t, u32 step, u32 end, u64 (&y)[N]) {
+    const u32 tile = mt * p.ntiles + nt, begin = tile * p.steps;
+    const u32* at = slots + (size_t)(t - nt * p.tt) * LIN_ROWS + row;
     for (u32 seg = 0; seg < p.segs; seg++) {
-        const u64 b = begin + seg * LIN_SEG, e = begin + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps);
-        const u32 last = (u32)((e - 1) / p.per);
-        for (u32 c = (u32)(b / p.per); c <= last; c++) s += slots[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words + in];
+        const u32 b = begin + seg * LIN_SEG, e = begin + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps), last = (e - 1) / p.per;
+#pragma unroll 4
+        for (u32 c = b / p.per; c <= last; c++) {
+            const u32* s = at + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words;
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (t + k * step < end) y[k] += s[(size_t)k * step * LIN_ROWS];
+        }
     }
-    return s;
 }
 // Four products of field elements fit 64 bits.
 __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
     const u64 s = (u64)a[0] * b[0] + (u64)a[1] * b[1] + (u64)a[2] * b[2] + (u64)a[3] * b[3];
     return (s & ZKB_P) + (s >> 31);
 }
-// One CTA: a tile's 256 rows, LIN_JOIN_TOKENS tokens.  The rows of B that a thread needs stay in registers, 16 values at a time, while tokens beside each
-// other have the same adapter.
-__global__ void __launch_bounds__(LIN_ROWS) linear_join_kernel(LinearArgs A, LinPlan p, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
-    extern __shared__ __align__(16) u32 lin_u[];         // [LIN_JOIN_TOKENS][rank rounded up to 16]
+// One CTA: 64 rows, up to 16 tokens of a tile of tokens, four of them a thread.  The adapters' B goes through shared memory 32 of its columns at a
+// time, once for all tokens beside each other that have the same one.
+constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 32;
+__global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan p, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
+    __shared__ __align__(16) u32 u[LIN_JOIN_TOKENS][LIN_JOIN_RANK], b[LIN_JOIN_ROWS][LIN_JOIN_RANK + 4];
     __shared__ int of[LIN_JOIN_TOKENS];
-    const u32 mt = blockIdx.x, t0 = blockIdx.y * LIN_JOIN_TOKENS, i = mt * LIN_ROWS + threadIdx.x, rank = A.rank, pad = (rank + 15) / 16 * 16;
-    const u32 count = A.tokens - t0 < LIN_JOIN_TOKENS ? A.tokens - t0 : LIN_JOIN_TOKENS;
+    const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS, nt = blockIdx.y / groups, t0 = nt * p.tt + (blockIdx.y - nt * groups) * LIN_JOIN_TOKENS;
+    const u32 tile_end = (nt + 1) * p.tt < p.tokens ? (nt + 1) * p.tt : p.tokens, end = t0 + LIN_JOIN_TOKENS < tile_end ? t0 + LIN_JOIN_TOKENS : tile_end;
+    if (t0 >= end) return;
+    const u32 i0 = blockIdx.x * LIN_JOIN_ROWS, in = threadIdx.x & (LIN_JOIN_ROWS - 1), i = i0 + in, mine = t0 + (threadIdx.x >> 6), rank = A.rank;
     if (threadIdx.x < LIN_JOIN_TOKENS && rank) {
-        const int a = threadIdx.x < count ? A.adapter_of[t0 + threadIdx.x] : -1;
+        const int a = t0 + threadIdx.x < end ? A.adapter_of[t0 + threadIdx.x] : -1;
         of[threadIdx.x] = a >= 0 && (u32)a < A.num_adapters ? a : -1;
     }
     const u64 bias = A.bias && i < A.m ? A.bias[i] : 0u;
+    u64 y[4] = {bias, bias, bias, bias};
     pdl_wait();
-    __syncthreads();
-    if (rank) {
-        for (u32 k = threadIdx.x; k < count * pad; k += LIN_ROWS) {
-            const u32 t = k / pad, r = k - t * pad;
-            u32 v = 0;
-            if (of[t] >= 0 && r < rank) {
-                const u32 row = (u32)of[t] * rank + r;
-                v = p.a_rows ? red64(lin_sum(p, slots, p.wtiles + row / LIN_ROWS, t0 + t, row % LIN_ROWS)) : u_own[(size_t)(t0 + t) * rank + r];
-            }
-            lin_u[k] = v;
-        }
+    if (i < A.m) lin_sums(p, slots, i / LIN_ROWS, nt, i % LIN_ROWS, mine, 4, end, y);
+    for (u32 r0 = 0; r0 < rank; r0 += LIN_JOIN_RANK) {
         __syncthreads();
-    }
-    if (i >= A.m) return;
-    u64 y[LIN_JOIN_TOKENS];
+        for (u32 k = threadIdx.x; k < LIN_JOIN_TOKENS * LIN_JOIN_RANK; k += 256) {
+            const u32 t = k / LIN_JOIN_RANK, r = r0 + k % LIN_JOIN_RANK;
+            u64 v[1] = {0};
+            if (r < rank && of[t] >= 0) {
+                const u32 row = (u32)of[t] * rank + r;
+                if (p.a_rows) lin_sums(p, slots, p.wtiles + row / LIN_ROWS, nt, row % LIN_ROWS, t0 + t, 1, end, v);
+                else v[0] = u_own[(size_t)(t0 + t) * rank + r];
+            }
+            u[t][k % LIN_JOIN_RANK] = red64(v[0]);
+        }
+        for (u32 first = 0; first < end - t0;) {               // tokens first .. until - 1 have the same adapter, or none
+            u32 until = first + 1;
+            while (until < end - t0 && of[until] == of[first]) until++;
+            if (of[first] >= 0) {
+                __syncthreads();
+                const u32* from = A.b + ((size_t)of[first] * A.m + i0) * rank + r0;
+                for (u32 k = threadIdx.x; k < LIN_JOIN_ROWS * LIN_JOIN_RANK; k += 256) {
+                    const u32 row = k / LIN_JOIN_RANK, r = k % LIN_JOIN_RANK;
+                    b[row][r] = i0 + row < A.m && r0 + r < rank ? from[(size_t)row * rank + r] : 0u;
+                }
+                __syncthreads();
 #pragma unroll
-    for (u32 t = 0; t < LIN_JOIN_TOKENS; t++) y[t] = t < count ? lin_sum(p, slots, mt, t0 + t, threadIdx.x) + bias : 0u;
-    for (u32 r0 = 0; r0 < rank; r0 += 16) {
-        u32 b[16];
-        int have = -1;
+                for (u32 k = 0; k < 4; k++) {
+                    const u32 t = (threadIdx.x >> 6) + 4 * k;
+                    if (t < first || t >= until) continue;
 #pragma unroll
-        for (u32 t = 0; t < LIN_JOIN_TOKENS; t++) {
-            if (t >= count || of[t] < 0) continue;
-            if (of[t] != have) {
-                have = of[t];
-                const u32* at = A.b + ((size_t)have * A.m + i) * rank + r0;
-                if (rank % 4 == 0 && !((uintptr_t)A.b & 15)) {
-#pragma unroll
-                    for (u32 k = 0; k < 4; k++) {
-                        const uint4 v = r0 + 4 * k < rank ? *reinterpret_cast<const uint4*>(at + 4 * k) : make_uint4(0, 0, 0, 0);
-                        b[4 * k] = v.x; b[4 * k + 1] = v.y; b[4 * k + 2] = v.z; b[4 * k + 3] = v.w;
+                    for (u32 c = 0; c < LIN_JOIN_RANK; c += 4) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(&b[in][c]), w = *reinterpret_cast<const uint4*>(&u[t][c]);
+                        const u32 pv[4] = {v.x, v.y, v.z, v.w}, pw[4] = {w.x, w.y, w.z, w.w};
+                        y[k] += lin_dot4(pv, pw);
                     }
-                } else {
-#pragma unroll
-                    for (u32 k = 0; k < 16; k++) b[k] = r0 + k < rank ? at[k] : 0u;
                 }
             }
-            const uint4* uv = reinterpret_cast<const uint4*>(lin_u + t * pad + r0);
-#pragma unroll
-            for (u32 k = 0; k < 4; k++) {
-                const uint4 v = uv[k];
-                const u32 w[4] = {v.x, v.y, v.z, v.w};
-                y[t] += lin_dot4(b + 4 * k, w);
-            }
+            first = until;
         }
     }
 #pragma unroll
-    for (u32 t = 0; t < LIN_JOIN_TOKENS; t++)
-        if (t < count) A.y[(t0 + t) * A.y_stride + i] = red64(y[t]);
+    for (u32 k = 0; k < 4; k++)
+        if (i < A.m && mine + 4 * k < end) A.y[(mine + 4 * k) * A.y_stride + i] = red64(y[k]);
 }
 
 // u[t][r] = A[of[t]][r] . x[t]; a CTA per (r, t).

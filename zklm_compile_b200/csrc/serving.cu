@@ -102,6 +102,10 @@ static LinSpace lin_space(int sm_count, u32 tokens, u32 m, u32 n, u32 num_adapte
     w.end = w.slots + lin_slot_bytes(sm_count, p);
     return w;
 }
+bool adapter_linear_fits(uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank) {
+    const u32 chunk = lin_chunk(tokens, n);
+    return lin_fits(chunk, m, n, lin_a_rows(chunk, m, num_adapters, rank));
+}
 size_t adapter_linear_workspace(int sm_count, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank) {
     return tokens ? lin_space(sm_count, tokens, m, n, num_adapters, rank).end : 0;
 }
@@ -147,8 +151,8 @@ cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const Linea
         if (copies) e = fused ? lin_product<true, true>(stream, early, map_w, map_a, p, c, digits, slots) : lin_product<true, false>(stream, early, map_w, map_a, p, c, digits, slots);
         else e = fused ? lin_product<false, true>(stream, early, map_w, map_a, p, c, digits, slots) : lin_product<false, false>(stream, early, map_w, map_a, p, c, digits, slots);
         if (e != cudaSuccess) return e;
-        e = launch_after(true, linear_join_kernel, dim3(p.wtiles, (c.tokens + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS), dim3(LIN_ROWS),
-                         (size_t)LIN_JOIN_TOKENS * ((a.rank + 15) / 16 * 16) * 4, stream, c, p, slots, u);
+        const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS;
+        e = launch_after(true, linear_join_kernel, dim3((a.m + LIN_JOIN_ROWS - 1) / LIN_JOIN_ROWS, p.ntiles * groups), dim3(256), 0, stream, c, p, slots, u);
         if (e != cudaSuccess) return e;
         *launches += 2;
     }

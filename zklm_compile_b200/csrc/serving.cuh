@@ -61,6 +61,7 @@ struct LinearArgs {
     void* workspace;
     int* gave_up;                                            // as above
 };
+bool adapter_linear_fits(uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank);
 size_t adapter_linear_workspace(int sm_count, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank);
 cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const LinearArgs& a, int* launches);
 
