@@ -236,6 +236,28 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
         // step was empty, and from that that its next one's was emptied the time before last; with fewer stages than warps it could be two phases ahead, where
         // a wait by parity sees the wrong one.
         const u32 fillers = p.stages < LIN_FILL / 32 ? p.stages : LIN_FILL / 32;
+        // A warp's groups of four values of x, fetched a turn ahead: token 4 i + lane / 8, columns 4 (lane & 7) .. of its next step.  A step's columns of x
+        // are the same whatever tile it belongs to.
+        u32 x[X_FILL ? LIN_TOKENS / 4 : 1][4];
+        u32 ahead = blockIdx.x * p.per + (warp - 6);
+        auto fetch = [&] {
+            if (!X_FILL || ahead >= walk.end) return;
+            const u32 j = ahead % p.steps * LIN_STEP + 4 * (lane & 7);
+#pragma unroll
+            for (u32 i = 0; i < LIN_TOKENS / 4; i++) {
+                if (4 * i >= p.tt) break;
+                const u32 t = 4 * i + (lane >> 3);
+                const u32* at = A.x + t * A.x_stride + j;
+                if (x_vec && t < p.tokens && j + 4 <= p.n) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(at);
+                    x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+                } else {
+#pragma unroll
+                    for (u32 e = 0; e < 4; e++) x[i][e] = t < p.tokens && j + e < p.n ? at[e] : 0u;
+                }
+            }
+        };
+        if (warp - 6 < fillers) fetch();
         u32 it = 0;
         bool ok = true;
         while (ok && walk.next()) {
@@ -256,41 +278,26 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
                         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
                 }
                 if (X_FILL) {
-                    // groups of four values of x: token (lane + 32 i) / 8, columns 4 (lane & 7) .. of the step
-                    const u32 q = lane & 7, j = step * LIN_STEP + 4 * q;
-                    for (u32 tok0 = 0; tok0 < p.tt; tok0 += 16) {
-                        u32 x[4][4];
 #pragma unroll
-                        for (u32 i = 0; i < 4; i++) {
-                            const u32 t = tok0 + 4 * i + (lane >> 3);
-                            const u32* at = A.x + t * A.x_stride + j;
-                            if (x_vec && t < p.tokens && j + 4 <= p.n) {
-                                const uint4 v = *reinterpret_cast<const uint4*>(at);
-                                x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
-                            } else {
+                    for (u32 i = 0; i < LIN_TOKENS / 4; i++) {
+                        if (4 * i >= p.tt) break;
+                        const u32 t = 4 * i + (lane >> 3), q = lane & 7;
+                        u32 w[4][4];
 #pragma unroll
-                                for (u32 e = 0; e < 4; e++) x[i][e] = t < p.tokens && j + e < p.n ? at[e] : 0u;
-                            }
+                        for (u32 e = 0; e < 4; e++) {
+                            u32 d[4];
+                            digit_words(x[i][e], d);
+#pragma unroll
+                            for (int c = 0; c < 4; c++) w[c][e] = d[c];
                         }
 #pragma unroll
-                        for (u32 i = 0; i < 4; i++) {
-                            const u32 t = tok0 + 4 * i + (lane >> 3);
-                            if (t >= p.tt) break;
-                            u32 w[4][4];
-#pragma unroll
-                            for (u32 e = 0; e < 4; e++) {
-                                u32 d[4];
-                                digit_words(x[i][e], d);
-#pragma unroll
-                                for (int c = 0; c < 4; c++) w[c][e] = d[c];
-                            }
-#pragma unroll
-                            for (u32 c = 0; c < 4; c++) {
-                                const u32 r = 4 * t + c;
-                                *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
-                            }
+                        for (u32 c = 0; c < 4; c++) {
+                            const u32 r = 4 * t + c;
+                            *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
                         }
                     }
+                    ahead += fillers;
+                    fetch();
                 }
                 if (!W_COPY) asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -307,21 +314,10 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
     if (threadIdx.x == 0 && gave_up) *A.gave_up = 1;
 }
 
-// Sums of slots (see LinPlan): row `row` of tile mt, tokens t, t + step, ... of one tile of tokens; those from `end` on are left out.
-template <int N>
-__device__ __forceinline__ void lin_sums(const LinPlan& p, const u32* __restrict__ slots, u32 mt, u32 nt, u32 row, u32 t, u32 step, u32 end, u64 (&y)[N]) {
-    const u32 tile = mt * p.ntiles + nt, begin = tile * p.steps;
-    const u32* at = slots + (size_t)(t - nt * p.tt) * LIN_ROWS + row;
-    for (u32 seg = 0; seg < p.segs; seg++) {
-        const u32 b = begin + seg * LIN_SEG, e = begin + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps), last = (e - 1) / p.per;
-#pragma unroll 4
-        for (u32 c = b / p.per; c <= last; c++) {
-            const u32* s = at + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words;
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                if (t + k * step < end) y[k] += s[(size_t)k * step * LIN_ROWS];
-        }
-    }
+// The slots that hold a tile (see LinPlan): segment seg's are c + tile * segs + seg for c from lin_first to lin_last.
+__device__ __forceinline__ u32 lin_first(const LinPlan& p, u32 tile, u32 seg) { return (tile * p.steps + seg * LIN_SEG) / p.per; }
+__device__ __forceinline__ u32 lin_last(const LinPlan& p, u32 tile, u32 seg) {
+    return (tile * p.steps + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps) - 1) / p.per;
 }
 // Four products of field elements fit 64 bits.
 __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
@@ -329,64 +325,117 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
     return (s & ZKB_P) + (s >> 31);
 }
 // One CTA: 64 rows, up to 16 tokens of a tile of tokens, four of them a thread.  The adapters' B goes through shared memory 32 of its columns at a
-// time, once for all tokens beside each other that have the same one.
-constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 32;
+// time, once for all tokens beside each other that have the same one, for up to four adapters together.
+constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 32, LIN_JOIN_RUNS = 4;
 __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan p, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
-    __shared__ __align__(16) u32 u[LIN_JOIN_TOKENS][LIN_JOIN_RANK], b[LIN_JOIN_ROWS][LIN_JOIN_RANK + 4];
-    __shared__ int of[LIN_JOIN_TOKENS];
-    const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS, nt = blockIdx.y / groups, t0 = nt * p.tt + (blockIdx.y - nt * groups) * LIN_JOIN_TOKENS;
-    const u32 tile_end = (nt + 1) * p.tt < p.tokens ? (nt + 1) * p.tt : p.tokens, end = t0 + LIN_JOIN_TOKENS < tile_end ? t0 + LIN_JOIN_TOKENS : tile_end;
-    if (t0 >= end) return;
-    const u32 i0 = blockIdx.x * LIN_JOIN_ROWS, in = threadIdx.x & (LIN_JOIN_ROWS - 1), i = i0 + in, mine = t0 + (threadIdx.x >> 6), rank = A.rank;
-    if (threadIdx.x < LIN_JOIN_TOKENS && rank) {
-        const int a = t0 + threadIdx.x < end ? A.adapter_of[t0 + threadIdx.x] : -1;
-        of[threadIdx.x] = a >= 0 && (u32)a < A.num_adapters ? a : -1;
-    }
-    const u64 bias = A.bias && i < A.m ? A.bias[i] : 0u;
-    u64 y[4] = {bias, bias, bias, bias};
-    pdl_wait();
-    if (i < A.m) lin_sums(p, slots, i / LIN_ROWS, nt, i % LIN_ROWS, mine, 4, end, y);
-    for (u32 r0 = 0; r0 < rank; r0 += LIN_JOIN_RANK) {
-        __syncthreads();
-        for (u32 k = threadIdx.x; k < LIN_JOIN_TOKENS * LIN_JOIN_RANK; k += 256) {
-            const u32 t = k / LIN_JOIN_RANK, r = r0 + k % LIN_JOIN_RANK;
-            u64 v[1] = {0};
-            if (r < rank && of[t] >= 0) {
-                const u32 row = (u32)of[t] * rank + r;
-                if (p.a_rows) lin_sums(p, slots, p.wtiles + row / LIN_ROWS, nt, row % LIN_ROWS, t0 + t, 1, end, v);
-                else v[0] = u_own[(size_t)(t0 + t) * rank + r];
-            }
-            u[t][k % LIN_JOIN_RANK] = red64(v[0]);
+    __shared__ __align__(16) u32 b[LIN_JOIN_RUNS][LIN_JOIN_ROWS][LIN_JOIN_RANK + 4];
+    __shared__ __align__(16) u32 u[LIN_JOIN_TOKENS][LIN_JOIN_RANK];
+    __shared__ int of[LIN_JOIN_TOKENS], run_of[LIN_JOIN_TOKENS], run_adapter[LIN_JOIN_TOKENS], runs;
+    const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS, nt = blockIdx.y / groups, in_tile = (blockIdx.y - nt * groups) * LIN_JOIN_TOKENS, t0 = nt * p.tt + in_tile;
+    const u32 tile_end = (nt + 1) * p.tt < p.tokens ? (nt + 1) * p.tt : p.tokens;
+    if (t0 >= tile_end) return;
+    const u32 count = tile_end - t0 < LIN_JOIN_TOKENS ? tile_end - t0 : LIN_JOIN_TOKENS;
+    const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = tid & (LIN_JOIN_ROWS - 1), mine = tid >> 6, i0 = blockIdx.x * LIN_JOIN_ROWS, i = i0 + row, rank = A.rank;
+    // what does not come from the product: before waiting for it
+    int n_runs = 0;
+    if (rank) {
+        if (warp == 0) {                       // runs of tokens with the same adapter; lanes 0 .. 15 are the tokens
+            const int a = lane < count ? A.adapter_of[t0 + lane] : -1;
+            const int mine_of = a >= 0 && (u32)a < A.num_adapters ? a : -1, before = __shfl_up_sync(0xffffffffu, mine_of, 1);
+            const bool begins = mine_of >= 0 && (lane == 0 || before != mine_of);
+            const u32 all = __ballot_sync(0xffffffffu, begins), run = __popc(all & (0xffffffffu >> (31 - lane))) - 1;
+            if (lane < LIN_JOIN_TOKENS) { of[lane] = mine_of; run_of[lane] = mine_of >= 0 ? (int)run : -1; }
+            if (begins) run_adapter[run] = mine_of;
+            if (lane == 0) runs = __popc(all);
         }
-        for (u32 first = 0; first < end - t0;) {               // tokens first .. until - 1 have the same adapter, or none
-            u32 until = first + 1;
-            while (until < end - t0 && of[until] == of[first]) until++;
-            if (of[first] >= 0) {
-                __syncthreads();
-                const u32* from = A.b + ((size_t)of[first] * A.m + i0) * rank + r0;
-                for (u32 k = threadIdx.x; k < LIN_JOIN_ROWS * LIN_JOIN_RANK; k += 256) {
-                    const u32 row = k / LIN_JOIN_RANK, r = k % LIN_JOIN_RANK;
-                    b[row][r] = i0 + row < A.m && r0 + r < rank ? from[(size_t)row * rank + r] : 0u;
+        __syncthreads();
+        n_runs = runs;
+    }
+    auto stage_b = [&](int run0, u32 r0) {
+        const u32 staged = n_runs - run0 < (int)LIN_JOIN_RUNS ? n_runs - run0 : LIN_JOIN_RUNS;
+#pragma unroll 8
+        for (u32 k = tid; k < staged * LIN_JOIN_ROWS * LIN_JOIN_RANK; k += 256) {
+            const u32 run = k / (LIN_JOIN_ROWS * LIN_JOIN_RANK), at = k / LIN_JOIN_RANK % LIN_JOIN_ROWS, r = k % LIN_JOIN_RANK;
+            b[run][at][r] = i0 + at < A.m && r0 + r < rank ? A.b[((size_t)run_adapter[run0 + run] * A.m + i0 + at) * rank + r0 + r] : 0u;
+        }
+    };
+    const u64 bias = A.bias && i < A.m ? A.bias[i] : 0u;
+    if (n_runs) stage_b(0, 0);
+    pdl_wait();
+    // A x of each token's own adapter, 32 of its rank at a time
+    auto sum_u = [&](u32 r0) {
+        for (u32 t = warp; t < LIN_JOIN_TOKENS; t += 8) {
+            u64 v = 0;
+            if (t < count && of[t] >= 0 && r0 + lane < rank) {
+                if (p.a_rows) {
+                    const u32 a_row = (u32)of[t] * rank + r0 + lane, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
+                    const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
+                    for (u32 seg = 0; seg < p.segs; seg++) {
+                        const u32 last = lin_last(p, tile, seg);
+#pragma unroll 8
+                        for (u32 c = lin_first(p, tile, seg); c <= last; c++) v += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
+                    }
+                } else {
+                    v = u_own[(size_t)(t0 + t) * rank + r0 + lane];
                 }
+            }
+            u[t][lane] = red64(v);
+        }
+    };
+    if (n_runs) sum_u(0);
+    u64 y[4] = {bias, bias, bias, bias};
+    if (i < A.m) {
+        const u32 tile = i / LIN_ROWS * p.ntiles + nt;
+        const u32* at = slots + (size_t)(in_tile + mine) * LIN_ROWS + i % LIN_ROWS;
+        for (u32 seg = 0; seg < p.segs; seg++) {
+            const u32 last = lin_last(p, tile, seg);
+#pragma unroll 4
+            for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
+                const u32* s = at + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words;
+#pragma unroll
+                for (u32 k = 0; k < 4; k++)
+                    if (mine + 4 * k < count) y[k] += s[k * 4 * LIN_ROWS];
+            }
+        }
+    }
+    for (u32 r0 = 0; n_runs && r0 < rank; r0 += LIN_JOIN_RANK) {
+        const u32 width = rank - r0 < LIN_JOIN_RANK ? rank - r0 : LIN_JOIN_RANK;
+        for (int run0 = 0; run0 < n_runs; run0 += LIN_JOIN_RUNS) {
+            if (r0 || run0) {
                 __syncthreads();
+                stage_b(run0, r0);
+                if (run0 == 0) sum_u(r0);
+            }
+            __syncthreads();
+            int run[4];
 #pragma unroll
-                for (u32 k = 0; k < 4; k++) {
-                    const u32 t = (threadIdx.x >> 6) + 4 * k;
-                    if (t < first || t >= until) continue;
+            for (u32 k = 0; k < 4; k++) run[k] = mine + 4 * k < count ? run_of[mine + 4 * k] - run0 : -1;
+            if (run[0] >= 0 && run[0] < (int)LIN_JOIN_RUNS && run[0] == run[1] && run[0] == run[2] && run[0] == run[3]) {
+                for (u32 c = 0; c < width; c += 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(&b[run[0]][row][c]);
+                    const u32 pv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (u32 c = 0; c < LIN_JOIN_RANK; c += 4) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(&b[in][c]), w = *reinterpret_cast<const uint4*>(&u[t][c]);
-                        const u32 pv[4] = {v.x, v.y, v.z, v.w}, pw[4] = {w.x, w.y, w.z, w.w};
+                    for (u32 k = 0; k < 4; k++) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(&u[mine + 4 * k][c]);
+                        const u32 pw[4] = {w.x, w.y, w.z, w.w};
                         y[k] += lin_dot4(pv, pw);
                     }
                 }
+            } else {
+#pragma unroll
+                for (u32 k = 0; k < 4; k++)
+                    if (run[k] >= 0 && run[k] < (int)LIN_JOIN_RUNS)
+                        for (u32 c = 0; c < width; c += 4) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(&b[run[k]][row][c]), w = *reinterpret_cast<const uint4*>(&u[mine + 4 * k][c]);
+                            const u32 pv[4] = {v.x, v.y, v.z, v.w}, pw[4] = {w.x, w.y, w.z, w.w};
+                            y[k] += lin_dot4(pv, pw);
+                        }
             }
-            first = until;
         }
     }
 #pragma unroll
     for (u32 k = 0; k < 4; k++)
-        if (i < A.m && mine + 4 * k < end) A.y[(mine + 4 * k) * A.y_stride + i] = red64(y[k]);
+        if (i < A.m && mine + 4 * k < count) A.y[(t0 + mine + 4 * k) * A.y_stride + i] = red64(y[k]);
 }
 
 // u[t][r] = A[of[t]][r] . x[t]; a CTA per (r, t).
