@@ -353,10 +353,13 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan 
     }
     auto stage_b = [&](int run0, u32 r0) {
         const u32 staged = n_runs - run0 < (int)LIN_JOIN_RUNS ? n_runs - run0 : LIN_JOIN_RUNS;
-#pragma unroll 8
-        for (u32 k = tid; k < staged * LIN_JOIN_ROWS * LIN_JOIN_RANK; k += 256) {
-            const u32 run = k / (LIN_JOIN_ROWS * LIN_JOIN_RANK), at = k / LIN_JOIN_RANK % LIN_JOIN_ROWS, r = k % LIN_JOIN_RANK;
-            b[run][at][r] = i0 + at < A.m && r0 + r < rank ? A.b[((size_t)run_adapter[run0 + run] * A.m + i0 + at) * rank + r0 + r] : 0u;
+        for (u32 run = 0; run < staged; run++) {
+            const u32* from = A.b + ((size_t)run_adapter[run0 + run] * A.m + i0) * rank + r0;
+            u32 v[LIN_JOIN_ROWS / 8];                        // all of a thread's loads before its first store: the compiler cannot tell that they do not meet
+#pragma unroll
+            for (u32 k = 0; k < LIN_JOIN_ROWS / 8; k++) v[k] = i0 + warp + 8 * k < A.m && r0 + lane < rank ? from[(size_t)(warp + 8 * k) * rank + lane] : 0u;
+#pragma unroll
+            for (u32 k = 0; k < LIN_JOIN_ROWS / 8; k++) b[run][warp + 8 * k][lane] = v[k];
         }
     };
     const u64 bias = A.bias && i < A.m ? A.bias[i] : 0u;
@@ -364,23 +367,26 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan 
     pdl_wait();
     // A x of each token's own adapter, 32 of its rank at a time
     auto sum_u = [&](u32 r0) {
-        for (u32 t = warp; t < LIN_JOIN_TOKENS; t += 8) {
-            u64 v = 0;
-            if (t < count && of[t] >= 0 && r0 + lane < rank) {
-                if (p.a_rows) {
-                    const u32 a_row = (u32)of[t] * rank + r0 + lane, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
-                    const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
-                    for (u32 seg = 0; seg < p.segs; seg++) {
-                        const u32 last = lin_last(p, tile, seg);
+        u64 v[LIN_JOIN_TOKENS / 8];
+#pragma unroll
+        for (u32 k = 0; k < LIN_JOIN_TOKENS / 8; k++) {
+            const u32 t = warp + 8 * k;
+            v[k] = 0;
+            if (t >= count || of[t] < 0 || r0 + lane >= rank) continue;
+            if (p.a_rows) {
+                const u32 a_row = (u32)of[t] * rank + r0 + lane, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
+                const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
+                for (u32 seg = 0; seg < p.segs; seg++) {
+                    const u32 last = lin_last(p, tile, seg);
 #pragma unroll 8
-                        for (u32 c = lin_first(p, tile, seg); c <= last; c++) v += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
-                    }
-                } else {
-                    v = u_own[(size_t)(t0 + t) * rank + r0 + lane];
+                    for (u32 c = lin_first(p, tile, seg); c <= last; c++) v[k] += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
                 }
+            } else {
+                v[k] = u_own[(size_t)(t0 + t) * rank + r0 + lane];
             }
-            u[t][lane] = red64(v);
         }
+#pragma unroll
+        for (u32 k = 0; k < LIN_JOIN_TOKENS / 8; k++) u[warp + 8 * k][lane] = red64(v[k]);
     };
     if (n_runs) sum_u(0);
     u64 y[4] = {bias, bias, bias, bias};
