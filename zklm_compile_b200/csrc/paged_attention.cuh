@@ -70,6 +70,7 @@ struct PaWork {                                // see paged_attention_launch
     u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
     u32* desc;                                 // [ctas][2]: 1 + item that begins in this CTA and goes on in the next, number of CTAs it goes on in
     int fast;                                  // tensor copies: rows are whole 16-byte groups on 16-byte boundaries, pages have 8 rows or more
+    int q_vec;                                 // q is read 16 bytes at a time
     int whole;                                 // a box has all the columns of its rows
     int* gave_up;
 };
@@ -112,33 +113,43 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     extern __shared__ __align__(16) unsigned char pa_raw[];
     unsigned char* const pa_smem = pa_raw + ((0u - smem_addr(pa_raw)) & 1023u);    // the swizzle goes by addresses
     uint4* qd = reinterpret_cast<uint4*>(pa_smem + WARPS * NS * S::HALF);          // [J][NT][32]
-    u32* acc_lo = reinterpret_cast<u32*>(qd + J * NT * 32);                        // [HEADS][DP]
-    u32* acc_hi = acc_lo + HEADS * DP;
-    unsigned char* digits = reinterpret_cast<unsigned char*>(acc_hi + HEADS * DP); // [WARPS][NT][ED]
+    u32* part = reinterpret_cast<u32*>(qd + J * NT * 32);                          // [WARPS][HEADS][DP]: sums of e v
+    unsigned char* digits = reinterpret_cast<unsigned char*>(part + WARPS * HEADS * DP);   // [WARPS][NT][ED]
+    __shared__ u32 es_part[WARPS][HEADS], flag_part[WARPS][HEADS];                 // sums of e, and what went wrong
+    __shared__ u32 off_q[HEADS], corr[HEADS], inv[HEADS], scan[32];
     __shared__ __align__(8) u64 bars[WARPS * NS];
     __shared__ volatile int gave_up;
-    __shared__ u32 off_q[HEADS][2], corr[HEADS], inv[HEADS], flags[HEADS], es_lo[HEADS], es_hi[HEADS], scan[32];
-    __shared__ u32 start_seq;
-    __shared__ u64 start_total;
     const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
     const u32 grps = A.c.num_kv_heads * P.slices, hpg = A.num_heads / A.c.num_kv_heads, d = A.c.d;
-    if (tid == 0) gave_up = 0;
+    if (tid == 0) {
+        gave_up = 0;
+        if (P.fast) { prefetch_tensor_map(&map_k); prefetch_tensor_map(&map_v); }
+    }
     pdl_launch_dependents();
 
     // ---- this CTA's share of the blocks ---------------------------------------------------------
+    // up to 256 sequences by every warp for itself, more by the CTA
+    constexpr int K = 8;
     u64 total = 0;
-    for (u32 s = tid; s < A.num_seqs; s += THREADS) { u32 len; total += pa_blocks(A, s, BLOCK, len); }
-    {   // sum over the CTA
-        __shared__ u64 part[WARPS];
+    u32 own_nb[K];
+    const bool few = A.num_seqs <= 32 * K;
+    if (few) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (lane == 0) part[warp] = total;
+        for (int k = 0; k < K; k++) { u32 len; own_nb[k] = 32 * k + lane < A.num_seqs ? pa_blocks(A, 32 * k + lane, BLOCK, len) : 0u; total += own_nb[k]; }
+    } else {
+        for (u32 s = tid; s < A.num_seqs; s += THREADS) { u32 len; total += pa_blocks(A, s, BLOCK, len); }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (!few) {
+        __shared__ u64 sums[WARPS];
+        if (lane == 0) sums[warp] = total;
         __syncthreads();
         total = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) total += part[w];
-        total *= grps;
+        for (int w = 0; w < WARPS; w++) total += sums[w];
     }
+    total *= grps;
     const u64 per = (total + P.ctas - 1) / P.ctas, from = per * blockIdx.x, to = from + per < total ? from + per : total;
     // rows without positions are zero
     for (u32 s = blockIdx.x; s < A.num_seqs; s += P.ctas) {
@@ -149,8 +160,26 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     }
     if (tid == 0) { P.desc[2 * blockIdx.x] = 0; P.desc[2 * blockIdx.x + 1] = 0; }
     if (from >= to) return;
-    {   // the sequence in which block `from` lies
-        u64 before = 0;
+    u32 start_seq = 0;                         // the sequence in which block `from` lies, and the blocks of it that lie before
+    u64 start_rest = 0, before = 0;
+    if (few) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (32u * k >= A.num_seqs) break;
+            u32 x = own_nb[k];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const u32 y = __shfl_up_sync(0xffffffffu, x, o); if ((int)lane >= o) x += y; }
+            const u64 end = (before + x) * grps, begin = end - (u64)own_nb[k] * grps;
+            const u32 here = __ballot_sync(0xffffffffu, begin <= from && from < end);
+            if (here) {
+                start_seq = 32 * k + __ffs(here) - 1;
+                start_rest = from - __shfl_sync(0xffffffffu, begin, __ffs(here) - 1);
+            }
+            before += __shfl_sync(0xffffffffu, x, 31);
+        }
+    } else {
+        __shared__ u32 found_seq;
+        __shared__ u64 found_rest;
         for (u32 base = 0;; base += THREADS) {
             u32 len, nb = base + tid < A.num_seqs ? pa_blocks(A, base + tid, BLOCK, len) : 0u, x = nb;
 #pragma unroll
@@ -161,11 +190,13 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
             for (int i = 0; i < WARPS; i++) { if (i < (int)warp) w += scan[i]; all += scan[i]; }
             const u64 end = (before + w + x) * grps, begin = end - (u64)nb * grps;
-            if (nb && begin <= from && from < end) { start_seq = base + tid; start_total = from - begin; }
+            if (nb && begin <= from && from < end) { found_seq = base + tid; found_rest = from - begin; }
             before += all;
             __syncthreads();
             if (before * grps > from) break;
         }
+        start_seq = found_seq;
+        start_rest = found_rest;
     }
     PaWalk cw{};
     cw.seq = start_seq;
@@ -173,10 +204,10 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     cw.slices = P.slices;
     cw.left = (u32)(to - from);
     cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
-    const u32 start_grp = (u32)(start_total / cw.nb);
+    const u32 start_grp = (u32)(start_rest / cw.nb);
     cw.kvh = start_grp / P.slices;
     cw.slice = start_grp - cw.kvh * P.slices;
-    cw.blk = (u32)(start_total - (u64)start_grp * cw.nb);
+    cw.blk = (u32)(start_rest - (u64)start_grp * cw.nb);
     PaWalk lw = cw;                            // the copies run ahead of the computation
 
     // ---- copies -------------------------------------------------------------------------------------
@@ -269,41 +300,48 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? cw.left : nb - first;
         const u32 item = seq * grps + cw.kvh * P.slices + cw.slice;
         __syncthreads();                        // the row before is done with these arrays
-        for (u32 i = tid; i < J * NT * 32; i += THREADS) {
-            // 16 bytes of the right operand of a lane: steps 2j, 2j + 1 of a tile of 8 columns
-            const u32 j = i / (NT * 32), nt = i / 32 % NT, n = i % 32 / 4, qq = i & 3, head = 2 * nt + (n >> 2), c = n & 3;
-            u32 w[4];
+        // The right operand of the scores: a thread takes four words' places of one head, whose digits are four lanes' 16 bytes for steps 2j and 2j + 1.
+        for (u32 i = tid; i < HEADS * J * 4; i += THREADS) {
+            const u32 head = i / (J * 4), j = i / 4 % J, qq = i & 3, e0 = (16 * j + 4 * qq) * (SMALL ? 2 : 1);
+            constexpr u32 N = SMALL ? 8 : 4;
+            const u32* from_q = A.q + seq * A.q_stride + (size_t)(head0 + head) * d + e0;
+            u32 qv[N];
+#pragma unroll
+            for (u32 k = 0; k < N; k += 4) {
+                if (P.q_vec) {
+                    const uint4 t = head < heads && e0 + k < d ? *reinterpret_cast<const uint4*>(from_q + k) : make_uint4(0, 0, 0, 0);
+                    qv[k] = t.x; qv[k + 1] = t.y; qv[k + 2] = t.z; qv[k + 3] = t.w;
+                } else {
+#pragma unroll
+                    for (u32 e = k; e < k + 4; e++) qv[e] = head < heads && e0 + e < d ? from_q[e] : 0u;
+                }
+            }
+            u32 w[4][4];                         // [column c][word]
 #pragma unroll
             for (u32 k = 0; k < 4; k++) {
-                const u32 word = 16 * j + 4 * qq + k;
-                const u32* qrow = A.q + seq * A.q_stride + (size_t)(head0 + head) * d;
-                u32 dw[4] = {0, 0, 0, 0};
+                u32 da[4], db[4];
                 if (SMALL) {
-                    u32 da[4], db[4];
-                    digit_words(head < heads && 2 * word < d ? qrow[2 * word] : 0u, da);
-                    digit_words(head < heads && 2 * word + 1 < d ? qrow[2 * word + 1] : 0u, db);
-                    w[k] = __byte_perm(c == 0 ? da[0] : c == 1 ? da[1] : c == 2 ? da[2] : da[3], c == 0 ? db[0] : c == 1 ? db[1] : c == 2 ? db[2] : db[3], 0x5410);
-                } else {
-                    digit_words(head < heads && word < d ? qrow[word] : 0u, dw);
-                    w[k] = c == 0 ? dw[0] : c == 1 ? dw[1] : c == 2 ? dw[2] : dw[3];
-                }
-            }
-            qd[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        for (u32 i = tid; i < 2 * HEADS * DP; i += THREADS) acc_lo[i] = 0;
-        if (tid < HEADS) { flags[tid] = 0; es_lo[tid] = 0; es_hi[tid] = 0; }
-        if (SMALL)
-            for (u32 h = warp; h < HEADS; h += WARPS) {
-                u64 s = 0;
-                for (u32 e = lane; e < (h < heads ? d : 0u); e += 32) s += A.q[seq * A.q_stride + (size_t)(head0 + h) * d + e];
+                    digit_words(qv[2 * k % N], da);
+                    digit_words(qv[(2 * k + 1) % N], db);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (lane == 0) {                    // what flipped top bits add to a score is taken off its digits 0 and 2 at the start
-                    const u32 less = neg31(mul31(red64(s), 32768u));
-                    off_q[h][0] = less & 0xffffu;
-                    off_q[h][1] = less >> 16;
+                    for (u32 c = 0; c < 4; c++) w[c][k] = __byte_perm(da[c], db[c], 0x5410);
+                } else {
+                    digit_words(qv[k], da);
+#pragma unroll
+                    for (u32 c = 0; c < 4; c++) w[c][k] = da[c];
                 }
             }
+#pragma unroll
+            for (u32 c = 0; c < 4; c++) qd[(j * NT + head / 2) * 32 + ((head & 1) * 4 + c) * 4 + qq] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+            if (SMALL) {                         // what flipped top bits add to a score, 2^15 sum q, is taken off its digits 0 and 2 at the start; J * 4 lanes have a head
+                u64 sum = 0;
+#pragma unroll
+                for (u32 k = 0; k < N; k++) sum += qv[k];
+#pragma unroll
+                for (u32 o = J * 2; o > 0; o >>= 1) sum += __shfl_xor_sync(J * 4 == 32 ? 0xffffffffu : ((1u << (J * 4 % 32)) - 1) << (lane & ~(J * 4 - 1)), sum, o);
+                if ((lane & (J * 4 - 1)) == 0) off_q[head] = neg31(mul31(red64(sum), 32768u));
+            }
+        }
         __syncthreads();
 
         int acc[MT][NT][4];
@@ -317,7 +355,9 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
                 for (int i = 0; i < 4; i++) acc[m][n][i] = 0;
         }
-        auto flush = [&]() {                    // sums of 32 bits to halves that add up in shared memory
+        bool flushed = false;
+        auto flush = [&]() {                    // sums of 32 bits to the warp's sums mod p
+            u32* to_part = part + (warp * HEADS + (q4 >> 1)) * DP;
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -326,11 +366,11 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                     const u32 v = pa_value(c, odd, weights);
                     // rows of the tile are elements (see the left operand below)
                     const u32 e = SMALL ? 8 * (8 * (m >> 2) + g) + 2 * (m & 3) + odd : 4 * (8 * (m >> 1) + g) + 2 * (m & 1) + odd;
-                    const u32 at = (2 * n + (q4 >> 1)) * DP + e;
-                    atomicAdd(acc_lo + at, v & 0xffffu);
-                    atomicAdd(acc_hi + at, v >> 16);
+                    u32* at = to_part + 2 * n * DP + e;
+                    *at = flushed ? add31(*at, v) : v;
                     c[0] = c[1] = c[2] = c[3] = 0;
                 }
+            flushed = true;
         };
         u32* ed = reinterpret_cast<u32*>(digits + warp * NT * S::ED);
         const u32 round_up = (1u << A.score_shift) >> 1;
@@ -345,7 +385,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     sc[n][1] = sc[n][3] = 0;
-                    sc[n][0] = sc[n][2] = SMALL ? (int)off_q[2 * n + (q4 >> 1)][odd] : 0;
+                    sc[n][0] = sc[n][2] = SMALL ? (int)((off_q[2 * n + (q4 >> 1)] >> (odd ? 16 : 0)) & 0xffffu) : 0;
                 }
 #pragma unroll
                 for (int j = 0; j < J; j++) {
@@ -450,7 +490,6 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             computed++;
             if ((b + 1) % PA_FLUSH == 0) flush();
         }
-        flush();
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             u32 s = red64(esum[n]);
@@ -460,39 +499,39 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 s = add31(s, __shfl_xor_sync(0xffffffffu, s, o));
                 f |= __shfl_xor_sync(0xffffffffu, f, o);
             }
-            if (g == 0 && !(q4 & 1)) {
-                const u32 h = 2 * n + (q4 >> 1);
-                atomicAdd(es_lo + h, s & 0xffffu);
-                atomicAdd(es_hi + h, s >> 16);
-                if (f) atomicOr(flags + h, f);
-            }
+            if (g == 0 && !odd) { es_part[warp][2 * n + (q4 >> 1)] = s; flag_part[warp][2 * n + (q4 >> 1)] = f; }
         }
         __syncthreads();
         const bool begins = first == 0, ends = first + count == nb;
-        if (begins && ends) {
-            if (tid < heads) {
-                const u32 s = red64(es_lo[tid] + ((u64)es_hi[tid] << 16)), f = flags[tid];
+        u32* slot = P.slots + (size_t)(2 * blockIdx.x + (begins ? 1 : 0)) * HEADS * (DP + 4);
+        if (tid < heads) {                      // while the other warps store their sums
+            u32 s = 0, f = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) { s = add31(s, es_part[w][tid]); f |= flag_part[w][tid]; }
+            if (begins && ends) {
                 const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : s == 0 ? SERVE_ZERO_SUM : 0;
                 if (code) atomicMax(A.status + seq, code);
                 inv[tid] = code ? 0u : inv31_chain(s);
                 corr[tid] = SMALL ? mul31(s, 32768u) : 0u;
+            } else {
+                slot[tid * (DP + 4) + DP] = s;
+                slot[tid * (DP + 4) + DP + 1] = f;
             }
-            __syncthreads();
-            for (u32 i = tid; i < heads * DP; i += THREADS) {
-                const u32 h = i / DP, e = i % DP;
-                if (e < d) pa_finish(A, seq, head0 + h, e, red64(acc_lo[i] + ((u64)acc_hi[i] << 16)), inv[h], corr[h]);
-            }
-        } else {
-            u32* slot = P.slots + (size_t)(2 * blockIdx.x + (begins ? 1 : 0)) * HEADS * (DP + 4);
-            for (u32 i = tid; i < heads * DP; i += THREADS) slot[i / DP * (DP + 4) + i % DP] = red64(acc_lo[i] + ((u64)acc_hi[i] << 16));
-            if (tid < heads) {
-                slot[tid * (DP + 4) + DP] = red64(es_lo[tid] + ((u64)es_hi[tid] << 16));
-                slot[tid * (DP + 4) + DP + 1] = flags[tid];
-            }
-            if (begins && tid == 0) {
-                P.desc[2 * blockIdx.x + 1] = (u32)((nb - first - count + per - 1) / per);
-                P.desc[2 * blockIdx.x] = item + 1;
-            }
+        }
+        __syncwarp();
+        flush();
+        __syncthreads();
+        for (u32 i = tid; i < heads * DP; i += THREADS) {
+            u64 sum = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) sum += part[w * HEADS * DP + i];
+            const u32 h = i / DP, e = i % DP;
+            if (!(begins && ends)) slot[h * (DP + 4) + e] = red64(sum);
+            else if (e < d) pa_finish(A, seq, head0 + h, e, red64(sum), inv[h], corr[h]);
+        }
+        if (begins && !ends && tid == 0) {
+            P.desc[2 * blockIdx.x + 1] = (u32)((nb - first - count + per - 1) / per);
+            P.desc[2 * blockIdx.x] = item + 1;
         }
         cw.step(A, count);
     }
@@ -547,7 +586,7 @@ inline PaChoice pa_choice(u32 d, u32 hpg) {
 template <int DP, bool SMALL, int NT>
 inline cudaError_t pa_launch(cudaStream_t stream, const CUtensorMap (&maps)[2], const PagedAttnArgs& a, PaWork w, int* launches) {
     using S = PaShape<DP, SMALL>;
-    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)4 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED + 1024;
+    constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)S::WARPS * 2 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED + 1024;
     static_assert(smem <= 226 * 1024, "with the kernel's own arrays below the 227 KB of a CTA");
     cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<DP, SMALL, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;

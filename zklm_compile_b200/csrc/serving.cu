@@ -47,6 +47,7 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
     w.slice_heads = c.slice_heads;
     w.ctas = (u32)sm_count;
     w.gave_up = a.gave_up;
+    w.q_vec = a.c.d % 4 == 0 && a.q_stride % 4 == 0 && !((uintptr_t)a.q & 15);
     w.slots = (u32*)a.workspace;
     w.desc = w.slots + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4);
     // Tensor copies want 16-byte boundaries; a box of less than the 8 rows of the swizzle's pattern is left to plain loads.

@@ -39,6 +39,7 @@ __device__ __forceinline__ void tensor_load_2d(u32 dst, const CUtensorMap* map, 
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // By one lane of a converged warp, all of whose lanes have the same operands: chosen inside the instruction's own statement, so that the compiler need not
 // provide for several lanes with operands of their own (a branch on the lane cost fifty instructions a copy).
 __device__ __forceinline__ void mbar_expect_one(u32 bar, u32 bytes) {
