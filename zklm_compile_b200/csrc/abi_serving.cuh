@@ -143,6 +143,7 @@ int32_t zkb_paged_attention(zkb_ctx* c, const zkb_kv_cache* cache, const uint32_
         a.out = out_dev; a.status = status_dev;
         ServeWorkspace ws(c, workspace_dev, workspace_bytes, paged_attention_workspace(c->sm_count, num_heads, a.c.num_kv_heads, a.c.d, num_seqs));
         a.workspace = ws.p;
+        a.counters = workspace_dev ? nullptr : c->serve_counts(paged_attention_counters(c->sm_count));
         a.gave_up = c->serve_flag();
         int n = 0;
         ZKB_CUDA(paged_attention_launch(c->stream, c->sm_count, a, &n));

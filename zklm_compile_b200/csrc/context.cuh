@@ -177,6 +177,18 @@ struct zkb_ctx {
         }
         return serve_gave_up;
     }
+    // Counters of the paged attention, zero between its calls (which are in order on `stream`); made at the first of them.
+    void* serve_counters = nullptr;
+    void* serve_counts(size_t bytes) {
+        if (!serve_counters) {
+            void* p = nullptr;
+            ZKB_CUDA(cudaMalloc(&p, bytes));
+            const cudaError_t e = cudaMemsetAsync(p, 0, bytes, stream);
+            if (e != cudaSuccess) { cudaFree(p); ZKB_CUDA(e); }
+            serve_counters = p;
+        }
+        return serve_counters;
+    }
     // Second stream for work that does not depend on the transcript (the fold / tree chain of a Basefold
     // opening), joined to `stream` through events; created on first use.
     cudaStream_t side = nullptr;

@@ -17,7 +17,7 @@
 // an mbarrier a slot counts, so warps never wait for one another within a row.  (A bulk copy a row instead of a box held the 16-bit cache to
 // 3.4 TB/s.)  The work
 // of a call is one list of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences'
-// lengths are; a row that CTAs share is added up by paged_attention_join_kernel.  Integer sums have no order, so results do not depend on
+// lengths are; a row that CTAs share is added up by the one that brings its last part.  Integer sums have no order, so results do not depend on
 // the split.
 #pragma once
 #include <type_traits>
@@ -68,7 +68,7 @@ struct PaShape {
 struct PaWork {                                // see paged_attention_launch
     u32 slices, slice_heads, ctas;
     u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
-    u32* desc;                                 // [ctas][2]: 1 + item that begins in this CTA and goes on in the next, number of CTAs it goes on in
+    u32* arrived;                              // [ctas], zero before and after a call: how many parts are there of the row that begins in this CTA
     int fast;                                  // tensor copies: rows are whole 16-byte groups on 16-byte boundaries, pages have 8 rows or more
     int q_vec;                                 // q is read 16 bytes at a time
     int whole;                                 // a box has all the columns of its rows
@@ -119,13 +119,13 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     __shared__ u32 off_q[HEADS], corr[HEADS], inv[HEADS], scan[32];
     __shared__ __align__(8) u64 bars[WARPS * NS];
     __shared__ volatile int gave_up;
+    __shared__ int last_part;
     const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
     const u32 grps = A.c.num_kv_heads * P.slices, hpg = A.num_heads / A.c.num_kv_heads, d = A.c.d;
     if (tid == 0) {
         gave_up = 0;
         if (P.fast) { prefetch_tensor_map(&map_k); prefetch_tensor_map(&map_v); }
     }
-    pdl_launch_dependents();
 
     // ---- this CTA's share of the blocks ---------------------------------------------------------
     // up to 256 sequences by every warp for itself, more by the CTA
@@ -150,7 +150,32 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         for (int w = 0; w < WARPS; w++) total += sums[w];
     }
     total *= grps;
-    const u64 per = (total + P.ctas - 1) / P.ctas, from = per * blockIdx.x, to = from + per < total ? from + per : total;
+    u64 per = (total + P.ctas - 1) / P.ctas;
+    // Where the rows are fewer than the CTAs each CTA keeps to one row (`aligned`: a share is `per` blocks of one item), if that costs no one much more;
+    // a second row in a CTA costs as much as several blocks.
+    bool aligned = false;
+    if (few) {
+        u32 rows = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++) rows += __popc(__ballot_sync(0xffffffffu, own_nb[k] != 0));
+        if (rows && (u64)rows * grps <= P.ctas) {
+            for (u32 more = 0; more < 3 && !aligned; more++) {
+                const u32 p = (u32)per + (more ? ((u32)per + 7) / 8 * more : 0);
+                u32 shares = 0;
+#pragma unroll
+                for (int k = 0; k < K; k++) shares += (own_nb[k] + p - 1) / p;
+                shares = __reduce_add_sync(0xffffffffu, shares);
+                if ((u64)shares * grps <= P.ctas) {
+                    aligned = true;
+                    per = p;
+                    total = (u64)shares * grps;
+#pragma unroll
+                    for (int k = 0; k < K; k++) own_nb[k] = (own_nb[k] + p - 1) / p;       // in shares from here on
+                }
+            }
+        }
+    }
+    const u64 from = aligned ? blockIdx.x : per * blockIdx.x, to = aligned ? (from < total ? from + 1 : from) : from + per < total ? from + per : total;
     // rows without positions are zero
     for (u32 s = blockIdx.x; s < A.num_seqs; s += P.ctas) {
         u32 len;
@@ -158,7 +183,6 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         for (u32 i = tid; i < A.num_heads * d; i += THREADS) A.out[(size_t)s * A.num_heads * d + i] = 0;
         if (tid == 0 && A.lens[s] != 0) atomicMax(A.status + s, (int)SERVE_PAGE);
     }
-    if (tid == 0) { P.desc[2 * blockIdx.x] = 0; P.desc[2 * blockIdx.x + 1] = 0; }
     if (from >= to) return;
     u32 start_seq = 0;                         // the sequence in which block `from` lies, and the blocks of it that lie before
     u64 start_rest = 0, before = 0;
@@ -202,12 +226,12 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     cw.seq = start_seq;
     cw.block = BLOCK;
     cw.slices = P.slices;
-    cw.left = (u32)(to - from);
     cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
-    const u32 start_grp = (u32)(start_rest / cw.nb);
+    const u32 parts = aligned ? (u32)((cw.nb + per - 1) / per) : cw.nb, start_grp = (u32)(start_rest / parts);       // of an item, in what the rest is counted in
     cw.kvh = start_grp / P.slices;
     cw.slice = start_grp - cw.kvh * P.slices;
-    cw.blk = (u32)(start_rest - (u64)start_grp * cw.nb);
+    cw.blk = (u32)(start_rest - (u64)start_grp * parts) * (aligned ? (u32)per : 1u);
+    cw.left = !aligned ? (u32)(to - from) : cw.nb - cw.blk < per ? cw.nb - cw.blk : (u32)per;
     PaWalk lw = cw;                            // the copies run ahead of the computation
 
     // ---- copies -------------------------------------------------------------------------------------
@@ -298,7 +322,6 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     while (cw.left) {
         const u32 seq = cw.seq, head0 = cw.kvh * hpg + cw.slice * P.slice_heads, rest = hpg - cw.slice * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
         const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? cw.left : nb - first;
-        const u32 item = seq * grps + cw.kvh * P.slices + cw.slice;
         __syncthreads();                        // the row before is done with these arrays
         // The right operand of the scores: a thread takes four words' places of one head, whose digits are four lanes' 16 bytes for steps 2j and 2j + 1.
         for (u32 i = tid; i < HEADS * J * 4; i += THREADS) {
@@ -529,9 +552,49 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             if (!(begins && ends)) slot[h * (DP + 4) + e] = red64(sum);
             else if (e < d) pa_finish(A, seq, head0 + h, e, red64(sum), inv[h], corr[h]);
         }
-        if (begins && !ends && tid == 0) {
-            P.desc[2 * blockIdx.x + 1] = (u32)((nb - first - count + per - 1) / per);
-            P.desc[2 * blockIdx.x] = item + 1;
+        if (!(begins && ends)) {
+            // The CTA that brings a row's last part adds the parts up.  They lie in the slot of the CTA in which the row begins and those of the next ones.
+            const u64 at = to - cw.left, row0 = at - first;
+            const u32 c0 = aligned ? blockIdx.x - first / (u32)per : (u32)(row0 / per), n = aligned ? (u32)((nb + per - 1) / per) : (u32)((row0 + nb - 1) / per) - c0 + 1;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const u32 before = atomicAdd(P.arrived + c0, 1u);
+                last_part = before == n - 1;
+                if (last_part) P.arrived[c0] = 0;
+            }
+            __syncthreads();
+            if (last_part) {
+                __threadfence();
+                auto slot_of = [&](u32 k) { return P.slots + (size_t)(2 * (c0 + k) + (k ? 0 : 1)) * HEADS * (DP + 4); };
+                for (u32 h = warp; h < heads; h += WARPS) {
+                    u64 s = 0;
+                    u32 f = 0;
+                    for (u32 k = lane; k < n; k += 32) {
+                        const u32* from_slot = slot_of(k) + h * (DP + 4) + DP;
+                        s += __ldcg(from_slot);
+                        f |= __ldcg(from_slot + 1);
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                    f = __reduce_or_sync(0xffffffffu, f);
+                    if (lane == 0) {
+                        const u32 sum = red64(s);
+                        const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : sum == 0 ? SERVE_ZERO_SUM : 0;
+                        if (code) atomicMax(A.status + seq, code);
+                        inv[h] = code ? 0u : inv31_chain(sum);
+                        corr[h] = SMALL ? mul31(sum, 32768u) : 0u;
+                    }
+                }
+                __syncthreads();
+                for (u32 i = tid; i < heads * DP; i += THREADS) {
+                    const u32 h = i / DP, e = i % DP;
+                    u64 sum = 0;
+#pragma unroll 8
+                    for (u32 k = 0; k < n; k++) sum += __ldcg(slot_of(k) + h * (DP + 4) + e);
+                    if (e < d) pa_finish(A, seq, head0 + h, e, red64(sum), inv[h], corr[h]);
+                }
+            }
         }
         cw.step(A, count);
     }
@@ -543,32 +606,6 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         }
         if (lane == 0) *P.gave_up = 1;
     }
-}
-
-// A row that several CTAs share, added up by the CTA of the same number as the one in which it begins; blockIdx.y: a head of the slice.
-template <int DP, bool SMALL, int NT>
-__global__ void __launch_bounds__(DP) paged_attention_join_kernel(PagedAttnArgs A, PaWork P) {
-    constexpr int HEADS = 2 * NT;
-    pdl_wait();
-    const u32 c = blockIdx.x, h = blockIdx.y, item = P.desc[2 * c];
-    if (!item) return;
-    const u32 more = P.desc[2 * c + 1], grps = A.c.num_kv_heads * P.slices, seq = (item - 1) / grps, grp = (item - 1) - seq * grps;
-    const u32 kvh = grp / P.slices, hpg = A.num_heads / A.c.num_kv_heads, in = (grp - kvh * P.slices) * P.slice_heads + h;
-    if (in >= hpg || h >= P.slice_heads) return;
-    const u32* at = P.slots + ((size_t)(2 * c + 1) * HEADS + h) * (DP + 4);
-    const u32 e = threadIdx.x;
-    u64 acc = at[e], es = at[DP];
-    u32 f = at[DP + 1];
-    for (u32 k = 1; k <= more; k++) {
-        const u32* s = P.slots + ((size_t)(2 * (c + k)) * HEADS + h) * (DP + 4);
-        acc += s[e];
-        es += s[DP];
-        f |= s[DP + 1];
-    }
-    const u32 s = red64(es);
-    const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : s == 0 ? SERVE_ZERO_SUM : 0;
-    if (code && e == 0) atomicMax(A.status + seq, code);
-    if (e < A.c.d) pa_finish(A, seq, kvh * hpg + in, e, red64(acc), code ? 0u : inv31_chain(s), SMALL ? mul31(s, 32768u) : 0u);
 }
 
 // ---- launch ---------------------------------------------------------------------------------------------
@@ -588,23 +625,13 @@ inline cudaError_t pa_launch(cudaStream_t stream, const CUtensorMap (&maps)[2], 
     using S = PaShape<DP, SMALL>;
     constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)S::WARPS * 2 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED + 1024;
     static_assert(smem <= 226 * 1024, "with the kernel's own arrays below the 227 KB of a CTA");
-    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<DP, SMALL, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem(paged_attention_kernel<DP, SMALL, NT>, smem);
     if (e != cudaSuccess) return e;
     const u64 most = (u64)a.num_seqs * a.c.num_kv_heads * w.slices * ((((u64)a.max_blocks << a.c.page_bits) + S::WARPS * 16 - 1) / (S::WARPS * 16));
     if (most < w.ctas) w.ctas = (u32)most;
     paged_attention_kernel<DP, SMALL, NT><<<w.ctas, S::WARPS * 32, smem, stream>>>(maps[0], maps[1], a, w);
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(w.ctas, w.slice_heads);
-    cfg.blockDim = DP;
-    cfg.stream = stream;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<DP, SMALL, NT>, a, w);
-    *launches += 2;
-    return e != cudaSuccess ? e : cudaGetLastError();
+    ++*launches;
+    return cudaGetLastError();
 }
 
 }  // namespace zkb

@@ -34,10 +34,11 @@ static cudaError_t rows_tensor_map(CUtensorMap* map, const u32* w, u32 rows, u32
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+size_t paged_attention_counters(int sm_count) { return ((size_t)sm_count * 4 + 255) / 256 * 256; }
 size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs) {
     if (!num_seqs) return 0;
     const PaChoice c = pa_choice(d, num_heads / num_kv_heads);
-    return ((size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4) + (size_t)sm_count * 2) * 4;
+    return paged_attention_counters(sm_count) + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4) * 4;
 }
 cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const PagedAttnArgs& a, int* launches) {
     const PaChoice c = pa_choice(a.c.d, a.num_heads / a.c.num_kv_heads);
@@ -48,8 +49,8 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
     w.ctas = (u32)sm_count;
     w.gave_up = a.gave_up;
     w.q_vec = a.c.d % 4 == 0 && a.q_stride % 4 == 0 && !((uintptr_t)a.q & 15);
-    w.slots = (u32*)a.workspace;
-    w.desc = w.slots + (size_t)sm_count * 2 * 2 * c.nt * (c.dp + 4);
+    w.arrived = a.counters ? (u32*)a.counters : (u32*)a.workspace;
+    w.slots = (u32*)((char*)a.workspace + paged_attention_counters(sm_count));
     // Tensor copies want 16-byte boundaries; a box of less than the 8 rows of the swizzle's pattern is left to plain loads.
     CUtensorMap maps[2] = {};
     const uint64_t row_bytes = (uint64_t)a.c.d * size, page_bytes = a.c.page_stride * size;
@@ -113,7 +114,7 @@ size_t adapter_linear_workspace(int sm_count, uint32_t tokens, uint32_t m, uint3
 template <bool W_COPY, bool X_FILL>
 static cudaError_t lin_product(cudaStream_t stream, bool early, const CUtensorMap& map_w, const CUtensorMap& map_a, const LinPlan& p, const LinearArgs& a, const unsigned char* digits,
                                u32* slots) {
-    cudaError_t e = cudaFuncSetAttribute(linear_bytes_kernel<W_COPY, X_FILL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 201 * 1024);
+    cudaError_t e = allow_smem(linear_bytes_kernel<W_COPY, X_FILL>, 201 * 1024);
     if (e != cudaSuccess) return e;
     const int x_vec = a.n % 4 == 0 && a.x_stride % 4 == 0 && !((uintptr_t)a.x & 15);
     const dim3 block(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL));

@@ -45,8 +45,10 @@ struct PagedAttnArgs {
     uint32_t* out;                                           // [num_seqs][num_heads][d]
     int32_t* status;
     void* workspace;
+    void* counters;                                          // paged_attention_counters bytes, zero before and after every call; NULL: the first of the workspace
     int* gave_up;                                            // set when a wait inside a kernel ran out
 };
+size_t paged_attention_counters(int sm_count);
 size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs);
 cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const PagedAttnArgs& a, int* launches);
 

@@ -2,9 +2,28 @@
 // shared memory, TMEM, and kind::i8 matrix instructions on unsigned bytes with 32-bit accumulators.
 #pragma once
 #include <cuda.h>
+#include <map>
+#include <mutex>
+#include <utility>
 #include "m31.cuh"
 
 namespace zkb {
+
+// Let a kernel use `bytes` of dynamic shared memory; once per kernel, size and device.
+template <class... KArgs>
+inline cudaError_t allow_smem(void (*kernel)(KArgs...), size_t bytes) {
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, size_t> allowed;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> g(mu);
+    size_t& have = allowed[{(const void*)kernel, device}];
+    if (have >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) have = bytes;
+    return e;
+}
 
 __device__ __forceinline__ u32 smem_addr(const void* p) { return (u32)__cvta_generic_to_shared(p); }
 

@@ -92,6 +92,7 @@ void zkb_ctx_destroy(zkb_ctx* c) {
     if (c->stage) cudaFreeHost(c->stage);
     if (c->tr_host) cudaFreeHost(c->tr_host);
     if (c->serve_gave_up) cudaFreeHost(c->serve_gave_up);
+    if (c->serve_counters) cudaFree(c->serve_counters);
     if (c->lifted) cudaStreamDestroy(c->lifted);
     if (c->stream) cudaStreamDestroy(c->stream);
     delete c;
@@ -109,6 +110,7 @@ int32_t zkb_ctx_sync(zkb_ctx* c) {
         ZKB_CUDA(cudaStreamSynchronize(c->stream));
         if (c->serve_gave_up && *(volatile int*)c->serve_gave_up) {
             *c->serve_gave_up = 0;
+            if (c->serve_counters) ZKB_CUDA(cudaMemset(c->serve_counters, 0, zkb::paged_attention_counters(c->sm_count)));
             throw ArgFail{ZKB_E_TIMEOUT, "a wait inside a kernel ran out: results of this context since its last synchronisation are not valid"};
         }
     });
