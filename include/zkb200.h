@@ -565,7 +565,7 @@ typedef struct {
 /* Keys and values of new tokens into the cache.  k, v: (num_tokens, num_kv_heads, d_head), tokens *_stride words apart (0: dense).  Sequence s
  * brings the tokens row_start[s] .. row_start[s + 1] - 1 (num_seqs + 1 nondecreasing entries); they get the positions from start[s] on, and
  * position p lies in row p % page_size of page block_table[s][p / page_size] (num_seqs x max_blocks entries; places that no new position needs
- * may hold anything).  Tokens before row_start[0] and from row_start[num_seqs] on are padding: nothing is read or written for them.  With a
+ * may hold anything).  Tokens before row_start[0] and from row_start[num_seqs] on are padding: nothing is written for them.  With a
  * rotation (NULL: none) K is rotated by its position, and q (num_tokens, num_heads, d_head) into q_out, which may be q itself; without one q is
  * copied.  Two sequences that append into one page in one call must not share its rows.  A token whose page or position is refused
  * (status) is left out; a value that does not fit a 16-bit cache is stored as its low 16 bits and reported. */

@@ -22,25 +22,118 @@ __device__ __forceinline__ u32 round_to_field(long long x, u32 shift) {
     return x < 0 ? neg31(r) : r;
 }
 
-// One CTA: one token, the rows (heads of k, v, q) y, y + gridDim.y, ... by warp.
-__global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs A) {
-    const u32 t = blockIdx.x;
-    u32 seq = 0;
+// Where a token goes.  All threads of the CTA call it; false: padding, or refused (and reported).
+struct AppendPlace { u32 seq; long long pos; int page; };
+__device__ __forceinline__ bool append_place(const AppendArgs& A, u32 t, AppendPlace& p) {
+    p.seq = 0;                                                // sequences that end before t
     for (u32 base = 0; base < A.num_seqs; base += APPEND_THREADS) {
         const u32 s = base + threadIdx.x;
-        seq += __syncthreads_count(s < A.num_seqs && A.row_start[s + 1] <= (int)t);
+        p.seq += __syncthreads_count(s < A.num_seqs && A.row_start[s + 1] <= (int)t);
     }
-    if (seq >= A.num_seqs) return;                            // behind the last sequence
-    const int first = A.row_start[seq];
-    if ((int)t < first) return;
-    const long long pos = (long long)A.start[seq] + ((int)t - first);
-    const long long block = pos >> A.c.page_bits;
-    const int page = pos >= 0 && block < A.max_blocks ? A.block_table[(size_t)seq * A.max_blocks + block] : -1;
-    const bool have_page = page >= 0 && (u32)page < A.c.num_pages, have_rot = A.rot == 0 || (pos >= 0 && pos < A.positions);
-    if (!have_page || !have_rot) {
-        if (threadIdx.x == 0) atomicMax(A.status + seq, have_page ? SERVE_ROTATION : SERVE_PAGE);
-        return;
+    if (p.seq >= A.num_seqs) return false;                    // behind the last sequence
+    const int first = A.row_start[p.seq];
+    if ((int)t < first) return false;
+    p.pos = (long long)A.start[p.seq] + ((int)t - first);
+    const long long block = p.pos >> A.c.page_bits;
+    p.page = p.pos >= 0 && block < A.max_blocks ? A.block_table[(size_t)p.seq * A.max_blocks + block] : -1;
+    const bool have_page = p.page >= 0 && (u32)p.page < A.c.num_pages, have_rot = A.rot == 0 || (p.pos >= 0 && p.pos < A.positions);
+    if (have_page && have_rot) return true;
+    if (threadIdx.x == 0) atomicMax(A.status + p.seq, have_page ? SERVE_ROTATION : SERVE_PAGE);
+    return false;
+}
+__device__ __forceinline__ void rotate_pair(u32& a, u32& b, int c, int s, u32 shift) {
+    const long long x = centred32(a), y = centred32(b);
+    a = round_to_field(x * c - y * s, shift);
+    b = round_to_field(x * s + y * c, shift);
+}
+
+// 16 bytes at a time, for rows, rotations and addresses that are whole groups of 16 bytes (see kv_append_launch).  What bounds it is the copy: K, V and
+// Q in, the cache and Q out.  A row has `items` items: four neighbours, or where halves turn four elements and their four partners; a thread has the same item in
+// every row that it takes, so its cosines and sines stay in registers.  The first rows are read before the place is looked up.
+// 8111 tokens of 32 + 2 x 8 heads of 128 into a field cache (390 MB): 5.7 TB/s.
+template <bool SMALL, bool PAIRS>
+__global__ void __launch_bounds__(APPEND_THREADS) kv_append_vec_kernel(AppendArgs A, u32 items, u32 rot_items) {
+    constexpr u32 BATCH = 3;
+    const u32 t = blockIdx.x, d = A.c.d, kv = A.c.num_kv_heads, half = A.rot / 2, rows = 2 * kv + (A.q ? A.num_heads : 0);
+    const u32 per_pass = APPEND_THREADS / items, item = threadIdx.x % items, in_pass = threadIdx.x / items, step = gridDim.y * per_pass;
+    const bool turns = item < rot_items, two = !PAIRS && turns;
+    const u32 e0 = PAIRS || turns ? 4 * item : A.rot + 4 * (item - rot_items), e1 = half + 4 * item;
+    u32 row = in_pass < per_pass ? blockIdx.y * per_pass + in_pass : rows;
+    uint4 a[BATCH], b[BATCH];
+    auto load = [&](u32 from_row) {
+#pragma unroll
+        for (u32 k = 0; k < BATCH; k++) {
+            const u32 r = from_row + k * step;
+            if (r >= rows) break;
+            const u32* src = r < kv ? A.k + t * A.k_stride + (size_t)r * d : r < 2 * kv ? A.v + t * A.v_stride + (size_t)(r - kv) * d : A.q + t * A.q_stride + (size_t)(r - 2 * kv) * d;
+            a[k] = *reinterpret_cast<const uint4*>(src + e0);
+            if (two) b[k] = *reinterpret_cast<const uint4*>(src + e1);
+        }
+    };
+    load(row);
+    AppendPlace p;
+    if (!append_place(A, t, p)) return;
+    int4 cs0 = make_int4(0, 0, 0, 0), cs1 = cs0;              // cos, sin of two pairs each
+    if (turns) {
+        const int4* cs = reinterpret_cast<const int4*>(A.cos_sin + (size_t)p.pos * A.rot + (PAIRS ? 4 : 8) * item);
+        cs0 = cs[0];
+        if (!PAIRS) cs1 = cs[1];
     }
+    const size_t at = (size_t)p.page * A.c.page_stride + (size_t)(p.pos & ((1u << A.c.page_bits) - 1)) * d;
+    bool out_of_range = false;
+    while (row < rows) {
+#pragma unroll
+        for (u32 k = 0; k < BATCH; k++) {
+            const u32 r = row + k * step;
+            if (r >= rows) break;
+            const bool is_k = r < kv, is_v = !is_k && r < 2 * kv;
+            if (turns && !is_v) {
+                if (PAIRS) {
+                    rotate_pair(a[k].x, a[k].y, cs0.x, cs0.y, A.shift);
+                    rotate_pair(a[k].z, a[k].w, cs0.z, cs0.w, A.shift);
+                } else {
+                    rotate_pair(a[k].x, b[k].x, cs0.x, cs0.y, A.shift);
+                    rotate_pair(a[k].y, b[k].y, cs0.z, cs0.w, A.shift);
+                    rotate_pair(a[k].z, b[k].z, cs1.x, cs1.y, A.shift);
+                    rotate_pair(a[k].w, b[k].w, cs1.z, cs1.w, A.shift);
+                }
+            }
+            if (!is_k && !is_v) {
+                u32* to = A.q_out + t * A.q_out_stride + (size_t)(r - 2 * kv) * d;
+                *reinterpret_cast<uint4*>(to + e0) = a[k];
+                if (two) *reinterpret_cast<uint4*>(to + e1) = b[k];
+                continue;
+            }
+            const size_t to = at + ((size_t)(is_k ? r : r - kv) << A.c.page_bits) * d;
+            if (SMALL) {
+                auto put = [&](u32 e, const uint4& v) {
+                    const int z[4] = {centred32(v.x), centred32(v.y), centred32(v.z), centred32(v.w)};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) out_of_range |= z[i] != (int)(int16_t)z[i];
+                    *reinterpret_cast<uint2*>((int16_t*)(is_k ? A.c.k : A.c.v) + to + e) = make_uint2(__byte_perm(z[0], z[1], 0x5410), __byte_perm(z[2], z[3], 0x5410));
+                };
+                put(e0, a[k]);
+                if (two) put(e1, b[k]);
+            } else {
+                u32* pages = (u32*)(is_k ? A.c.k : A.c.v) + to;
+                *reinterpret_cast<uint4*>(pages + e0) = a[k];
+                if (two) *reinterpret_cast<uint4*>(pages + e1) = b[k];
+            }
+        }
+        row += BATCH * step;
+        load(row);
+    }
+    if (out_of_range) atomicMax(A.status + p.seq, SERVE_RANGE);
+}
+
+// Any sizes and alignment.  One CTA: one token, the rows (heads of k, v, q) y, y + gridDim.y, ... by warp.
+__global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs A) {
+    const u32 t = blockIdx.x;
+    AppendPlace place;
+    if (!append_place(A, t, place)) return;
+    const u32 seq = place.seq;
+    const long long pos = place.pos;
+    const int page = place.page;
     const u32 d = A.c.d, kv = A.c.num_kv_heads, half = A.rot / 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const u32 rows = 2 * kv + (A.q ? A.num_heads : 0);
     const int* cs = A.cos_sin + (size_t)pos * A.rot;
@@ -65,9 +158,10 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs A)
         const u32 rot = is_v ? 0 : A.rot;
         for (u32 p = lane; p < rot / 2; p += 32) {             // both of a pair by one thread: q may be rotated in place
             const u32 i = A.pairs ? 2 * p : p, j = A.pairs ? 2 * p + 1 : p + half;
-            const long long c = cs[2 * p], s = cs[2 * p + 1], x = centred32(src[i]), y = centred32(src[j]);
-            put(i, round_to_field(x * c - y * s, A.shift));
-            put(j, round_to_field(x * s + y * c, A.shift));
+            u32 x = src[i], y = src[j];
+            rotate_pair(x, y, cs[2 * p], cs[2 * p + 1], A.shift);
+            put(i, x);
+            put(j, y);
         }
         for (u32 i = rot + lane; i < d; i += 32) put(i, src[i]);
     }

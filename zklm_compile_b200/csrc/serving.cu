@@ -8,7 +8,21 @@ namespace zkb {
 
 cudaError_t kv_append_launch(cudaStream_t stream, int sm_count, const AppendArgs& a, int* launches) {
     const u32 rows = 2 * a.c.num_kv_heads + (a.q ? a.num_heads : 0);
-    kv_append_kernel<<<dim3(a.num_tokens, (rows + 7) / 8), APPEND_THREADS, 0, stream>>>(a);
+    const uintptr_t words = (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q | (uintptr_t)a.q_out | (uintptr_t)a.cos_sin | (a.c.small ? 0 : (uintptr_t)a.c.k | (uintptr_t)a.c.v);
+    const uint64_t strides = a.k_stride | a.v_stride | a.q_stride | a.q_out_stride | a.c.page_stride | a.c.d;
+    const bool vec = !(words & 15) && !(((uintptr_t)a.c.k | (uintptr_t)a.c.v) & 7) && strides % 4 == 0 && a.rot % (a.pairs ? 4 : 8) == 0;
+    if (vec) {
+        const u32 rot_items = a.pairs ? a.rot / 4 : a.rot / 8, items = a.pairs ? a.c.d / 4 : rot_items + (a.c.d - a.rot) / 4;
+        // as many CTAs a token as give every SM a few; one for many tokens, which then amortises the look-up
+        const u32 per_pass = APPEND_THREADS / items, passes = (rows + per_pass - 1) / per_pass, want = ((u32)sm_count * 4 + a.num_tokens - 1) / a.num_tokens;
+        const dim3 grid(a.num_tokens, want < passes ? want : passes);
+        if (a.c.small && a.pairs) kv_append_vec_kernel<true, true><<<grid, APPEND_THREADS, 0, stream>>>(a, items, rot_items);
+        else if (a.c.small) kv_append_vec_kernel<true, false><<<grid, APPEND_THREADS, 0, stream>>>(a, items, rot_items);
+        else if (a.pairs) kv_append_vec_kernel<false, true><<<grid, APPEND_THREADS, 0, stream>>>(a, items, rot_items);
+        else kv_append_vec_kernel<false, false><<<grid, APPEND_THREADS, 0, stream>>>(a, items, rot_items);
+    } else {
+        kv_append_kernel<<<dim3(a.num_tokens, (rows + 7) / 8), APPEND_THREADS, 0, stream>>>(a);
+    }
     ++*launches;
     return cudaGetLastError();
 }
