@@ -14,12 +14,12 @@ namespace zkb {
 constexpr int APPEND_THREADS = 256;
 
 __device__ __forceinline__ int centred32(u32 v) { return v > ZKB_P / 2 ? (int)(v - ZKB_P) : (int)v; }
-// |x| <= 2^62 -> (rounded half away from zero) mod p
+// |x| <= 2^62 -> x / 2^shift rounded half away from zero, mod p.  Half less one unit, where x is negative, makes the floor of a shift round away from zero there too;
+// 2^32 p = 2^63 - 2^32 makes the sum positive.
 __device__ __forceinline__ u32 round_to_field(long long x, u32 shift) {
-    u64 m = (u64)(x < 0 ? -x : x);
-    if (shift) m = (m + (1ull << (shift - 1))) >> shift;
-    const u32 r = red64(m);
-    return x < 0 ? neg31(r) : r;
+    const long long away = shift ? x >> 63 : 0;
+    const long long y = (x + (long long)((1ull << shift) >> 1) + away) >> shift;
+    return red64((u64)y + ((u64)ZKB_P << 32));
 }
 
 // Where a token goes.  All threads of the CTA call it; false: padding, or refused (and reported).
@@ -52,11 +52,14 @@ __device__ __forceinline__ void rotate_pair(u32& a, u32& b, int c, int s, u32 sh
 // every row that it takes, so its cosines and sines stay in registers.  The first rows are read before the place is looked up.
 // 8111 tokens of 32 + 2 x 8 heads of 128 into a field cache (390 MB): 5.7 TB/s.
 template <bool SMALL, bool PAIRS>
-__global__ void __launch_bounds__(APPEND_THREADS) kv_append_vec_kernel(AppendArgs A, u32 items, u32 rot_items) {
-    constexpr u32 BATCH = 3;
+__global__ void __launch_bounds__(APPEND_THREADS, 4) kv_append_vec_kernel(AppendArgs A, u32 items, u32 rot_items) {
+    constexpr u32 BATCH = PAIRS ? 6 : 3;                       // rows under way, 16 bytes or 32 of each
     const u32 t = blockIdx.x, d = A.c.d, kv = A.c.num_kv_heads, half = A.rot / 2, rows = 2 * kv + (A.q ? A.num_heads : 0);
-    const u32 per_pass = APPEND_THREADS / items, item = threadIdx.x % items, in_pass = threadIdx.x / items, step = gridDim.y * per_pass;
-    const bool turns = item < rot_items, two = !PAIRS && turns;
+    const u32 per_pass = APPEND_THREADS / items, step = gridDim.y * per_pass, turning = per_pass * rot_items;
+    // the first threads have the items that turn, so that few warps have both kinds
+    const bool turns = threadIdx.x < turning, two = !PAIRS && turns;
+    const u32 still = items - rot_items, rest = threadIdx.x - turning;
+    const u32 item = turns ? threadIdx.x % rot_items : still ? rot_items + rest % still : 0, in_pass = turns ? threadIdx.x / rot_items : still ? rest / still : per_pass;
     const u32 e0 = PAIRS || turns ? 4 * item : A.rot + 4 * (item - rot_items), e1 = half + 4 * item;
     u32 row = in_pass < per_pass ? blockIdx.y * per_pass + in_pass : rows;
     uint4 a[BATCH], b[BATCH];
@@ -66,8 +69,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_vec_kernel(AppendArg
             const u32 r = from_row + k * step;
             if (r >= rows) break;
             const u32* src = r < kv ? A.k + t * A.k_stride + (size_t)r * d : r < 2 * kv ? A.v + t * A.v_stride + (size_t)(r - kv) * d : A.q + t * A.q_stride + (size_t)(r - 2 * kv) * d;
-            a[k] = *reinterpret_cast<const uint4*>(src + e0);
-            if (two) b[k] = *reinterpret_cast<const uint4*>(src + e1);
+            a[k] = __ldcs(reinterpret_cast<const uint4*>(src + e0));
+            if (two) b[k] = __ldcs(reinterpret_cast<const uint4*>(src + e1));
         }
     };
     load(row);
@@ -100,8 +103,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_vec_kernel(AppendArg
             }
             if (!is_k && !is_v) {
                 u32* to = A.q_out + t * A.q_out_stride + (size_t)(r - 2 * kv) * d;
-                *reinterpret_cast<uint4*>(to + e0) = a[k];
-                if (two) *reinterpret_cast<uint4*>(to + e1) = b[k];
+                __stcs(reinterpret_cast<uint4*>(to + e0), a[k]);
+                if (two) __stcs(reinterpret_cast<uint4*>(to + e1), b[k]);
                 continue;
             }
             const size_t to = at + ((size_t)(is_k ? r : r - kv) << A.c.page_bits) * d;
