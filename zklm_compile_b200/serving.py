@@ -51,15 +51,26 @@ def _fn(name):
     return f
 
 
-def _count(v, what: str, most: int = 0xffffffff) -> int:
-    v = int(v)
-    if not 0 <= v <= most:
-        raise ValueError(f"{what}: {v} is not in [0, {most}]")
-    return v
+def _counts(**sizes) -> None:
+    """Every size fits the C interface's unsigned 32 bits."""
+    for what, v in sizes.items():
+        if not 0 <= v <= 0xffffffff:
+            raise ValueError(f"{what}: {v} is not in [0, 2^32)")
 
 
 def _addr(ctx: Context, x, least: int, what: str, size: int = 4) -> int:
     """Address of a device array of at least `least` elements of `size` bytes."""
+    if type(x) is not DeviceBuffer:
+        try:
+            if x.nbytes >= least * size and x.itemsize == size and x.get_device() == ctx.device and x.is_contiguous():
+                return x.data_ptr()
+        except AttributeError:
+            pass
+    return _addr_or_why(ctx, x, least, what, size)
+
+
+def _addr_or_why(ctx: Context, x, least: int, what: str, size: int) -> int:
+    """The same for DeviceBuffers and other libraries' tensors, and what is wrong with an array that cannot be taken."""
     if isinstance(x, DeviceBuffer):
         if x.ctx.device != ctx.device:
             raise ValueError(f"{what} lies on another GPU than the context")
@@ -67,11 +78,8 @@ def _addr(ctx: Context, x, least: int, what: str, size: int = 4) -> int:
         at = C.cast(x.ptr, C.c_void_p).value or 0
     else:
         try:
-            at = x.data_ptr()
-            unit = x.element_size()
+            at, unit, dense, on = x.data_ptr(), x.element_size(), x.is_contiguous(), x.get_device()
             have = x.numel() * unit
-            on = x.get_device()
-            dense = x.is_contiguous()
         except AttributeError:
             raise TypeError(f"{what}: a DeviceBuffer or a tensor on the GPU is wanted, not {type(x).__name__}") from None
         if on != ctx.device:
@@ -85,9 +93,11 @@ def _addr(ctx: Context, x, least: int, what: str, size: int = 4) -> int:
 
 def _rows(count: int, row: int, stride: int) -> int:
     """Elements that `count` rows of `row` reach over, `stride` apart (0: dense)."""
-    if stride and stride < row:
+    if not stride:
+        return count * row
+    if stride < row:
         raise ValueError(f"a stride of {stride} is less than a row of {row}")
-    return (count - 1) * (stride or row) + row if count else 0
+    return (count - 1) * stride + row if count else 0
 
 
 class KvCache:
@@ -135,8 +145,8 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
     """Put k, v (num_tokens, num_kv_heads, d_head) into the cache: sequence s brings tokens row_start[s] .. row_start[s + 1] - 1, which get the positions
     from start[s] on; position p is row p % page_size of page block_table[s][p / page_size].  With a rotation K turns by its position, and so does
     q (num_tokens, num_heads, d_head) on its way to q_out (which may be q).  Rows outside every sequence are padding and left alone."""
-    ctx, t, s = cache.ctx, _count(num_tokens, "num_tokens"), _count(num_seqs, "num_seqs")
-    blocks, heads, row = _count(max_blocks, "max_blocks"), _count(num_heads, "num_heads"), cache.num_kv_heads * cache.d_head
+    ctx, t, s, blocks, heads, row = cache.ctx, num_tokens, num_seqs, max_blocks, num_heads, cache.num_kv_heads * cache.d_head
+    _counts(num_tokens=t, num_seqs=s, max_blocks=blocks, num_heads=heads)
     if (q is None) != (q_out is None):
         raise ValueError("q and q_out: both or neither")
     rot = None
@@ -152,8 +162,10 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
 
 
 def paged_attention_workspace(cache: KvCache, num_seqs: int, num_heads: int) -> int:
-    """Bytes of workspace for calls of this size (a captured call needs one of its own, 256-byte aligned)."""
-    return int(_fn("zkb_paged_attention_workspace")(cache.ctx.h, cache._at, _count(num_seqs, "num_seqs"), _count(num_heads, "num_heads")))
+    """Bytes of workspace for calls of this size: a captured call needs one of its own, 256-byte aligned, zeroed once before its first call and used by this
+    operator alone from then on."""
+    _counts(num_seqs=num_seqs, num_heads=num_heads)
+    return int(_fn("zkb_paged_attention_workspace")(cache.ctx.h, cache._at, num_seqs, num_heads))
 
 
 def paged_attention(cache: KvCache, q, block_table, num_seqs: int, max_blocks: int, lens, num_heads: int, exp_table, out, status, score_shift: int = 0,
@@ -161,28 +173,31 @@ def paged_attention(cache: KvCache, q, block_table, num_seqs: int, max_blocks: i
     """One new token per sequence: q (num_seqs, num_heads, d_head) over the first lens[s] positions of the cache, into out (num_seqs, num_heads, d_head).
     The score q . k_j, divided by 2^score_shift and rounded half away from zero, must be an input of the exp table; a sequence of length 0 and a
     row that is refused (status) give zeros."""
-    ctx, s, blocks, heads = cache.ctx, _count(num_seqs, "num_seqs"), _count(max_blocks, "max_blocks"), _count(num_heads, "num_heads")
-    row = heads * cache.d_head
+    ctx, s, blocks, heads, row = cache.ctx, num_seqs, max_blocks, num_heads, num_heads * cache.d_head
+    _counts(num_seqs=s, max_blocks=blocks, num_heads=heads, score_shift=score_shift)
     check(ctx.h, _fn("zkb_paged_attention")(
         ctx.h, cache._at, _addr(ctx, q, _rows(s, row, q_stride), "q"), q_stride, heads, _addr(ctx, block_table, s * blocks, "block_table"), s, blocks,
-        _addr(ctx, lens, s, "lens"), _addr(ctx, exp_table, n_table, "exp_table"), n_table, _count(score_shift, "score_shift"), _addr(ctx, out, s * row, "out"),
+        _addr(ctx, lens, s, "lens"), _addr(ctx, exp_table, n_table, "exp_table"), n_table, score_shift, _addr(ctx, out, s * row, "out"),
         _addr(ctx, status, s, "status"), *_workspace(ctx, workspace)))
 
 
 def adapter_linear_workspace(ctx: Context, tokens: int, m: int, n: int, num_adapters: int = 0, rank: int = 0) -> int:
-    return int(_fn("zkb_adapter_linear_workspace")(ctx.h, *(_count(v, "a size") for v in (tokens, m, n, num_adapters, rank))))
+    """Bytes of workspace for calls of this size; more tokens may need less than fewer, so ask for the size that is called."""
+    _counts(tokens=tokens, m=m, n=n, num_adapters=num_adapters, rank=rank)
+    return int(_fn("zkb_adapter_linear_workspace")(ctx.h, tokens, m, n, num_adapters, rank))
 
 
 def adapter_linear(ctx: Context, x, w, tokens: int, m: int, n: int, out, bias=None, adapters: Adapters | None = None, adapter_of=None, x_stride: int = 0,
                    out_stride: int = 0, workspace=None) -> None:
     """out[t] = W x[t] + bias + B[a] (A[a] x[t]), a = adapter_of[t] (outside the adapters: none), for `tokens` rows x of n words; W is m x n, row-major."""
-    tokens, m, n = _count(tokens, "tokens"), _count(m, "m"), _count(n, "n")
+    _counts(tokens=tokens, m=m, n=n)
     if (adapters is None) != (adapter_of is None):
         raise ValueError("adapters and adapter_of: both or neither")
     a = b = of = None
     count = rank = 0
     if adapters is not None:
-        count, rank = _count(adapters.count, "adapters"), _count(adapters.rank, "rank")
+        count, rank = adapters.count, adapters.rank
+        _counts(adapters=count, rank=rank)
         a, b, of = _addr(ctx, adapters.a, count * rank * n, "A"), _addr(ctx, adapters.b, count * m * rank, "B"), _addr(ctx, adapter_of, tokens, "adapter_of")
     check(ctx.h, _fn("zkb_adapter_linear")(
         ctx.h, _addr(ctx, x, _rows(tokens, n, x_stride), "x"), x_stride, _addr(ctx, w, m * n, "w"), _addr(ctx, bias, m, "bias") if bias is not None else None, tokens, m,
