@@ -20,7 +20,9 @@ constexpr u32 LIN_STEP = 32;                   // columns of W per step: 128 byt
 constexpr u32 LIN_SEG = 256;                   // steps after which the accumulators are emptied (8192 columns)
 constexpr u32 LIN_TOKENS = 64;                 // tokens per tile at most: 256 columns of an accumulator
 constexpr u32 LIN_MAX_STAGES = 8;
-constexpr u32 LIN_FILL = 128;                  // threads that fill operands by plain stores, where a kernel has such
+constexpr u32 LIN_FILL = 8;                     // warps that fill operands by plain stores, two a step
+constexpr u32 LIN_THREADS = (6 + LIN_FILL) * 32;
+constexpr u32 LIN_CHUNK = 2048;                // tokens of one pass
 
 // Byte c of the four rotations of x by 8i, i = 0 .. 3, for c = 0 .. 3.  All of them are bytes of x, of x >> 7, or of x without the top bits of its bytes.
 __device__ __forceinline__ void digit_words(u32 x, u32 (&w)[4]) {
@@ -66,38 +68,9 @@ inline u32 lin_a_rows(u32 tokens, u32 m, u32 num_adapters, u32 rank) {
     const u64 rows = (u64)num_adapters * rank, tiles = (rows + LIN_ROWS - 1) / LIN_ROWS, wtiles = (m + LIN_ROWS - 1) / LIN_ROWS;
     return rows && (tiles <= (wtiles < 8 ? 1 : wtiles / 8) || tiles * LIN_ROWS <= (u64)tokens * rank / 2) && rows < (1u << 30) ? (u32)rows : 0u;
 }
-// Tokens of one pass: their operand (16 bytes a value) is read by every row of tiles and should stay in L2.
-inline u32 lin_chunk(u32 tokens, u32 n) {
-    const u64 fit = ((u64)64 << 20) / ((u64)(n + LIN_STEP - 1) / LIN_STEP * LIN_STEP * 16) / LIN_TOKENS * LIN_TOKENS;
-    const u32 most = fit < LIN_TOKENS ? LIN_TOKENS : (fit > 2048 ? 2048u : (u32)fit);
-    return tokens < most ? tokens : most;
-}
-inline bool lin_fused(const LinPlan& p) { return p.ntiles == 1; }
-inline size_t lin_digit_bytes(const LinPlan& p) { return lin_fused(p) ? 0 : (size_t)p.ntiles * p.steps * p.tt * 512; }
+inline u32 lin_chunk(u32 tokens) { return tokens < LIN_CHUNK ? tokens : LIN_CHUNK; }
 // For any number of tokens up to the plan's: fewer of them may be shared by more CTAs.
 inline size_t lin_slot_bytes(int sm_count, const LinPlan& p) { return ((size_t)sm_count + (size_t)p.mtiles * p.ntiles * p.segs) * p.slot_words * 4; }
-
-// The tokens' operand, in the order in which the tiles are copied: per (tile of tokens, step) 4 tt rows of 128 bytes, swizzled.
-__global__ void __launch_bounds__(512) linear_digits_kernel(const u32* __restrict__ x, u64 x_stride, LinPlan p, unsigned char* __restrict__ out) {
-    pdl_launch_dependents();
-    const u32 step = blockIdx.x, nt = blockIdx.y, tok = threadIdx.x >> 3, q = threadIdx.x & 7;
-    const u32 t = nt * p.tt + tok, j = step * LIN_STEP + 4 * q;
-    unsigned char* tile = out + ((size_t)nt * p.steps + step) * p.tt * 512;
-    u32 w[4][4];
-#pragma unroll
-    for (u32 e = 0; e < 4; e++) {
-        const u32 v = t < p.tokens && j + e < p.n ? x[t * x_stride + j + e] : 0u;
-        u32 d[4];
-        digit_words(v, d);
-#pragma unroll
-        for (int c = 0; c < 4; c++) w[c][e] = d[c];
-    }
-#pragma unroll
-    for (u32 c = 0; c < 4; c++) {
-        const u32 r = 4 * tok + c;
-        *reinterpret_cast<uint4*>(tile + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
-    }
-}
 
 struct LinWalk {                               // a CTA's stretches, the same for every role
     const LinPlan& p;
@@ -118,14 +91,12 @@ struct LinWalk {                               // a CTA's stretches, the same fo
     }
 };
 
-// Warp 0 copies, warp 1 issues, warps 2 to 5 empty the accumulators, and where W or the tokens' operand is filled by plain stores warps 6 to 9 do that.
-// W_COPY: W by tensor copies; otherwise (rows that start on no 16-byte boundary) word by word.  X_FILL: the tokens' operand is made here from x,
-// which for one tile of tokens costs less than copying its 16 bytes a value; otherwise it is copied from where linear_digits_kernel left it.
-template <bool W_COPY, bool X_FILL>
-__global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) linear_bytes_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a,
-                                                                                              LinPlan p, LinearArgs A, int x_vec, const unsigned char* __restrict__ digits,
-                                                                                              u32* __restrict__ slots) {
-    constexpr bool FILL = !W_COPY || X_FILL;
+// Warp 0 copies W, warp 1 issues, warps 2 to 5 empty the accumulators, the others make the tokens' operand from x: 16 bytes of it a value, which would
+// be four times x to copy (that was bound by L2: 0.92 us a step of 64 KB at 256 columns).  W_COPY: W by tensor copies; otherwise (rows that start on no
+// 16-byte boundary) word by word, by the warps that fill.
+template <bool W_COPY>
+__global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, LinPlan p, LinearArgs A, int x_vec,
+                                                                   u32* __restrict__ slots) {
     extern __shared__ __align__(16) unsigned char lin_raw[];
     __shared__ __align__(8) u64 bars[2 * LIN_MAX_STAGES + 2];
     __shared__ u32 tmem_base;
@@ -135,7 +106,7 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
     const u32 base = smem_addr(smem);
     const u32 full = smem_addr(bars), empty = full + 8 * LIN_MAX_STAGES, acc_full = empty + 8 * LIN_MAX_STAGES, acc_empty = acc_full + 8;
     if (threadIdx.x == 0) {
-        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, FILL ? 2 : 1); mbar_init(empty + 8 * s, 1); }
+        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 3); mbar_init(empty + 8 * s, 1); }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 4);
         gave_up = 0;
@@ -146,27 +117,24 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
     __syncthreads();
     tc_fence_after();
     pdl_launch_dependents();
-    const u32 tmem = tmem_base, b_bytes = p.tt * 512;
+    const u32 tmem = tmem_base;
     LinWalk walk(p);
     if (warp == 0) {
         if (lane == 0) {
             u32 it = 0;
             bool ok = true;
-            if (!X_FILL) pdl_wait();             // the digits come from the kernel before this one
             while (ok && walk.next()) {
                 const bool of_w = walk.mt < p.wtiles;
                 const int row = (int)((of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS);
                 for (u32 k = 0; k < walk.count; k++, it++) {
                     const u32 s = it % p.stages, round = it / p.stages, st = base + s * p.stage_bytes;
                     if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
-                    mbar_expect(full + 8 * s, (W_COPY ? LIN_ROWS * 128 : 0u) + (X_FILL ? 0u : b_bytes));
+                    mbar_expect(full + 8 * s, W_COPY ? LIN_ROWS * 128 : 0u);
                     if (W_COPY) tensor_load_2d(st, of_w ? &map_w : &map_a, (int)((walk.first + k) * LIN_STEP), row, full + 8 * s);
-                    if (!X_FILL) bulk_load(st + LIN_ROWS * 128, digits + ((size_t)walk.nt * p.steps + walk.first + k) * b_bytes, b_bytes, full + 8 * s);
                 }
             }
-            // Where x is read directly, the kernel before this one (if it is one of the same call) makes what the join reads: the join, which waits for this
-            // kernel, must find it done.
-            if (X_FILL) pdl_wait();
+            // The kernel before this one (where it is one of the same call) makes what the join reads: the join, which waits for this kernel, must find it done.
+            pdl_wait();
             if (!ok)                             // given up: nothing of this CTA may still be in flight when it ends
                 for (u32 i = it > p.stages ? it - p.stages : 0; i < it; i++)
                     for (u32 n = 0; n < (1u << 16) && !mbar_try(full + 8 * (i % p.stages), (i / p.stages) & 1); n++) {}
@@ -231,74 +199,72 @@ __global__ void __launch_bounds__(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL)) line
             if (lane == 0) mbar_arrive(acc_empty);
             n++;
         }
-    } else if (FILL) {
-        // Each warp takes every fourth step, so that four steps' loads are under way - but no more warps than stages: a warp knows that the stage of its last
-        // step was empty, and from that that its next one's was emptied the time before last; with fewer stages than warps it could be two phases ahead, where
-        // a wait by parity sees the wrong one.
-        const u32 fillers = p.stages < LIN_FILL / 32 ? p.stages : LIN_FILL / 32;
-        // A warp's groups of four values of x, fetched a turn ahead: token 4 i + lane / 8, columns 4 (lane & 7) .. of its next step.  A step's columns of x
-        // are the same whatever tile it belongs to.
-        u32 x[X_FILL ? LIN_TOKENS / 4 : 1][4];
-        u32 ahead = blockIdx.x * p.per + (warp - 6);
+    } else {
+        // Each pair of warps takes every fourth step, so that four steps' loads are under way - but no more pairs than stages: a pair knows that the stage of
+        // its last step was empty, and from that that its next one's was emptied the time before last; with fewer stages than pairs it could be two phases
+        // ahead, where a wait by parity sees the wrong one.
+        const u32 pairs = p.stages < LIN_FILL / 2 ? p.stages : LIN_FILL / 2, pair = (warp - 6) >> 1, half = warp & 1;
+        constexpr u32 GROUPS = LIN_TOKENS / 8;
+        // A warp's groups of four values of x, fetched a turn ahead: token 4 (2 i + half) + lane / 8 of the tile, columns 4 (lane & 7) .. of its next step.
+        u32 x[GROUPS][4];
+        u32 ahead = blockIdx.x * p.per + pair;
         auto fetch = [&] {
-            if (!X_FILL || ahead >= walk.end) return;
-            const u32 j = ahead % p.steps * LIN_STEP + 4 * (lane & 7);
+            if (ahead >= walk.end) return;
+            const u32 tile = ahead / p.steps, j = (ahead - tile * p.steps) * LIN_STEP + 4 * (lane & 7), tok0 = tile % p.ntiles * p.tt;
 #pragma unroll
-            for (u32 i = 0; i < LIN_TOKENS / 4; i++) {
-                if (4 * i >= p.tt) break;
-                const u32 t = 4 * i + (lane >> 3);
+            for (u32 i = 0; i < GROUPS; i++) {
+                const u32 in = 4 * (2 * i + half) + (lane >> 3), t = tok0 + in;
+                const bool there = in < p.tt && t < p.tokens;
                 const u32* at = A.x + t * A.x_stride + j;
-                if (x_vec && t < p.tokens && j + 4 <= p.n) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at);
+                if (x_vec) {                     // n is a multiple of 4 then
+                    const uint4 v = there && j < p.n ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
                     x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
                 } else {
 #pragma unroll
-                    for (u32 e = 0; e < 4; e++) x[i][e] = t < p.tokens && j + e < p.n ? at[e] : 0u;
+                    for (u32 e = 0; e < 4; e++) x[i][e] = there && j + e < p.n ? at[e] : 0u;
                 }
             }
         };
-        if (warp - 6 < fillers) fetch();
+        if (pair < pairs) fetch();
         u32 it = 0;
         bool ok = true;
         while (ok && walk.next()) {
             const bool of_w = walk.mt < p.wtiles;
             const u32 row0 = (of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS, rows = (of_w ? p.m : p.a_rows) - row0, most = rows < LIN_ROWS ? rows : LIN_ROWS;
             for (u32 k = 0; k < walk.count; k++, it++) {
-                if (it % fillers != warp - 6) continue;
+                if (it % pairs != pair) continue;
                 const u32 s = it % p.stages, round = it / p.stages, step = walk.first + k;
                 unsigned char* st = smem + s * p.stage_bytes;
                 if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
                 if (!W_COPY) {
                     const u32 j = step * LIN_STEP + lane, bytes = j < p.n ? 4 : 0;      // past the end of a row nothing is read and zero is stored
-                    const u32* src = bytes ? (of_w ? A.w : A.a) + (size_t)row0 * p.n + j : A.w;
-                    const size_t next = bytes ? p.n : 0;
+                    const u32* src = bytes ? (of_w ? A.w : A.a) + (size_t)(row0 + half) * p.n + j : A.w;
+                    const size_t next = bytes ? 2 * (size_t)p.n : 0;
                     const u32 to = smem_addr(st) + (lane & 3) * 4;
 #pragma unroll 8
-                    for (u32 r = 0; r < most; r++, src += next)
+                    for (u32 r = half; r < most; r += 2, src += next)
                         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
                 }
-                if (X_FILL) {
 #pragma unroll
-                    for (u32 i = 0; i < LIN_TOKENS / 4; i++) {
-                        if (4 * i >= p.tt) break;
-                        const u32 t = 4 * i + (lane >> 3), q = lane & 7;
-                        u32 w[4][4];
+                for (u32 i = 0; i < GROUPS; i++) {
+                    const u32 t = 4 * (2 * i + half) + (lane >> 3), q = lane & 7;
+                    if (4 * (2 * i + half) >= p.tt) break;
+                    u32 w[4][4];
 #pragma unroll
-                        for (u32 e = 0; e < 4; e++) {
-                            u32 d[4];
-                            digit_words(x[i][e], d);
+                    for (u32 e = 0; e < 4; e++) {
+                        u32 d[4];
+                        digit_words(x[i][e], d);
 #pragma unroll
-                            for (int c = 0; c < 4; c++) w[c][e] = d[c];
-                        }
-#pragma unroll
-                        for (u32 c = 0; c < 4; c++) {
-                            const u32 r = 4 * t + c;
-                            *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
-                        }
+                        for (int c = 0; c < 4; c++) w[c][e] = d[c];
                     }
-                    ahead += fillers;
-                    fetch();
+#pragma unroll
+                    for (u32 c = 0; c < 4; c++) {
+                        const u32 r = 4 * t + c;
+                        *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+                    }
                 }
+                ahead += pairs;
+                fetch();
                 if (!W_COPY) asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();

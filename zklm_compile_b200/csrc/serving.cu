@@ -107,40 +107,35 @@ static cudaError_t launch_after(bool early, void (*kernel)(KArgs...), dim3 grid,
 }
 
 // Where the parts of a call's workspace begin.
-struct LinSpace { size_t digits, slots, end; u32 chunk, a_rows; };
+struct LinSpace { size_t slots, end; u32 chunk, a_rows; };
 static LinSpace lin_space(int sm_count, u32 tokens, u32 m, u32 n, u32 num_adapters, u32 rank) {
     LinSpace w{};
-    w.chunk = lin_chunk(tokens, n);
+    w.chunk = lin_chunk(tokens);
     w.a_rows = lin_a_rows(w.chunk, m, num_adapters, rank);
     const LinPlan p = lin_plan(sm_count, w.chunk, m, n, w.a_rows);
-    w.digits = num_adapters && !w.a_rows ? round256((size_t)w.chunk * rank * 4) : 0;
-    w.slots = w.digits + round256(lin_digit_bytes(p));
+    w.slots = num_adapters && !w.a_rows ? round256((size_t)w.chunk * rank * 4) : 0;
     w.end = w.slots + lin_slot_bytes(sm_count, p);
     return w;
 }
 bool adapter_linear_fits(uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank) {
-    const u32 chunk = lin_chunk(tokens, n);
-    return lin_fits(chunk, m, n, lin_a_rows(chunk, m, num_adapters, rank));
+    return lin_fits(lin_chunk(tokens), m, n, lin_a_rows(lin_chunk(tokens), m, num_adapters, rank));
 }
 size_t adapter_linear_workspace(int sm_count, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank) {
     return tokens ? lin_space(sm_count, tokens, m, n, num_adapters, rank).end : 0;
 }
-template <bool W_COPY, bool X_FILL>
-static cudaError_t lin_product(cudaStream_t stream, bool early, const CUtensorMap& map_w, const CUtensorMap& map_a, const LinPlan& p, const LinearArgs& a, const unsigned char* digits,
-                               u32* slots) {
-    cudaError_t e = allow_smem(linear_bytes_kernel<W_COPY, X_FILL>, 201 * 1024);
+template <bool W_COPY>
+static cudaError_t lin_product(cudaStream_t stream, bool early, const CUtensorMap& map_w, const CUtensorMap& map_a, const LinPlan& p, const LinearArgs& a, u32* slots) {
+    const cudaError_t e = allow_smem(linear_bytes_kernel<W_COPY>, 201 * 1024);
     if (e != cudaSuccess) return e;
     const int x_vec = a.n % 4 == 0 && a.x_stride % 4 == 0 && !((uintptr_t)a.x & 15);
-    const dim3 block(192 + (W_COPY && !X_FILL ? 0 : LIN_FILL));
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
-    return launch_after(early, linear_bytes_kernel<W_COPY, X_FILL>, dim3(p.ctas), block, smem, stream, map_w, map_a, p, a, x_vec, digits, slots);
+    return launch_after(early, linear_bytes_kernel<W_COPY>, dim3(p.ctas), dim3(LIN_THREADS), smem, stream, map_w, map_a, p, a, x_vec, slots);
 }
 cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const LinearArgs& a, int* launches) {
     const LinSpace space = lin_space(sm_count, a.tokens, a.m, a.n, a.num_adapters, a.rank);
     u32* u = (u32*)a.workspace;
-    unsigned char* digits = (unsigned char*)a.workspace + space.digits;
     u32* slots = (u32*)((unsigned char*)a.workspace + space.slots);
-    const bool copies = a.n % 4 == 0 && !((uintptr_t)a.w & 15) && !(space.a_rows && ((uintptr_t)a.a & 15));
+    const bool copies = a.n % 4 == 0 && !((uintptr_t)a.w & 15) && !(space.a_rows && ((uintptr_t)a.a & 15)), apart = a.rank && !space.a_rows;
     CUtensorMap map_w = {}, map_a = {};
     cudaError_t e = cudaSuccess;
     if (copies) {
@@ -154,18 +149,12 @@ cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const Linea
         c.y += t0 * a.y_stride;
         if (a.rank) c.adapter_of += t0;
         const LinPlan p = lin_plan(sm_count, c.tokens, a.m, a.n, space.a_rows);
-        if (a.rank && !space.a_rows) {
+        if (apart) {
             const int vec = a.n % 4 == 0 && a.x_stride % 4 == 0 && !((uintptr_t)a.x & 15) && !((uintptr_t)a.a & 15);
             adapter_shrink_kernel<<<dim3(a.rank, c.tokens), 128, 0, stream>>>(c, vec, u);
             ++*launches;
         }
-        const bool fused = lin_fused(p), early = !fused || (a.rank && !space.a_rows);
-        if (!fused) {
-            linear_digits_kernel<<<dim3(p.steps, p.ntiles), 8 * p.tt, 0, stream>>>(c.x, c.x_stride, p, digits);
-            ++*launches;
-        }
-        if (copies) e = fused ? lin_product<true, true>(stream, early, map_w, map_a, p, c, digits, slots) : lin_product<true, false>(stream, early, map_w, map_a, p, c, digits, slots);
-        else e = fused ? lin_product<false, true>(stream, early, map_w, map_a, p, c, digits, slots) : lin_product<false, false>(stream, early, map_w, map_a, p, c, digits, slots);
+        e = copies ? lin_product<true>(stream, apart, map_w, map_a, p, c, slots) : lin_product<false>(stream, apart, map_w, map_a, p, c, slots);
         if (e != cudaSuccess) return e;
         const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS;
         e = launch_after(true, linear_join_kernel, dim3((a.m + LIN_JOIN_ROWS - 1) / LIN_JOIN_ROWS, p.ntiles * groups), dim3(256), 0, stream, c, p, slots, u);
