@@ -290,12 +290,13 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
     const u64 s = (u64)a[0] * b[0] + (u64)a[1] * b[1] + (u64)a[2] * b[2] + (u64)a[3] * b[3];
     return (s & ZKB_P) + (s >> 31);
 }
-// One CTA: 64 rows, up to 16 tokens of a tile of tokens, four of them a thread.  The adapters' B goes through shared memory 32 of its columns at a
-// time, once for all tokens beside each other that have the same one, for up to four adapters together.
-constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 32, LIN_JOIN_RUNS = 4;
-__global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan p, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
-    __shared__ __align__(16) u32 b[LIN_JOIN_RUNS][LIN_JOIN_ROWS][LIN_JOIN_RANK + 4];
-    __shared__ __align__(16) u32 u[LIN_JOIN_TOKENS][LIN_JOIN_RANK];
+// One CTA: 64 rows, up to 16 tokens of a tile of tokens.  B (A x) is a product of bytes too, on the warps' tensor cores: the rows of B are the left operand as
+// they lie in memory, read once for all tokens beside each other that have the same adapter (a run); each token's A x has four columns in the
+// right one, zero for the adapters of other tokens.  (With a multiplication a term this was 47 of 260 us for 1024 tokens of rank 32; now 17.)
+constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 64;
+__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, int b_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
+    __shared__ uint4 ud[LIN_JOIN_RANK / 16][LIN_JOIN_TOKENS / 2][32];              // digits of A x, 64 of the rank at a time
+    __shared__ u32 lora[LIN_JOIN_TOKENS][LIN_JOIN_ROWS + 8];
     __shared__ int of[LIN_JOIN_TOKENS], run_of[LIN_JOIN_TOKENS], run_adapter[LIN_JOIN_TOKENS], runs;
     const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS, nt = blockIdx.y / groups, in_tile = (blockIdx.y - nt * groups) * LIN_JOIN_TOKENS, t0 = nt * p.tt + in_tile;
     const u32 tile_end = (nt + 1) * p.tt < p.tokens ? (nt + 1) * p.tt : p.tokens;
@@ -316,46 +317,14 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan 
         }
         __syncthreads();
         n_runs = runs;
+        const u32 rows = A.m - i0 < LIN_JOIN_ROWS ? A.m - i0 : LIN_JOIN_ROWS, lines = (rows * rank + 31) / 32;
+        for (int r = 0; r < n_runs; r++)
+            for (u32 k = tid; k < lines; k += 256) prefetch_l2(A.b + ((size_t)run_adapter[r] * A.m + i0) * rank + 32 * (size_t)k);
     }
-    auto stage_b = [&](int run0, u32 r0) {
-        const u32 staged = n_runs - run0 < (int)LIN_JOIN_RUNS ? n_runs - run0 : LIN_JOIN_RUNS;
-        for (u32 run = 0; run < staged; run++) {
-            const u32* from = A.b + ((size_t)run_adapter[run0 + run] * A.m + i0) * rank + r0;
-            u32 v[LIN_JOIN_ROWS / 8];                        // all of a thread's loads before its first store: the compiler cannot tell that they do not meet
-#pragma unroll
-            for (u32 k = 0; k < LIN_JOIN_ROWS / 8; k++) v[k] = i0 + warp + 8 * k < A.m && r0 + lane < rank ? from[(size_t)(warp + 8 * k) * rank + lane] : 0u;
-#pragma unroll
-            for (u32 k = 0; k < LIN_JOIN_ROWS / 8; k++) b[run][warp + 8 * k][lane] = v[k];
-        }
-    };
-    const u64 bias = A.bias && i < A.m ? A.bias[i] : 0u;
-    if (n_runs) stage_b(0, 0);
+    u64 y[4];
+    y[0] = A.bias && i < A.m ? A.bias[i] : 0u;
+    y[1] = y[2] = y[3] = y[0];
     pdl_wait();
-    // A x of each token's own adapter, 32 of its rank at a time
-    auto sum_u = [&](u32 r0) {
-        u64 v[LIN_JOIN_TOKENS / 8];
-#pragma unroll
-        for (u32 k = 0; k < LIN_JOIN_TOKENS / 8; k++) {
-            const u32 t = warp + 8 * k;
-            v[k] = 0;
-            if (t >= count || of[t] < 0 || r0 + lane >= rank) continue;
-            if (p.a_rows) {
-                const u32 a_row = (u32)of[t] * rank + r0 + lane, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
-                const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
-                for (u32 seg = 0; seg < p.segs; seg++) {
-                    const u32 last = lin_last(p, tile, seg);
-#pragma unroll 8
-                    for (u32 c = lin_first(p, tile, seg); c <= last; c++) v[k] += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
-                }
-            } else {
-                v[k] = u_own[(size_t)(t0 + t) * rank + r0 + lane];
-            }
-        }
-#pragma unroll
-        for (u32 k = 0; k < LIN_JOIN_TOKENS / 8; k++) u[warp + 8 * k][lane] = red64(v[k]);
-    };
-    if (n_runs) sum_u(0);
-    u64 y[4] = {bias, bias, bias, bias};
     if (i < A.m) {
         const u32 tile = i / LIN_ROWS * p.ntiles + nt;
         const u32* at = slots + (size_t)(in_tile + mine) * LIN_ROWS + i % LIN_ROWS;
@@ -370,40 +339,101 @@ __global__ void __launch_bounds__(256) linear_join_kernel(LinearArgs A, LinPlan 
             }
         }
     }
-    for (u32 r0 = 0; n_runs && r0 < rank; r0 += LIN_JOIN_RANK) {
-        const u32 width = rank - r0 < LIN_JOIN_RANK ? rank - r0 : LIN_JOIN_RANK;
-        for (int run0 = 0; run0 < n_runs; run0 += LIN_JOIN_RUNS) {
-            if (r0 || run0) {
-                __syncthreads();
-                stage_b(run0, r0);
-                if (run0 == 0) sum_u(r0);
-            }
-            __syncthreads();
-            int run[4];
+    if (n_runs) {
+        const u32 g = lane >> 2, q4 = lane & 3, row_a = i0 + (warp & 3) * 16 + g, nt0 = (warp >> 2) * 4;
+        int acc[4][4] = {};
+        for (u32 rb = 0; rb < rank; rb += LIN_JOIN_RANK) {
+            if (rb) __syncthreads();
+            // A x, four of the rank a thread, and its digits
+            {
+                const u32 t = tid >> 4, r0 = rb + 4 * (tid & 15);
+                u64 v[4] = {0, 0, 0, 0};
+                if (t < count && of[t] >= 0 && r0 < rank) {
+                    if (!p.a_rows) {
 #pragma unroll
-            for (u32 k = 0; k < 4; k++) run[k] = mine + 4 * k < count ? run_of[mine + 4 * k] - run0 : -1;
-            if (run[0] >= 0 && run[0] < (int)LIN_JOIN_RUNS && run[0] == run[1] && run[0] == run[2] && run[0] == run[3]) {
-                for (u32 c = 0; c < width; c += 4) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(&b[run[0]][row][c]);
-                    const u32 pv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (u32 k = 0; k < 4; k++) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(&u[mine + 4 * k][c]);
-                        const u32 pw[4] = {w.x, w.y, w.z, w.w};
-                        y[k] += lin_dot4(pv, pw);
+                        for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? u_own[(size_t)(t0 + t) * rank + r0 + k] : 0u;
+                    } else if (rank % 4 == 0) {  // four neighbours of one tile
+                        const u32 a_row = (u32)of[t] * rank + r0, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
+                        const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
+                        for (u32 seg = 0; seg < p.segs; seg++) {
+                            const u32 last = lin_last(p, tile, seg);
+#pragma unroll 4
+                            for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(from + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words);
+                                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+                            }
+                        }
+                    } else {
+                        for (u32 k = 0; k < 4 && r0 + k < rank; k++) {
+                            const u32 a_row = (u32)of[t] * rank + r0 + k, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
+                            const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
+                            u64 sum = 0;
+                            for (u32 seg = 0; seg < p.segs; seg++) {
+                                const u32 last = lin_last(p, tile, seg);
+#pragma unroll 4
+                                for (u32 c = lin_first(p, tile, seg); c <= last; c++) sum += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
+                            }
+                            if (k == 0) v[0] = sum; else if (k == 1) v[1] = sum; else if (k == 2) v[2] = sum; else v[3] = sum;
+                        }
                     }
                 }
-            } else {
+                u32 w[4][4];
 #pragma unroll
-                for (u32 k = 0; k < 4; k++)
-                    if (run[k] >= 0 && run[k] < (int)LIN_JOIN_RUNS)
-                        for (u32 c = 0; c < width; c += 4) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(&b[run[k]][row][c]), w = *reinterpret_cast<const uint4*>(&u[mine + 4 * k][c]);
-                            const u32 pv[4] = {v.x, v.y, v.z, v.w}, pw[4] = {w.x, w.y, w.z, w.w};
-                            y[k] += lin_dot4(pv, pw);
-                        }
+                for (u32 k = 0; k < 4; k++) {
+                    u32 d[4];
+                    digit_words(red64(v[k]), d);
+#pragma unroll
+                    for (u32 c = 0; c < 4; c++) w[c][k] = d[c];
+                }
+                const u32 at = tid & 15;
+#pragma unroll
+                for (u32 c = 0; c < 4; c++) ud[at >> 2][t >> 1][((t & 1) * 4 + c) * 4 + (at & 3)] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
             }
+            __syncthreads();
+            for (u32 r0 = rb; r0 < rank && r0 < rb + LIN_JOIN_RANK; r0 += 16)
+                for (int run0 = 0; run0 < n_runs; run0 += 2) {
+                    u32 fa[2][4], fc[2][4];     // rows row_a and row_a + 8 of up to two adapters, columns r0 + 4 q4 .. + 3
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        if (run0 + k >= n_runs) break;
+                        const u32* from = A.b + ((size_t)run_adapter[run0 + k] * A.m + row_a) * rank + r0 + 4 * q4;
+                        const u32* from8 = from + 8 * (size_t)rank;
+                        if (b_vec) {
+                            const bool in = r0 + 4 * q4 < rank;
+                            const uint4 va = in && row_a < A.m ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+                            const uint4 vc = in && row_a + 8 < A.m ? *reinterpret_cast<const uint4*>(from8) : make_uint4(0, 0, 0, 0);
+                            fa[k][0] = va.x; fa[k][1] = va.y; fa[k][2] = va.z; fa[k][3] = va.w;
+                            fc[k][0] = vc.x; fc[k][1] = vc.y; fc[k][2] = vc.z; fc[k][3] = vc.w;
+                        } else {
+#pragma unroll
+                            for (u32 e = 0; e < 4; e++) {
+                                const bool in = r0 + 4 * q4 + e < rank;
+                                fa[k][e] = in && row_a < A.m ? from[e] : 0u;
+                                fc[k][e] = in && row_a + 8 < A.m ? from8[e] : 0u;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        if (run0 + k >= n_runs) break;
+#pragma unroll
+                        for (u32 n = 0; n < 4; n++) {
+                            const u32 tok = 2 * (nt0 + n);
+                            if (run_of[tok] != run0 + k && run_of[tok + 1] != run0 + k) continue;
+                            const uint4 b = run_of[tok + (lane >> 4)] == run0 + k ? ud[(r0 - rb) / 16][nt0 + n][lane] : make_uint4(0, 0, 0, 0);
+                            mma_u8_16x8x32(acc[n], fa[k][0], fc[k][0], fa[k][1], fc[k][1], b.x, b.y);
+                            mma_u8_16x8x32(acc[n], fa[k][2], fc[k][2], fa[k][3], fc[k][3], b.z, b.w);
+                        }
+                    }
+                }
         }
+        const bool odd = q4 & 1;
+        const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
+#pragma unroll
+        for (u32 n = 0; n < 4; n++) lora[2 * (nt0 + n) + (q4 >> 1)][(warp & 3) * 16 + g + (odd ? 8 : 0)] = digit_value(acc[n], odd, weights);
+        __syncthreads();
+#pragma unroll
+        for (u32 k = 0; k < 4; k++) y[k] += lora[mine + 4 * k][row];
     }
 #pragma unroll
     for (u32 k = 0; k < 4; k++)

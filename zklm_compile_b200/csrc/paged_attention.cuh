@@ -38,22 +38,6 @@ __device__ __forceinline__ u32 inv31_chain(u32 x) {
     return mul31(sq(t29, 2), x);               // 4 (2^29 - 1) + 1 = 2^31 - 3
 }
 
-__device__ __forceinline__ void mma_u8_16x8x32(int (&c)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// The four columns of a head are digits c of weight 2^(8c), sums below 2^31; a lane with an even q4 holds digits 0 and 1 of rows g and g + 8, the odd
-// one beside it digits 2 and 3.  Even lanes finish row g, odd ones row g + 8: the value mod p.  `weight`: of the lane's own two digits and of
-// its neighbour's.
-struct PaWeights { u32 own0, own1, other0, other1; };
-__device__ __forceinline__ u32 pa_value(const int (&c)[4], bool odd, const PaWeights& w) {
-    const u32 o0 = __shfl_xor_sync(0xffffffffu, (u32)(odd ? c[0] : c[2]), 1), o1 = __shfl_xor_sync(0xffffffffu, (u32)(odd ? c[1] : c[3]), 1);
-    const u64 v = (u64)(u32)(odd ? c[2] : c[0]) * w.own0 + (u64)(u32)(odd ? c[3] : c[1]) * w.own1 + (u64)o0 * w.other0 + (u64)o1 * w.other1;   // below 2^56
-    const u32 s = ((u32)v & ZKB_P) + (u32)(v >> 31);                                  // below 2^31 + 2^25
-    return umin32(s, s - ZKB_P);
-}
-
 // How the kernels are built for a head of up to DP elements: warps, and half tiles (16 keys or 16 values) in a warp's ring.  A half tile lies as the
 // tensor copies leave it: columns of 128 bytes, 16 rows of one behind the other, the 16-byte groups of a row swizzled by the row's low bits.
 // Which position becomes which row of an operand is free, and is chosen so that no two lanes of a phase meet in a bank.
@@ -312,7 +296,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     const u32 k_row = (g >> 1) + 4 * (g & 1), k_at = k_row * 128 + ((q4 ^ k_row) << 4);
     const u32 v_at0 = 2 * q4 * 128 + ((g ^ (2 * q4)) << 4), v_at1 = (2 * q4 + 1) * 128 + ((g ^ (2 * q4 + 1)) << 4);
     const bool odd = q4 & 1;
-    const PaWeights weights = odd ? PaWeights{1u << 16, 1u << 24, 1u, 1u << 8} : PaWeights{1u, 1u << 8, 1u << 16, 1u << 24};
+    const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
     u32 slot_out = 0, phase = 0;
     auto wait_half = [&] { mbar_wait(bar0 + 8 * slot_out, phase, &gave_up); };
     auto next_slot = [&] { if (++slot_out == NS) { slot_out = 0; phase ^= 1; } };
@@ -386,7 +370,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     int(&c)[4] = acc[m][n];
-                    const u32 v = pa_value(c, odd, weights);
+                    const u32 v = digit_value(c, odd, weights);
                     // rows of the tile are elements (see the left operand below)
                     const u32 e = SMALL ? 8 * (8 * (m >> 2) + g) + 2 * (m & 3) + odd : 4 * (8 * (m >> 1) + g) + 2 * (m & 1) + odd;
                     u32* at = to_part + 2 * n * DP + e;
@@ -437,7 +421,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                 u32 ev[NT];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const u32 s = pa_value(sc[n], odd, weights), minus = ZKB_P - s;
+                    const u32 s = digit_value(sc[n], odd, weights), minus = ZKB_P - s;
                     const bool neg = minus < s;
                     const u32 m = (umin32(s, minus) + round_up) >> A.score_shift;
                     const u32 index = neg ? 0u - m : m;

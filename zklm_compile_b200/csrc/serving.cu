@@ -136,6 +136,7 @@ cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const Linea
     u32* u = (u32*)a.workspace;
     u32* slots = (u32*)((unsigned char*)a.workspace + space.slots);
     const bool copies = a.n % 4 == 0 && !((uintptr_t)a.w & 15) && !(space.a_rows && ((uintptr_t)a.a & 15)), apart = a.rank && !space.a_rows;
+    const int b_vec = a.rank % 4 == 0 && !((uintptr_t)a.b & 15);
     CUtensorMap map_w = {}, map_a = {};
     cudaError_t e = cudaSuccess;
     if (copies) {
@@ -157,7 +158,7 @@ cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const Linea
         e = copies ? lin_product<true>(stream, apart, map_w, map_a, p, c, slots) : lin_product<false>(stream, apart, map_w, map_a, p, c, slots);
         if (e != cudaSuccess) return e;
         const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS;
-        e = launch_after(true, linear_join_kernel, dim3((a.m + LIN_JOIN_ROWS - 1) / LIN_JOIN_ROWS, p.ntiles * groups), dim3(256), 0, stream, c, p, slots, u);
+        e = launch_after(true, linear_join_kernel, dim3((a.m + LIN_JOIN_ROWS - 1) / LIN_JOIN_ROWS, p.ntiles * groups), dim3(256), 0, stream, c, p, b_vec, slots, u);
         if (e != cudaSuccess) return e;
         *launches += 2;
     }

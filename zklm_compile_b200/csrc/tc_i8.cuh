@@ -101,4 +101,21 @@ __device__ __forceinline__ void tmem_load16(u32 addr, u32 (&v)[16]) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// The integer tensor cores of a warp, for products that are too small or too scattered to stage: 16 rows x 8 columns, 32 bytes deep.
+__device__ __forceinline__ void mma_u8_16x8x32(int (&c)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four columns of such a product stand for one value: digits c of weight 2^(8c), sums below 2^31; a lane with an even q4 holds digits 0 and 1 of rows g and g + 8, the odd
+// one beside it digits 2 and 3.  Even lanes finish row g, odd ones row g + 8: the value mod p.  `weight`: of the lane's own two digits and of
+// its neighbour's.
+struct DigitWeights { u32 own0, own1, other0, other1; };
+__device__ __forceinline__ u32 digit_value(const int (&c)[4], bool odd, const DigitWeights& w) {
+    const u32 o0 = __shfl_xor_sync(0xffffffffu, (u32)(odd ? c[0] : c[2]), 1), o1 = __shfl_xor_sync(0xffffffffu, (u32)(odd ? c[1] : c[3]), 1);
+    const u64 v = (u64)(u32)(odd ? c[2] : c[0]) * w.own0 + (u64)(u32)(odd ? c[3] : c[1]) * w.own1 + (u64)o0 * w.other0 + (u64)o1 * w.other1;   // below 2^56
+    const u32 s = ((u32)v & ZKB_P) + (u32)(v >> 31);                                  // below 2^31 + 2^25
+    return umin32(s, s - ZKB_P);
+}
+
 }  // namespace zkb
