@@ -290,11 +290,11 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
     const u64 s = (u64)a[0] * b[0] + (u64)a[1] * b[1] + (u64)a[2] * b[2] + (u64)a[3] * b[3];
     return (s & ZKB_P) + (s >> 31);
 }
-// One CTA: 64 rows, up to 16 tokens of a tile of tokens.  B (A x) is a product of bytes too, on the warps' tensor cores: the rows of B are the left operand as
+// One CTA: `blocks` times 64 rows, up to 16 tokens of a tile of tokens.  B (A x) is a product of bytes too, on the warps' tensor cores: the rows of B are the left operand as
 // they lie in memory, read once for all tokens beside each other that have the same adapter (a run); each token's A x has four columns in the
 // right one, zero for the adapters of other tokens.  (With a multiplication a term this was 47 of 260 us for 1024 tokens of rank 32; now 17.)
 constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 64;
-__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, int b_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
+__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
     __shared__ uint4 ud[LIN_JOIN_RANK / 16][LIN_JOIN_TOKENS / 2][32];              // digits of A x, 64 of the rank at a time
     __shared__ u32 lora[LIN_JOIN_TOKENS][LIN_JOIN_ROWS + 8];
     __shared__ int of[LIN_JOIN_TOKENS], run_of[LIN_JOIN_TOKENS], run_adapter[LIN_JOIN_TOKENS], runs;
@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPl
     const u32 tile_end = (nt + 1) * p.tt < p.tokens ? (nt + 1) * p.tt : p.tokens;
     if (t0 >= tile_end) return;
     const u32 count = tile_end - t0 < LIN_JOIN_TOKENS ? tile_end - t0 : LIN_JOIN_TOKENS;
-    const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = tid & (LIN_JOIN_ROWS - 1), mine = tid >> 6, i0 = blockIdx.x * LIN_JOIN_ROWS, i = i0 + row, rank = A.rank;
+    const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = tid & (LIN_JOIN_ROWS - 1), mine = tid >> 6, begin = blockIdx.x * blocks * LIN_JOIN_ROWS, rank = A.rank;
+    const u32 stop = A.m - begin < blocks * LIN_JOIN_ROWS ? A.m : begin + blocks * LIN_JOIN_ROWS;
     // what does not come from the product: before waiting for it
     int n_runs = 0;
     if (rank) {
@@ -317,127 +318,134 @@ __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPl
         }
         __syncthreads();
         n_runs = runs;
-        const u32 rows = A.m - i0 < LIN_JOIN_ROWS ? A.m - i0 : LIN_JOIN_ROWS, lines = (rows * rank + 31) / 32;
+        const u32 lines = ((stop - begin) * rank + 31) / 32;
         for (int r = 0; r < n_runs; r++)
-            for (u32 k = tid; k < lines; k += 256) prefetch_l2(A.b + ((size_t)run_adapter[r] * A.m + i0) * rank + 32 * (size_t)k);
+            for (u32 k = tid; k < lines; k += 256) prefetch_l2(A.b + ((size_t)run_adapter[r] * A.m + begin) * rank + 32 * (size_t)k);
     }
-    u64 y[4];
-    y[0] = A.bias && i < A.m ? A.bias[i] : 0u;
-    y[1] = y[2] = y[3] = y[0];
+    // A x from column rb of the rank on, four of it a thread, and its digits
+    auto make_digits = [&](u32 rb) {
+                        const u32 t = tid >> 4, r0 = rb + 4 * (tid & 15);
+                        u64 v[4] = {0, 0, 0, 0};
+                        if (t < count && of[t] >= 0 && r0 < rank) {
+                            if (!p.a_rows) {
+        #pragma unroll
+                                for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? u_own[(size_t)(t0 + t) * rank + r0 + k] : 0u;
+                            } else if (rank % 4 == 0) {  // four neighbours of one tile
+                                const u32 a_row = (u32)of[t] * rank + r0, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
+                                const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
+                                for (u32 seg = 0; seg < p.segs; seg++) {
+                                    const u32 last = lin_last(p, tile, seg);
+        #pragma unroll 4
+                                    for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
+                                        const uint4 x = *reinterpret_cast<const uint4*>(from + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words);
+                                        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+                                    }
+                                }
+                            } else {
+                                for (u32 k = 0; k < 4 && r0 + k < rank; k++) {
+                                    const u32 a_row = (u32)of[t] * rank + r0 + k, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
+                                    const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
+                                    u64 sum = 0;
+                                    for (u32 seg = 0; seg < p.segs; seg++) {
+                                        const u32 last = lin_last(p, tile, seg);
+        #pragma unroll 4
+                                        for (u32 c = lin_first(p, tile, seg); c <= last; c++) sum += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
+                                    }
+                                    if (k == 0) v[0] = sum; else if (k == 1) v[1] = sum; else if (k == 2) v[2] = sum; else v[3] = sum;
+                                }
+                            }
+                        }
+                        u32 w[4][4];
+        #pragma unroll
+                        for (u32 k = 0; k < 4; k++) {
+                            u32 d[4];
+                            digit_words(red64(v[k]), d);
+        #pragma unroll
+                            for (u32 c = 0; c < 4; c++) w[c][k] = d[c];
+                        }
+                        const u32 at = tid & 15;
+        #pragma unroll
+                        for (u32 c = 0; c < 4; c++) ud[at >> 2][t >> 1][((t & 1) * 4 + c) * 4 + (at & 3)] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+    };
     pdl_wait();
-    if (i < A.m) {
-        const u32 tile = i / LIN_ROWS * p.ntiles + nt;
-        const u32* at = slots + (size_t)(in_tile + mine) * LIN_ROWS + i % LIN_ROWS;
-        for (u32 seg = 0; seg < p.segs; seg++) {
-            const u32 last = lin_last(p, tile, seg);
+    const u32 g = lane >> 2, q4 = lane & 3, nt0 = (warp >> 2) * 4;
+    const bool odd = q4 & 1;
+    const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
+    if (n_runs) make_digits(0);
+    for (u32 i0 = begin; i0 < stop; i0 += LIN_JOIN_ROWS) {
+        const u32 i = i0 + row, row_a = i0 + (warp & 3) * 16 + g;
+        u64 y[4];
+        y[0] = A.bias && i < A.m ? A.bias[i] : 0u;
+        y[1] = y[2] = y[3] = y[0];
+        if (i < A.m) {
+            const u32 tile = i / LIN_ROWS * p.ntiles + nt;
+            const u32* at = slots + (size_t)(in_tile + mine) * LIN_ROWS + i % LIN_ROWS;
+            for (u32 seg = 0; seg < p.segs; seg++) {
+                const u32 last = lin_last(p, tile, seg);
 #pragma unroll 4
-            for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
-                const u32* s = at + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words;
+                for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
+                    const u32* s = at + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words;
 #pragma unroll
-                for (u32 k = 0; k < 4; k++)
-                    if (mine + 4 * k < count) y[k] += s[k * 4 * LIN_ROWS];
+                    for (u32 k = 0; k < 4; k++)
+                        if (mine + 4 * k < count) y[k] += s[k * 4 * LIN_ROWS];
+                }
             }
         }
-    }
-    if (n_runs) {
-        const u32 g = lane >> 2, q4 = lane & 3, row_a = i0 + (warp & 3) * 16 + g, nt0 = (warp >> 2) * 4;
-        int acc[4][4] = {};
-        for (u32 rb = 0; rb < rank; rb += LIN_JOIN_RANK) {
-            if (rb) __syncthreads();
-            // A x, four of the rank a thread, and its digits
-            {
-                const u32 t = tid >> 4, r0 = rb + 4 * (tid & 15);
-                u64 v[4] = {0, 0, 0, 0};
-                if (t < count && of[t] >= 0 && r0 < rank) {
-                    if (!p.a_rows) {
-#pragma unroll
-                        for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? u_own[(size_t)(t0 + t) * rank + r0 + k] : 0u;
-                    } else if (rank % 4 == 0) {  // four neighbours of one tile
-                        const u32 a_row = (u32)of[t] * rank + r0, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
-                        const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
-                        for (u32 seg = 0; seg < p.segs; seg++) {
-                            const u32 last = lin_last(p, tile, seg);
-#pragma unroll 4
-                            for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
-                                const uint4 x = *reinterpret_cast<const uint4*>(from + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words);
-                                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        if (n_runs) {
+            int acc[4][4] = {};
+            for (u32 rb = 0; rb < rank; rb += LIN_JOIN_RANK) {
+                if (rb || (rank > LIN_JOIN_RANK && i0 > begin)) {
+                    __syncthreads();
+                    make_digits(rb);
+                }
+                __syncthreads();
+                for (u32 r0 = rb; r0 < rank && r0 < rb + LIN_JOIN_RANK; r0 += 16)
+                    for (int run0 = 0; run0 < n_runs; run0 += 2) {
+                        u32 fa[2][4], fc[2][4];     // rows row_a and row_a + 8 of up to two adapters, columns r0 + 4 q4 .. + 3
+    #pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            if (run0 + k >= n_runs) break;
+                            const u32* from = A.b + ((size_t)run_adapter[run0 + k] * A.m + row_a) * rank + r0 + 4 * q4;
+                            const u32* from8 = from + 8 * (size_t)rank;
+                            if (b_vec) {
+                                const bool in = r0 + 4 * q4 < rank;
+                                const uint4 va = in && row_a < A.m ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+                                const uint4 vc = in && row_a + 8 < A.m ? *reinterpret_cast<const uint4*>(from8) : make_uint4(0, 0, 0, 0);
+                                fa[k][0] = va.x; fa[k][1] = va.y; fa[k][2] = va.z; fa[k][3] = va.w;
+                                fc[k][0] = vc.x; fc[k][1] = vc.y; fc[k][2] = vc.z; fc[k][3] = vc.w;
+                            } else {
+    #pragma unroll
+                                for (u32 e = 0; e < 4; e++) {
+                                    const bool in = r0 + 4 * q4 + e < rank;
+                                    fa[k][e] = in && row_a < A.m ? from[e] : 0u;
+                                    fc[k][e] = in && row_a + 8 < A.m ? from8[e] : 0u;
+                                }
                             }
                         }
-                    } else {
-                        for (u32 k = 0; k < 4 && r0 + k < rank; k++) {
-                            const u32 a_row = (u32)of[t] * rank + r0 + k, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
-                            const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
-                            u64 sum = 0;
-                            for (u32 seg = 0; seg < p.segs; seg++) {
-                                const u32 last = lin_last(p, tile, seg);
-#pragma unroll 4
-                                for (u32 c = lin_first(p, tile, seg); c <= last; c++) sum += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
+    #pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            if (run0 + k >= n_runs) break;
+    #pragma unroll
+                            for (u32 n = 0; n < 4; n++) {
+                                const u32 tok = 2 * (nt0 + n);
+                                if (run_of[tok] != run0 + k && run_of[tok + 1] != run0 + k) continue;
+                                const uint4 b = run_of[tok + (lane >> 4)] == run0 + k ? ud[(r0 - rb) / 16][nt0 + n][lane] : make_uint4(0, 0, 0, 0);
+                                mma_u8_16x8x32(acc[n], fa[k][0], fc[k][0], fa[k][1], fc[k][1], b.x, b.y);
+                                mma_u8_16x8x32(acc[n], fa[k][2], fc[k][2], fa[k][3], fc[k][3], b.z, b.w);
                             }
-                            if (k == 0) v[0] = sum; else if (k == 1) v[1] = sum; else if (k == 2) v[2] = sum; else v[3] = sum;
                         }
                     }
-                }
-                u32 w[4][4];
-#pragma unroll
-                for (u32 k = 0; k < 4; k++) {
-                    u32 d[4];
-                    digit_words(red64(v[k]), d);
-#pragma unroll
-                    for (u32 c = 0; c < 4; c++) w[c][k] = d[c];
-                }
-                const u32 at = tid & 15;
-#pragma unroll
-                for (u32 c = 0; c < 4; c++) ud[at >> 2][t >> 1][((t & 1) * 4 + c) * 4 + (at & 3)] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
             }
+#pragma unroll
+            for (u32 n = 0; n < 4; n++) lora[2 * (nt0 + n) + (q4 >> 1)][(warp & 3) * 16 + g + (odd ? 8 : 0)] = digit_value(acc[n], odd, weights);
             __syncthreads();
-            for (u32 r0 = rb; r0 < rank && r0 < rb + LIN_JOIN_RANK; r0 += 16)
-                for (int run0 = 0; run0 < n_runs; run0 += 2) {
-                    u32 fa[2][4], fc[2][4];     // rows row_a and row_a + 8 of up to two adapters, columns r0 + 4 q4 .. + 3
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        if (run0 + k >= n_runs) break;
-                        const u32* from = A.b + ((size_t)run_adapter[run0 + k] * A.m + row_a) * rank + r0 + 4 * q4;
-                        const u32* from8 = from + 8 * (size_t)rank;
-                        if (b_vec) {
-                            const bool in = r0 + 4 * q4 < rank;
-                            const uint4 va = in && row_a < A.m ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
-                            const uint4 vc = in && row_a + 8 < A.m ? *reinterpret_cast<const uint4*>(from8) : make_uint4(0, 0, 0, 0);
-                            fa[k][0] = va.x; fa[k][1] = va.y; fa[k][2] = va.z; fa[k][3] = va.w;
-                            fc[k][0] = vc.x; fc[k][1] = vc.y; fc[k][2] = vc.z; fc[k][3] = vc.w;
-                        } else {
-#pragma unroll
-                            for (u32 e = 0; e < 4; e++) {
-                                const bool in = r0 + 4 * q4 + e < rank;
-                                fa[k][e] = in && row_a < A.m ? from[e] : 0u;
-                                fc[k][e] = in && row_a + 8 < A.m ? from8[e] : 0u;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        if (run0 + k >= n_runs) break;
-#pragma unroll
-                        for (u32 n = 0; n < 4; n++) {
-                            const u32 tok = 2 * (nt0 + n);
-                            if (run_of[tok] != run0 + k && run_of[tok + 1] != run0 + k) continue;
-                            const uint4 b = run_of[tok + (lane >> 4)] == run0 + k ? ud[(r0 - rb) / 16][nt0 + n][lane] : make_uint4(0, 0, 0, 0);
-                            mma_u8_16x8x32(acc[n], fa[k][0], fc[k][0], fa[k][1], fc[k][1], b.x, b.y);
-                            mma_u8_16x8x32(acc[n], fa[k][2], fc[k][2], fa[k][3], fc[k][3], b.z, b.w);
-                        }
-                    }
-                }
+            for (u32 k = 0; k < 4; k++) y[k] += lora[mine + 4 * k][row];
         }
-        const bool odd = q4 & 1;
-        const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
 #pragma unroll
-        for (u32 n = 0; n < 4; n++) lora[2 * (nt0 + n) + (q4 >> 1)][(warp & 3) * 16 + g + (odd ? 8 : 0)] = digit_value(acc[n], odd, weights);
-        __syncthreads();
-#pragma unroll
-        for (u32 k = 0; k < 4; k++) y[k] += lora[mine + 4 * k][row];
+        for (u32 k = 0; k < 4; k++)
+            if (i < A.m && mine + 4 * k < count) A.y[(t0 + mine + 4 * k) * A.y_stride + i] = red64(y[k]);
     }
-#pragma unroll
-    for (u32 k = 0; k < 4; k++)
-        if (i < A.m && mine + 4 * k < count) A.y[(t0 + mine + 4 * k) * A.y_stride + i] = red64(y[k]);
 }
 
 // u[t][r] = A[of[t]][r] . x[t]; a CTA per (r, t).
