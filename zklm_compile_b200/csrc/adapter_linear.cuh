@@ -294,15 +294,15 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
 // they lie in memory, read once for all tokens beside each other that have the same adapter (a run); each token's A x has four columns in the
 // right one, zero for the adapters of other tokens.  (With a multiplication a term this was 47 of 260 us for 1024 tokens of rank 32; now 17.)
 constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 64;
-__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
+__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, int y_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
     __shared__ uint4 ud[LIN_JOIN_RANK / 16][LIN_JOIN_TOKENS / 2][32];              // digits of A x, 64 of the rank at a time
-    __shared__ u32 lora[LIN_JOIN_TOKENS][LIN_JOIN_ROWS + 8];
+    __shared__ __align__(16) u32 lora[LIN_JOIN_TOKENS][LIN_JOIN_ROWS + 4];
     __shared__ int of[LIN_JOIN_TOKENS], run_of[LIN_JOIN_TOKENS], run_adapter[LIN_JOIN_TOKENS], runs;
     const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS, nt = blockIdx.y / groups, in_tile = (blockIdx.y - nt * groups) * LIN_JOIN_TOKENS, t0 = nt * p.tt + in_tile;
     const u32 tile_end = (nt + 1) * p.tt < p.tokens ? (nt + 1) * p.tt : p.tokens;
     if (t0 >= tile_end) return;
     const u32 count = tile_end - t0 < LIN_JOIN_TOKENS ? tile_end - t0 : LIN_JOIN_TOKENS;
-    const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = tid & (LIN_JOIN_ROWS - 1), mine = tid >> 6, begin = blockIdx.x * blocks * LIN_JOIN_ROWS, rank = A.rank;
+    const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = 4 * (tid & 15), mine = tid >> 4, begin = blockIdx.x * blocks * LIN_JOIN_ROWS, rank = A.rank;
     const u32 stop = A.m - begin < blocks * LIN_JOIN_ROWS ? A.m : begin + blocks * LIN_JOIN_ROWS;
     // what does not come from the product: before waiting for it
     int n_runs = 0;
@@ -372,22 +372,23 @@ __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPl
     const bool odd = q4 & 1;
     const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
     if (n_runs) make_digits(0);
+    // a thread has one token and four rows of a block
+    const bool has = mine < count;
+    const u32 tile = begin / LIN_ROWS * p.ntiles + nt, first = lin_first(p, tile, 0), last = lin_last(p, tile, 0);       // the rows of a CTA lie in one tile
     for (u32 i0 = begin; i0 < stop; i0 += LIN_JOIN_ROWS) {
-        const u32 i = i0 + row, row_a = i0 + (warp & 3) * 16 + g;
+        const u32 i = i0 + quad, row_a = i0 + (warp & 3) * 16 + g;
         u64 y[4];
-        y[0] = A.bias && i < A.m ? A.bias[i] : 0u;
-        y[1] = y[2] = y[3] = y[0];
-        if (i < A.m) {
-            const u32 tile = i / LIN_ROWS * p.ntiles + nt;
+#pragma unroll
+        for (u32 e = 0; e < 4; e++) y[e] = A.bias && i + e < A.m ? A.bias[i + e] : 0u;
+        if (has && i < A.m) {                  // rows of the tile that are behind the last one hold nothing of use, but are there
             const u32* at = slots + (size_t)(in_tile + mine) * LIN_ROWS + i % LIN_ROWS;
             for (u32 seg = 0; seg < p.segs; seg++) {
-                const u32 last = lin_last(p, tile, seg);
+                const u32 from = seg ? lin_first(p, tile, seg) : first, to = seg ? lin_last(p, tile, seg) : last;
+                const u32* s = at + ((size_t)from + (size_t)tile * p.segs + seg) * p.slot_words;
 #pragma unroll 4
-                for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
-                    const u32* s = at + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words;
-#pragma unroll
-                    for (u32 k = 0; k < 4; k++)
-                        if (mine + 4 * k < count) y[k] += s[k * 4 * LIN_ROWS];
+                for (u32 c = from; c <= to; c++, s += p.slot_words) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(s);
+                    y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
                 }
             }
         }
@@ -439,12 +440,21 @@ __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPl
 #pragma unroll
             for (u32 n = 0; n < 4; n++) lora[2 * (nt0 + n) + (q4 >> 1)][(warp & 3) * 16 + g + (odd ? 8 : 0)] = digit_value(acc[n], odd, weights);
             __syncthreads();
-#pragma unroll
-            for (u32 k = 0; k < 4; k++) y[k] += lora[mine + 4 * k][row];
+            const uint4 v = *reinterpret_cast<const uint4*>(&lora[mine][quad]);
+            y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
         }
-#pragma unroll
-        for (u32 k = 0; k < 4; k++)
-            if (i < A.m && mine + 4 * k < count) A.y[(t0 + mine + 4 * k) * A.y_stride + i] = red64(y[k]);
+        if (has && i < A.m) {
+            u32* to = A.y + (t0 + mine) * A.y_stride + i;
+            const uint4 v = make_uint4(red64(y[0]), red64(y[1]), red64(y[2]), red64(y[3]));
+            if (y_vec && i + 4 <= A.m) {
+                *reinterpret_cast<uint4*>(to) = v;
+            } else {
+                to[0] = v.x;
+                if (i + 1 < A.m) to[1] = v.y;
+                if (i + 2 < A.m) to[2] = v.z;
+                if (i + 3 < A.m) to[3] = v.w;
+            }
+        }
     }
 }
 

@@ -136,7 +136,7 @@ cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const Linea
     u32* u = (u32*)a.workspace;
     u32* slots = (u32*)((unsigned char*)a.workspace + space.slots);
     const bool copies = a.n % 4 == 0 && !((uintptr_t)a.w & 15) && !(space.a_rows && ((uintptr_t)a.a & 15)), apart = a.rank && !space.a_rows;
-    const int b_vec = a.rank % 4 == 0 && !((uintptr_t)a.b & 15);
+    const int b_vec = a.rank % 4 == 0 && !((uintptr_t)a.b & 15), y_vec = a.y_stride % 4 == 0 && !((uintptr_t)a.y & 15);
     CUtensorMap map_w = {}, map_a = {};
     cudaError_t e = cudaSuccess;
     if (copies) {
@@ -160,7 +160,7 @@ cudaError_t adapter_linear_launch(cudaStream_t stream, int sm_count, const Linea
         // four blocks of rows a CTA where there are many of them: the tokens' A x is then summed up a quarter as often
         const u32 groups = (p.tt + LIN_JOIN_TOKENS - 1) / LIN_JOIN_TOKENS, row_blocks = (a.m + LIN_JOIN_ROWS - 1) / LIN_JOIN_ROWS;
         const u32 blocks = (u64)row_blocks * p.ntiles * groups > 8ull * sm_count ? 4 : 1;
-        e = launch_after(true, linear_join_kernel, dim3((row_blocks + blocks - 1) / blocks, p.ntiles * groups), dim3(256), 0, stream, c, p, blocks, b_vec, slots, u);
+        e = launch_after(true, linear_join_kernel, dim3((row_blocks + blocks - 1) / blocks, p.ntiles * groups), dim3(256), 0, stream, c, p, blocks, b_vec, y_vec, slots, u);
         if (e != cudaSuccess) return e;
         *launches += 2;
     }
