@@ -20,7 +20,7 @@ constexpr u32 LIN_STEP = 32;                   // columns of W per step: 128 byt
 constexpr u32 LIN_SEG = 256;                   // steps after which the accumulators are emptied (8192 columns)
 constexpr u32 LIN_TOKENS = 64;                 // tokens per tile at most: 256 columns of an accumulator
 constexpr u32 LIN_MAX_STAGES = 8;
-constexpr u32 LIN_FILL = 8;                     // warps that fill operands by plain stores, two a step
+constexpr u32 LIN_TEAM = 4, LIN_FILL = 3 * LIN_TEAM;   // warps that fill operands by plain stores: teams that take a step each
 constexpr u32 LIN_THREADS = (6 + LIN_FILL) * 32;
 constexpr u32 LIN_CHUNK = 2048;                // tokens of one pass
 
@@ -52,7 +52,7 @@ inline LinPlan lin_plan(int sm_count, u32 tokens, u32 m, u32 n, u32 a_rows) {
     p.per = (p.total + sm_count - 1) / sm_count;
     p.ctas = (p.total + p.per - 1) / p.per;
     p.stage_bytes = LIN_ROWS * 128 + (4 * p.tt * 128 + 1023) / 1024 * 1024;
-    p.stages = 200 * 1024 / p.stage_bytes < LIN_MAX_STAGES ? 200 * 1024 / p.stage_bytes : LIN_MAX_STAGES;
+    p.stages = 200 * 1024 / p.stage_bytes < LIN_MAX_STAGES ? 200 * 1024 / p.stage_bytes : LIN_MAX_STAGES;     // 3 at least, as many as teams of warps that fill
     p.tmem_cols = 32;
     while (p.tmem_cols < 8 * p.tt) p.tmem_cols *= 2;
     p.slot_words = (size_t)p.tt * LIN_ROWS;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
     const u32 base = smem_addr(smem);
     const u32 full = smem_addr(bars), empty = full + 8 * LIN_MAX_STAGES, acc_full = empty + 8 * LIN_MAX_STAGES, acc_empty = acc_full + 8;
     if (threadIdx.x == 0) {
-        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 3); mbar_init(empty + 8 * s, 1); }
+        for (u32 s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 1 + LIN_TEAM); mbar_init(empty + 8 * s, 1); }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 4);
         gave_up = 0;
@@ -200,20 +200,21 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
             n++;
         }
     } else {
-        // Each pair of warps takes every fourth step, so that four steps' loads are under way - but no more pairs than stages: a pair knows that the stage of
-        // its last step was empty, and from that that its next one's was emptied the time before last; with fewer stages than pairs it could be two phases
-        // ahead, where a wait by parity sees the wrong one.
-        const u32 pairs = p.stages < LIN_FILL / 2 ? p.stages : LIN_FILL / 2, pair = (warp - 6) >> 1, half = warp & 1;
-        constexpr u32 GROUPS = LIN_TOKENS / 8;
-        // A warp's groups of four values of x, fetched a turn ahead: token 4 (2 i + half) + lane / 8 of the tile, columns 4 (lane & 7) .. of its next step.
+        // Each team of warps takes every third step, so that three steps' loads are under way.  There are at least as many stages as teams: a team knows that
+        // the stage of its last step was empty, and from that that its next one's was emptied the time before last; with fewer stages than teams it could
+        // be two phases ahead, where a wait by parity sees the wrong one.  (Two warps a step took 0.92 us a step of 64 tokens.)
+        constexpr u32 teams = LIN_FILL / LIN_TEAM;
+        const u32 team = (warp - 6) / LIN_TEAM, member = (warp - 6) % LIN_TEAM;
+        constexpr u32 GROUPS = LIN_TOKENS / (4 * LIN_TEAM);
+        // A warp's groups of four values of x, fetched a turn ahead: token 4 (4 i + member) + lane / 8 of the tile, columns 4 (lane & 7) .. of its next step.
         u32 x[GROUPS][4];
-        u32 ahead = blockIdx.x * p.per + pair;
+        u32 ahead = blockIdx.x * p.per + team;
         auto fetch = [&] {
             if (ahead >= walk.end) return;
             const u32 tile = ahead / p.steps, j = (ahead - tile * p.steps) * LIN_STEP + 4 * (lane & 7), tok0 = tile % p.ntiles * p.tt;
 #pragma unroll
             for (u32 i = 0; i < GROUPS; i++) {
-                const u32 in = 4 * (2 * i + half) + (lane >> 3), t = tok0 + in;
+                const u32 in = 4 * (LIN_TEAM * i + member) + (lane >> 3), t = tok0 + in;
                 const bool there = in < p.tt && t < p.tokens;
                 const u32* at = A.x + t * A.x_stride + j;
                 if (x_vec) {                     // n is a multiple of 4 then
@@ -225,30 +226,30 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
                 }
             }
         };
-        if (pair < pairs) fetch();
+        fetch();
         u32 it = 0;
         bool ok = true;
         while (ok && walk.next()) {
             const bool of_w = walk.mt < p.wtiles;
             const u32 row0 = (of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS, rows = (of_w ? p.m : p.a_rows) - row0, most = rows < LIN_ROWS ? rows : LIN_ROWS;
             for (u32 k = 0; k < walk.count; k++, it++) {
-                if (it % pairs != pair) continue;
+                if (it % teams != team) continue;
                 const u32 s = it % p.stages, round = it / p.stages, step = walk.first + k;
                 unsigned char* st = smem + s * p.stage_bytes;
                 if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
                 if (!W_COPY) {
                     const u32 j = step * LIN_STEP + lane, bytes = j < p.n ? 4 : 0;      // past the end of a row nothing is read and zero is stored
-                    const u32* src = bytes ? (of_w ? A.w : A.a) + (size_t)(row0 + half) * p.n + j : A.w;
-                    const size_t next = bytes ? 2 * (size_t)p.n : 0;
+                    const u32* src = bytes ? (of_w ? A.w : A.a) + (size_t)(row0 + member) * p.n + j : A.w;
+                    const size_t next = bytes ? LIN_TEAM * (size_t)p.n : 0;
                     const u32 to = smem_addr(st) + (lane & 3) * 4;
 #pragma unroll 8
-                    for (u32 r = half; r < most; r += 2, src += next)
+                    for (u32 r = member; r < most; r += LIN_TEAM, src += next)
                         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + r * 128 + (((lane >> 2) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
                 }
 #pragma unroll
                 for (u32 i = 0; i < GROUPS; i++) {
-                    const u32 t = 4 * (2 * i + half) + (lane >> 3), q = lane & 7;
-                    if (4 * (2 * i + half) >= p.tt) break;
+                    const u32 t = 4 * (LIN_TEAM * i + member) + (lane >> 3), q = lane & 7;
+                    if (4 * (LIN_TEAM * i + member) >= p.tt) break;
                     u32 w[4][4];
 #pragma unroll
                     for (u32 e = 0; e < 4; e++) {
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
                         *reinterpret_cast<uint4*>(st + LIN_ROWS * 128 + r * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
                     }
                 }
-                ahead += pairs;
+                ahead += teams;
                 fetch();
                 if (!W_COPY) asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
