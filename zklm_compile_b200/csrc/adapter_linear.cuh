@@ -120,53 +120,50 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
     const u32 tmem = tmem_base;
     LinWalk walk(p);
     if (warp == 0) {
-        if (lane == 0) {
-            u32 it = 0;
-            bool ok = true;
-            while (ok && walk.next()) {
-                const bool of_w = walk.mt < p.wtiles;
-                const int row = (int)((of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS);
-                for (u32 k = 0; k < walk.count; k++, it++) {
-                    const u32 s = it % p.stages, round = it / p.stages, st = base + s * p.stage_bytes;
-                    if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
-                    mbar_expect(full + 8 * s, W_COPY ? LIN_ROWS * 128 : 0u);
-                    if (W_COPY) tensor_load_2d(st, of_w ? &map_w : &map_a, (int)((walk.first + k) * LIN_STEP), row, full + 8 * s);
-                }
+        u32 it = 0;
+        bool ok = true;
+        while (ok && walk.next()) {
+            const bool of_w = walk.mt < p.wtiles;
+            const CUtensorMap* map = of_w ? &map_w : &map_a;
+            const int row = (int)((of_w ? walk.mt : walk.mt - p.wtiles) * LIN_ROWS);
+            for (u32 k = 0; k < walk.count; k++, it++) {
+                const u32 s = it % p.stages, round = it / p.stages, st = base + s * p.stage_bytes;
+                if (round && !(ok = mbar_wait(empty + 8 * s, (round - 1) & 1, &gave_up))) break;
+                mbar_expect_one(full + 8 * s, W_COPY ? LIN_ROWS * 128 : 0u);
+                if (W_COPY) tensor_load_2d_one(st, map, (int)((walk.first + k) * LIN_STEP), row, full + 8 * s);
             }
-            // The kernel before this one (where it is one of the same call) makes what the join reads: the join, which waits for this kernel, must find it done.
-            pdl_wait();
-            if (!ok)                             // given up: nothing of this CTA may still be in flight when it ends
-                for (u32 i = it > p.stages ? it - p.stages : 0; i < it; i++)
-                    for (u32 n = 0; n < (1u << 16) && !mbar_try(full + 8 * (i % p.stages), (i / p.stages) & 1); n++) {}
         }
+        // The kernel before this one (where it is one of the same call) makes what the join reads: the join, which waits for this kernel, must find it done.
+        pdl_wait();
+        if (!ok)                                 // given up: nothing of this CTA may still be in flight when it ends
+            for (u32 i = it > p.stages ? it - p.stages : 0; i < it; i++)
+                for (u32 n = 0; n < (1u << 16) && !mbar_try(full + 8 * (i % p.stages), (i / p.stages) & 1); n++) {}
     } else if (warp == 1) {
-        if (lane == 0) {
-            const u32 idesc = i8_instr_desc(4 * p.tt);
-            u32 it = 0, n = 0;
-            bool ok = true;
-            while (ok && walk.next()) {
-                if (n && !(ok = mbar_wait(acc_empty, (n - 1) & 1, &gave_up))) { mma_commit(acc_full); n++; break; }
+        const u32 idesc = i8_instr_desc(4 * p.tt);
+        u32 it = 0, n = 0;
+        bool ok = true;
+        while (ok && walk.next()) {
+            if (n && !(ok = mbar_wait(acc_empty, (n - 1) & 1, &gave_up))) { mma_commit_one(acc_full); n++; break; }
+            tc_fence_after();
+            const bool two = walk.mt < p.wtiles ? walk.mt * LIN_ROWS + 128 < p.m : (walk.mt - p.wtiles) * LIN_ROWS + 128 < p.a_rows;
+            for (u32 k = 0; k < walk.count; k++, it++) {
+                const u32 s = it % p.stages, st = base + s * p.stage_bytes;
+                if (!(ok = mbar_wait(full + 8 * s, (it / p.stages) & 1, &gave_up))) break;
                 tc_fence_after();
-                const bool two = walk.mt < p.wtiles ? walk.mt * LIN_ROWS + 128 < p.m : (walk.mt - p.wtiles) * LIN_ROWS + 128 < p.a_rows;
-                for (u32 k = 0; k < walk.count; k++, it++) {
-                    const u32 s = it % p.stages, st = base + s * p.stage_bytes;
-                    if (!(ok = mbar_wait(full + 8 * s, (it / p.stages) & 1, &gave_up))) break;
-                    tc_fence_after();
-                    const u64 a = smem_desc_sw128(st), b = smem_desc_sw128(st + LIN_ROWS * 128);
+                const u64 a = smem_desc_sw128(st), b = smem_desc_sw128(st + LIN_ROWS * 128);
 #pragma unroll
-                    for (u32 kk = 0; kk < 4; kk++) mma_u8(tmem, a + 2 * kk, b + 2 * kk, idesc, k || kk);
-                    if (two) {
+                for (u32 kk = 0; kk < 4; kk++) mma_u8_one(tmem, a + 2 * kk, b + 2 * kk, idesc, k || kk);
+                if (two) {
 #pragma unroll
-                        for (u32 kk = 0; kk < 4; kk++) mma_u8(tmem + 4 * p.tt, a + (16384 >> 4) + 2 * kk, b + 2 * kk, idesc, k || kk);
-                    }
-                    mma_commit(empty + 8 * s);
+                    for (u32 kk = 0; kk < 4; kk++) mma_u8_one(tmem + 4 * p.tt, a + (16384 >> 4) + 2 * kk, b + 2 * kk, idesc, k || kk);
                 }
-                mma_commit(acc_full);
-                n++;
+                mma_commit_one(empty + 8 * s);
             }
-            if (!ok)
-                for (u32 i = 0; i < (1u << 16) && !mbar_try(acc_full, (n - 1) & 1); i++) {}
+            mma_commit_one(acc_full);
+            n++;
         }
+        if (!ok)
+            for (u32 i = 0; i < (1u << 16) && !mbar_try(acc_full, (n - 1) & 1); i++) {}
     } else if (warp < 6) {
         const u32 quarter = warp & 3;            // the lanes of TMEM that this warp may read
         u32 n = 0;

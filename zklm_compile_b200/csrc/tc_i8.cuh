@@ -28,9 +28,6 @@ inline cudaError_t allow_smem(void (*kernel)(KArgs...), size_t bytes) {
 __device__ __forceinline__ u32 smem_addr(const void* p) { return (u32)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void mbar_init(u32 bar, u32 count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
-__device__ __forceinline__ void mbar_expect(u32 bar, u32 bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void mbar_arrive(u32 bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool mbar_try(u32 bar, u32 parity) {
     u32 ok;
@@ -48,21 +45,17 @@ __device__ __forceinline__ bool mbar_wait(u32 bar, u32 parity, volatile int* gav
     return false;
 }
 
-// 16-byte aligned addresses, a size that is a multiple of 16.
-__device__ __forceinline__ void bulk_load(u32 dst, const void* src, u32 bytes, u32 bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-// x: innermost coordinate in elements (x times the element size is a multiple of 16 bytes).
-__device__ __forceinline__ void tensor_load_2d(u32 dst, const CUtensorMap* map, int x, int y, u32 bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
-                 : "memory");
-}
-
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // By one lane of a converged warp, all of whose lanes have the same operands: chosen inside the instruction's own statement, so that the compiler need not
 // provide for several lanes with operands of their own (a branch on the lane cost fifty instructions a copy).
 __device__ __forceinline__ void mbar_expect_one(u32 bar, u32 bytes) {
     asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; @p mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(bar), "r"(bytes) : "memory");
+}
+// x: innermost coordinate in elements (x times the element size is a multiple of 16 bytes).
+__device__ __forceinline__ void tensor_load_2d_one(u32 dst, const CUtensorMap* map, int x, int y, u32 bar) {
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff;\n"
+                 "@p cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4]; }" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void tensor_load_4d_one(u32 dst, const CUtensorMap* map, int x, int y, int z, int w, u32 bar) {
     asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff;\n"
@@ -86,12 +79,14 @@ __device__ __forceinline__ u64 smem_desc_sw128(u32 addr) {
 }
 // D s32, A and B unsigned bytes, 128 x n.
 ZKB_HD u32 i8_instr_desc(u32 n) { return (2u << 4) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
-__device__ __forceinline__ void mma_u8(u32 d, u64 a, u64 b, u32 idesc, bool accumulate) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((u32)accumulate)
+// These, too, by one lane of a converged warp - the same one every time, so that a commit covers the products before it.
+__device__ __forceinline__ void mma_u8_one(u32 d, u64 a, u64 b, u32 idesc, bool accumulate) {
+    asm volatile("{ .reg .pred p, q; elect.sync _|p, 0xffffffff; setp.ne.u32 q, %4, 0;\n"
+                 "@p tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, q; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((u32)accumulate)
                  : "memory");
 }
-__device__ __forceinline__ void mma_commit(u32 bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void mma_commit_one(u32 bar) {
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; @p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tmem_load16(u32 addr, u32 (&v)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
