@@ -175,19 +175,23 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
             for (u32 half = 0; half < 2; half++) {
                 const u32 row = half * 128 + quarter * 32 + lane;
                 if (half * 128 >= rows) break;
+                const u32 from = tmem + (quarter << 21) + half * 4 * p.tt;
                 for (u32 t0 = 0; t0 < p.tt; t0 += 16) {
                     u32 v[4][16];
 #pragma unroll
                     for (u32 g = 0; g < 4; g++)
-                        if (t0 + 4 * g < p.tt) tmem_load16(tmem + (quarter << 21) + half * 4 * p.tt + 4 * t0 + 16 * g, v[g]);
+                        if (t0 + 4 * g < p.tt) tmem_load16(from + 4 * t0 + 16 * g, v[g]);
                     tmem_wait_load();
+                    u32* to = slot + (size_t)t0 * LIN_ROWS + row;
 #pragma unroll
                     for (u32 g = 0; g < 4; g++)
                         if (t0 + 4 * g < p.tt) {
 #pragma unroll
-                            for (u32 e = 0; e < 4; e++)
-                                slot[(size_t)(t0 + 4 * g + e) * LIN_ROWS + row] =
-                                    red64((u64)v[g][4 * e] + ((u64)v[g][4 * e + 1] << 8) + ((u64)v[g][4 * e + 2] << 16) + ((u64)v[g][4 * e + 3] << 24));
+                            for (u32 e = 0; e < 4; e++) {
+                                // digits below 2^31: the value is below 2^56, and its two parts add up to less than 2^32, which will do for a term of a sum
+                                const u64 x = v[g][4 * e] + (u64)v[g][4 * e + 1] * (1u << 8) + (u64)v[g][4 * e + 2] * (1u << 16) + (u64)v[g][4 * e + 3] * (1u << 24);
+                                to[(4 * g + e) * LIN_ROWS] = ((u32)x & ZKB_P) + (u32)(x >> 31);
+                            }
                         }
                 }
             }
