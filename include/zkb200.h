@@ -534,7 +534,7 @@ int32_t zkb_oplist_prove(zkb_oplist* list, const uint32_t* x, uint8_t* out, size
  * elements and the centred integers they stand for, so a row computed over the cache is the row that zkb_row_attention(_gqa)_forward
  * computes and zkb_prove_row_attention(_gqa) proves, and a projection with an adapter is the product with the merged matrix W + B A.
  * All pointers are device memory of the context's GPU; calls are enqueued on the context's stream and nothing is waited for, so
- * they can be captured into a graph from that stream.  What only the device sees goes into the caller's status words, one per sequence:
+ * they can be captured into a graph from that stream (after a first call outside, which loads the kernels).  What only the device sees goes into the caller's status words, one per sequence:
  * status[s] becomes the largest code that a call found, and stays until the caller clears it. */
 enum { ZKB_SERVE_PAGE = 1,        /* a length or position outside the block table, or a page number outside the pool */
        ZKB_SERVE_ROTATION = 2,    /* a position that the rotation's table does not have */
@@ -566,8 +566,8 @@ typedef struct {
  * brings the tokens row_start[s] .. row_start[s + 1] - 1 (num_seqs + 1 nondecreasing entries); they get the positions from start[s] on, and
  * position p lies in row p % page_size of page block_table[s][p / page_size] (num_seqs x max_blocks entries; places that no new position needs
  * may hold anything).  Tokens before row_start[0] and from row_start[num_seqs] on are padding: nothing is written for them.  With a
- * rotation (NULL: none) K is rotated by its position, and q (num_tokens, num_heads, d_head) into q_out, which may be q itself; without one q is
- * copied.  Two sequences that append into one page in one call must not share its rows.  A token whose page or position is refused
+ * rotation (NULL: none) K is rotated by its position, and q (num_tokens, num_heads, d_head) into q_out, which is q itself or does not overlap it; without one
+ * q is copied.  Two sequences that append into one page in one call must not share its rows.  A token whose page or position is refused
  * (status) is left out; a value that does not fit a 16-bit cache is stored as its low 16 bits and reported. */
 int32_t zkb_kv_append(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint32_t* k_dev, size_t k_stride, const uint32_t* v_dev, size_t v_stride, uint32_t num_tokens,
                       const int32_t* block_table_dev, uint32_t num_seqs, uint32_t max_blocks, const int32_t* row_start_dev, const int32_t* start_dev,

@@ -471,3 +471,178 @@ def test_nothing_to_do(ctx):
     zs.kv_append(cache, z(1), z(1), 0, z(1), 1, 1, z(2), z(1), z(1))
     zs.adapter_linear(ctx, z(1), z(128), 0, 8, 16, z(1))
     assert ctx.launches == before
+
+
+# ---- strides, streams, graphs, threads ------------------------------------------------------------------------
+@pytest.mark.parametrize("pad", [4, 3])
+def test_append_rows_inside_wider_ones(ctx, pad):
+    """k, v and q as slices of a fused projection's rows, q_out with a stride of its own: on 16-byte boundaries and off them."""
+    rng = np.random.default_rng(pad)
+    h, kv, d, page, new, start = 4, 2, 32, 8, [3, 2], [6, 0]
+    t = sum(new) + 1
+    paged = Paged(ctx, rng, [9, 2], kv, d, page, False)
+    row = (h + 2 * kv) * d + pad
+    fused = np.stack([np.concatenate([small(rng, 127, h * d + kv * d), field(rng, kv * d + pad)]) for _ in range(t)])
+    q, k, v = (np.ascontiguousarray(fused[:, a:b]) for a, b in ((0, h * d), (h * d, (h + kv) * d), ((h + kv) * d, (h + 2 * kv) * d)))
+    buf, out = ctx.upload(fused), ctx.upload(np.full((t, h * d + pad), 9, np.uint32))
+    part = lambda at: zk.DeviceBuffer.wrap(ctx, buf_address(buf) + 4 * at, fused.size - at)
+    cs = rng.integers(-(1 << 14), 1 << 14, (9, d // 2, 2)).astype(np.int32)
+    status = ctx.upload(np.zeros(2, np.uint32))
+    rows = np.array([0, 3, 5], np.int32)
+    zs.kv_append(paged.cache, part(h * d), part((h + kv) * d), t, paged.table_dev, 2, paged.max_blocks, ctx.upload(words(rows)), ctx.upload(words(np.array(start, np.int32))), status,
+                 rotation=zs.Rotation(ctx.upload(words(cs)), 9, d, 14), q=part(0), q_out=out, num_heads=h, k_stride=row, v_stride=row, q_stride=row, q_out_stride=h * d + pad)
+    want = np.full((t, h, d), 9, np.int64)
+    assert not R.append(paged.k, paged.v, k.reshape(t, kv, d), v.reshape(t, kv, d), paged.table, rows, start, cs, 14, False, q.reshape(t, h, d), want).any()
+    got_k, got_v = paged.fetch()
+    assert np.array_equal(got_k, paged.k) and np.array_equal(got_v, paged.v)
+    got = out.download().reshape(t, -1)
+    assert np.array_equal(got[:, :h * d].reshape(t, h, d), want) and (got[:, h * d:] == 9).all() and not status.download().any()
+
+
+class Decoder:
+    """A layer's attention for one new token a sequence: fused projection with adapters, append with rotation, attention, output projection."""
+
+    def __init__(self, ctx, rng, lens, h=4, kv=2, d=32, page=8, model=48, rank=4, adapters=2, room=6):
+        self.ctx, self.lens, self.h, self.kv, self.d, self.model, self.b = ctx, list(lens), h, kv, d, model, len(lens)
+        self.rank, self.adapters = rank, adapters
+        self.paged = Paged(ctx, rng, [n + room for n in lens], kv, d, page, False)
+        self.qkv = (h + 2 * kv) * d
+        # weights in {-1, 0, 1} with few of them set, so that values stay small and scores inside the table
+        sparse = lambda *s: embed(rng.integers(-1, 2, s) * (rng.random(s) < 0.2))
+        self.w, self.w_out, self.a, self.bb = sparse(self.qkv, model), sparse(model, h * d), sparse(adapters, rank, model), sparse(adapters, self.qkv, rank)
+        self.of = rng.integers(-1, adapters, self.b)
+        angle = rng.uniform(0, 6.3, (max(lens) + room, d // 2))
+        self.cs = np.round(np.stack([np.cos(angle), np.sin(angle)], -1) * (1 << 14)).astype(np.int32)
+        self.table = tables.build_exp_table(1000)
+        up, z = ctx.upload, lambda n: ctx.upload(np.zeros(n, np.uint32))
+        self.dev = dict(w=up(self.w), w_out=up(self.w_out), a=up(self.a), b=up(self.bb), of=up(words(self.of.astype(np.int32))), cs=up(words(self.cs)), table=up(self.table),
+                        rows=up(words(np.arange(self.b + 1, dtype=np.int32))), fused=z(self.b * self.qkv), q=z(self.b * h * d), att=z(self.b * h * d), y=z(self.b * model), status=z(self.b),
+                        x=z(self.b * model), start=z(self.b), after=z(self.b))
+        self.ws = [z(zs.adapter_linear_workspace(ctx, self.b, self.qkv, model, adapters, rank) // 4 + 64), z(zs.adapter_linear_workspace(ctx, self.b, model, h * d) // 4 + 64),
+                   z(zs.paged_attention_workspace(self.paged.cache, self.b, h) // 4 + 64)]
+
+    def set(self, x):
+        import ctypes
+        from zklm_compile_b200 import _lib
+        for name, v in (("x", x), ("start", np.array(self.lens, np.uint32)), ("after", np.array(self.lens, np.uint32) + 1)):
+            v = np.ascontiguousarray(v, np.uint32).reshape(-1)
+            _lib.check(self.ctx.h, _lib.lib().zkb_buf_upload_u32(self.ctx.h, v.ctypes.data_as(_lib.u32p), ctypes.c_size_t(v.size), self.dev[name].ptr))
+
+    def step(self, workspaces=True):
+        ctx, v, h, kv, d, b = self.ctx, self.dev, self.h, self.kv, self.d, self.b
+        ws = self.ws if workspaces else [None] * 3
+        part = lambda at: zk.DeviceBuffer.wrap(ctx, buf_address(v["fused"]) + 4 * at, b * self.qkv - at)
+        zs.adapter_linear(ctx, v["x"], v["w"], b, self.qkv, self.model, v["fused"], adapters=zs.Adapters(v["a"], v["b"], self.adapters, self.rank), adapter_of=v["of"], workspace=ws[0])
+        zs.kv_append(self.paged.cache, part(h * d), part((h + kv) * d), b, self.paged.table_dev, b, self.paged.max_blocks, v["rows"], v["start"], v["status"],
+                     rotation=zs.Rotation(v["cs"], len(self.cs), d, 14), q=part(0), q_out=v["q"], num_heads=h, k_stride=self.qkv, v_stride=self.qkv, q_stride=self.qkv)
+        zs.paged_attention(self.paged.cache, v["q"], self.paged.table_dev, b, self.paged.max_blocks, v["after"], h, v["table"], v["att"], v["status"], score_shift=4, workspace=ws[2])
+        zs.adapter_linear(ctx, v["att"], v["w_out"], b, self.model, h * d, v["y"], workspace=ws[1])
+
+    def expect(self, x):
+        h, kv, d, b = self.h, self.kv, self.d, self.b
+        fused = R.linear(x, self.w, None, self.a, self.bb, self.of).reshape(b, -1, d)
+        q = np.zeros((b, h, d), np.int64)
+        status = R.append(self.paged.k, self.paged.v, fused[:, h:h + kv], fused[:, h + kv:], self.paged.table, list(range(b + 1)), self.lens, self.cs, 14, False, fused[:, :h], q)
+        att, more = R.attend(self.paged.k, self.paged.v, q, self.paged.table, np.array(self.lens) + 1, self.table, 4)
+        self.lens = [n + 1 for n in self.lens]
+        assert not status.any() and not more.any()
+        return R.linear(att.reshape(b, -1), self.w_out)
+
+    def check(self, want):
+        zs.check_status(self.ctx, self.dev["status"])
+        assert np.array_equal(self.dev["y"].download().reshape(self.b, -1), want)
+        got_k, got_v = self.paged.fetch()
+        assert np.array_equal(got_k, self.paged.k) and np.array_equal(got_v, self.paged.v)
+
+
+@pytest.mark.parametrize("workspaces", [False, True])
+def test_tokens_one_after_the_other(ctx, workspaces):
+    """Projection with adapters, rotation and append, attention, projection, token after token, against the definitions."""
+    rng = np.random.default_rng(21)
+    dec = Decoder(ctx, rng, [0, 5, 17, 8, 30])
+    for _ in range(4):
+        x = small(rng, 20, dec.b, dec.model)
+        dec.set(x)
+        dec.step(workspaces)
+        dec.check(dec.expect(x))
+
+
+def test_captured_steps_replayed(ctx):
+    """Two decoders' steps captured once each on the context's stream, with workspaces of their own, and replayed in turn for token after token."""
+    import torch
+    rng = np.random.default_rng(22)
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    decs = [Decoder(ctx, rng, [3, 9, 0, 14]), Decoder(ctx, rng, [40, 1], h=6, kv=2, d=64, page=16, model=64)]
+    graphs = []
+    for dec in decs:
+        x = small(rng, 20, dec.b, dec.model)
+        dec.set(x)
+        dec.step()
+        dec.check(dec.expect(x))
+        ctx.sync()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream, capture_error_mode="relaxed"):
+            dec.step()
+        graphs.append(g)
+    for _ in range(3):
+        xs = [small(rng, 20, dec.b, dec.model) for dec in decs]
+        for dec, x in zip(decs, xs):
+            dec.set(x)
+        with torch.cuda.stream(stream):
+            for g in graphs:
+                g.replay()
+        for dec, x in zip(decs, xs):
+            dec.check(dec.expect(x))
+
+
+def test_captured_call_without_a_workspace_is_refused(ctx):
+    import torch
+    rng = np.random.default_rng(23)
+    dec = Decoder(ctx, rng, [3])
+    dec.set(small(rng, 20, 1, dec.model))
+    dec.step()
+    ctx.sync()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(ctx.stream), capture_error_mode="relaxed"):
+        with pytest.raises(zk.ZkbError, match="workspace"):
+            dec.step(workspaces=False)
+
+
+def test_two_contexts_at_once():
+    """Two host threads, a context and a decoder each, with nothing between their streams."""
+    import threading
+    failures = []
+
+    def work(seed, lens):
+        try:
+            c = zk.Context(0)
+            rng = np.random.default_rng(seed)
+            dec = Decoder(c, rng, lens, room=9)
+            for _ in range(8):
+                x = small(rng, 20, dec.b, dec.model)
+                dec.set(x)
+                dec.step(workspaces=False)
+                dec.check(dec.expect(x))
+            c.close()
+        except BaseException as e:          # noqa: BLE001 - reported by the main thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(s, lens)) for s, lens in ((31, [0, 70, 3]), (32, [9, 9, 200, 1, 5]))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+
+
+def test_tensors_of_another_library(ctx):
+    """torch tensors are taken as they are; strided ones, ones of another type and ones on the host are refused."""
+    import torch
+    x, w, out = (torch.randint(0, P, s, dtype=torch.int32, device="cuda") for s in ((3, 64), (40, 64), (3, 40)))
+    torch.cuda.synchronize()
+    zs.adapter_linear(ctx, x, w, 3, 40, 64, out)
+    ctx.sync()
+    assert np.array_equal(out.cpu().numpy(), R.linear(x.cpu().numpy(), w.cpu().numpy()))
+    for bad in (x.t(), x.to(torch.int64), x.cpu(), [1, 2]):
+        with pytest.raises((ValueError, TypeError)):
+            zs.adapter_linear(ctx, bad, w, 3, 40, 64, out)

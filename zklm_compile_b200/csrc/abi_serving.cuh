@@ -119,6 +119,7 @@ size_t zkb_paged_attention_workspace(zkb_ctx* c, const zkb_kv_cache* cache, uint
         paged_attention_dims(k, num_heads, num_seqs);
         return paged_attention_workspace(c->sm_count, num_heads, k.num_kv_heads, k.d, num_seqs);
     } catch (const ArgFail& e) { c->err = e.msg; return 0; }
+    catch (const std::bad_alloc&) { return 0; }
 }
 int32_t zkb_paged_attention(zkb_ctx* c, const zkb_kv_cache* cache, const uint32_t* q_dev, size_t q_stride, uint32_t num_heads, const int32_t* block_table_dev,
                             uint32_t num_seqs, uint32_t max_blocks, const int32_t* lens_dev, const uint32_t* table_out_dev, size_t n_table, uint32_t score_shift,
@@ -163,6 +164,7 @@ size_t zkb_adapter_linear_workspace(zkb_ctx* c, uint32_t tokens, uint32_t m, uin
         adapter_linear_dims(tokens, m, n, num_adapters, rank);
         return adapter_linear_workspace(c->sm_count, tokens, m, n, num_adapters, rank);
     } catch (const ArgFail& e) { c->err = e.msg; return 0; }
+    catch (const std::bad_alloc&) { return 0; }
 }
 int32_t zkb_adapter_linear(zkb_ctx* c, const uint32_t* x_dev, size_t x_stride, const uint32_t* w_dev, const uint32_t* bias_dev, uint32_t tokens, uint32_t m, uint32_t n,
                            const uint32_t* a_dev, const uint32_t* b_dev, uint32_t num_adapters, uint32_t rank, const int32_t* adapter_of_dev, uint32_t* y_dev,

@@ -57,6 +57,7 @@ int32_t zkb_ctx_create(int32_t device, zkb_ctx** out) {
         c->rec_cap = size_t(1) << 21;                       // 8 MiB of proof record (a layer with eight Basefold openings needs ~4)
         ZKB_CUDA(cudaMalloc(&c->rec_dev, c->rec_cap * 4));
         ZKB_CUDA(cudaHostAlloc(&c->rec_host, c->rec_cap * 4, cudaHostAllocDefault));
+        c->serve_flag();                                    // not at its first use, which may be inside a stream capture
         ZKB_CUDA(cudaEventCreate(&c->t0));
         ZKB_CUDA(cudaEventCreate(&c->t1));
         ZKB_CUDA(cudaStreamSynchronize(c->stream));
