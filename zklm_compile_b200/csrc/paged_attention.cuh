@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         for (int w = 0; w < WARPS; w++) total += sums[w];
     }
     total *= grps;
-    u64 per = (total + P.ctas - 1) / P.ctas;
+    u64 per = total >> 31 ? (total + P.ctas - 1) / P.ctas : ((u32)total + P.ctas - 1) / P.ctas;      // a 64-bit division is hundreds of cycles
     // Where the rows are fewer than the CTAs each CTA keeps to one row (`aligned`: a share is `per` blocks of one item), if that costs no one much more;
     // a second row in a CTA costs as much as several blocks.
     bool aligned = false;
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     cw.block = BLOCK;
     cw.slices = P.slices;
     cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
-    const u32 parts = aligned ? (u32)((cw.nb + per - 1) / per) : cw.nb, start_grp = (u32)(start_rest / parts);       // of an item, in what the rest is counted in
+    const u32 parts = aligned ? (cw.nb + (u32)per - 1) / (u32)per : cw.nb, start_grp = start_rest >> 32 ? (u32)(start_rest / parts) : (u32)start_rest / parts;       // of an item, in what the rest is counted in
     cw.kvh = start_grp / P.slices;
     cw.slice = start_grp - cw.kvh * P.slices;
     cw.blk = (u32)(start_rest - (u64)start_grp * parts) * (aligned ? (u32)per : 1u);
@@ -288,7 +288,31 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         if (is_v) { lw.step(A, 1); fetch_page(); }
         slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
     };
+    // A thread's elements of q for a row: four words' places of one head for each of its items, fetched ahead of their use.
+    constexpr int Q_ITEMS = (HEADS * J * 4 + THREADS - 1) / THREADS;
+    constexpr u32 Q_WORDS = SMALL ? 8 : 4;
+    u32 qv[Q_ITEMS][Q_WORDS];
+    auto fetch_q = [&](u32 seq, u32 head0, u32 heads) {
+#pragma unroll
+        for (int it = 0; it < Q_ITEMS; it++) {
+            const u32 i = tid + it * THREADS, head = i / (J * 4), e0 = (16 * (i / 4 % J) + 4 * (i & 3)) * (SMALL ? 2 : 1);
+            const u32* from_q = A.q + seq * A.q_stride + (size_t)(head0 + head) * d + e0;
+#pragma unroll
+            for (u32 k = 0; k < Q_WORDS; k += 4) {
+                if (P.q_vec) {
+                    const uint4 t = head < heads && e0 + k < d ? *reinterpret_cast<const uint4*>(from_q + k) : make_uint4(0, 0, 0, 0);
+                    qv[it][k] = t.x; qv[it][k + 1] = t.y; qv[it][k + 2] = t.z; qv[it][k + 3] = t.w;
+                } else {
+#pragma unroll
+                    for (u32 e = k; e < k + 4; e++) qv[it][e] = head < heads && e0 + e < d ? from_q[e] : 0u;
+                }
+            }
+        }
+    };
+    auto heads_of = [&](const PaWalk& w) { const u32 rest = hpg - w.slice * P.slice_heads; return rest < P.slice_heads ? rest : P.slice_heads; };
+    auto head0_of = [&](const PaWalk& w) { return w.kvh * hpg + w.slice * P.slice_heads; };
     fetch_page();
+    fetch_q(cw.seq, head0_of(cw), heads_of(cw));
 #pragma unroll
     for (int h = 0; h < NS; h++) load_half(h & 1);
 
@@ -304,36 +328,25 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
     // ---- the stretches of items ---------------------------------------------------------------------
     u32 computed = 0;
     while (cw.left) {
-        const u32 seq = cw.seq, head0 = cw.kvh * hpg + cw.slice * P.slice_heads, rest = hpg - cw.slice * P.slice_heads, heads = rest < P.slice_heads ? rest : P.slice_heads;
+        const u32 seq = cw.seq, head0 = head0_of(cw), heads = heads_of(cw);
         const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? cw.left : nb - first;
         __syncthreads();                        // the row before is done with these arrays
         // The right operand of the scores: a thread takes four words' places of one head, whose digits are four lanes' 16 bytes for steps 2j and 2j + 1.
-        for (u32 i = tid; i < HEADS * J * 4; i += THREADS) {
-            const u32 head = i / (J * 4), j = i / 4 % J, qq = i & 3, e0 = (16 * j + 4 * qq) * (SMALL ? 2 : 1);
-            constexpr u32 N = SMALL ? 8 : 4;
-            const u32* from_q = A.q + seq * A.q_stride + (size_t)(head0 + head) * d + e0;
-            u32 qv[N];
 #pragma unroll
-            for (u32 k = 0; k < N; k += 4) {
-                if (P.q_vec) {
-                    const uint4 t = head < heads && e0 + k < d ? *reinterpret_cast<const uint4*>(from_q + k) : make_uint4(0, 0, 0, 0);
-                    qv[k] = t.x; qv[k + 1] = t.y; qv[k + 2] = t.z; qv[k + 3] = t.w;
-                } else {
-#pragma unroll
-                    for (u32 e = k; e < k + 4; e++) qv[e] = head < heads && e0 + e < d ? from_q[e] : 0u;
-                }
-            }
+        for (int it = 0; it < Q_ITEMS; it++) {
+            const u32 i = tid + it * THREADS, head = i / (J * 4), j = i / 4 % J, qq = i & 3;
+            if (i >= HEADS * J * 4) break;
             u32 w[4][4];                         // [column c][word]
 #pragma unroll
             for (u32 k = 0; k < 4; k++) {
                 u32 da[4], db[4];
                 if (SMALL) {
-                    digit_words(qv[2 * k % N], da);
-                    digit_words(qv[(2 * k + 1) % N], db);
+                    digit_words(qv[it][2 * k % Q_WORDS], da);
+                    digit_words(qv[it][(2 * k + 1) % Q_WORDS], db);
 #pragma unroll
                     for (u32 c = 0; c < 4; c++) w[c][k] = __byte_perm(da[c], db[c], 0x5410);
                 } else {
-                    digit_words(qv[k], da);
+                    digit_words(qv[it][k], da);
 #pragma unroll
                     for (u32 c = 0; c < 4; c++) w[c][k] = da[c];
                 }
@@ -343,7 +356,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             if (SMALL) {                         // what flipped top bits add to a score, 2^15 sum q, is taken off its digits 0 and 2 at the start; J * 4 lanes have a head
                 u64 sum = 0;
 #pragma unroll
-                for (u32 k = 0; k < N; k++) sum += qv[k];
+                for (u32 k = 0; k < Q_WORDS; k++) sum += qv[it][k];
 #pragma unroll
                 for (u32 o = J * 2; o > 0; o >>= 1) sum += __shfl_xor_sync(J * 4 == 32 ? 0xffffffffu : ((1u << (J * 4 % 32)) - 1) << (lane & ~(J * 4 - 1)), sum, o);
                 if ((lane & (J * 4 - 1)) == 0) off_q[head] = neg31(mul31(red64(sum), 32768u));
@@ -539,7 +552,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
         if (!(begins && ends)) {
             // The CTA that brings a row's last part adds the parts up.  They lie in the slot of the CTA in which the row begins and those of the next ones.
             const u64 at = to - cw.left, row0 = at - first;
-            const u32 c0 = aligned ? blockIdx.x - first / (u32)per : (u32)(row0 / per), n = aligned ? (u32)((nb + per - 1) / per) : (u32)((row0 + nb - 1) / per) - c0 + 1;
+            const u32 c0 = aligned ? blockIdx.x - first / (u32)per : (u32)(row0 / per), n = aligned ? (nb + (u32)per - 1) / (u32)per : (u32)((row0 + nb - 1) / per) - c0 + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -551,6 +564,19 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
             if (last_part) {
                 __threadfence();
                 auto slot_of = [&](u32 k) { return P.slots + (size_t)(2 * (c0 + k) + (k ? 0 : 1)) * HEADS * (DP + 4); };
+                constexpr int PER = (HEADS * DP + THREADS - 1) / THREADS;
+                u64 sum[PER];                    // the elements' loads are under way while the weights are added up and inverted
+#pragma unroll
+                for (int v = 0; v < PER; v++) sum[v] = 0;
+#pragma unroll 2
+                for (u32 k = 0; k < n; k++) {
+                    const u32* from_slot = slot_of(k);
+#pragma unroll
+                    for (int v = 0; v < PER; v++) {
+                        const u32 i = tid + v * THREADS;
+                        if (i < heads * DP) sum[v] += __ldcg(from_slot + i / DP * (DP + 4) + i % DP);
+                    }
+                }
                 for (u32 h = warp; h < heads; h += WARPS) {
                     u64 s = 0;
                     u32 f = 0;
@@ -563,24 +589,23 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_atten
                     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
                     f = __reduce_or_sync(0xffffffffu, f);
                     if (lane == 0) {
-                        const u32 sum = red64(s);
-                        const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : sum == 0 ? SERVE_ZERO_SUM : 0;
+                        const u32 all = red64(s);
+                        const int code = f & PA_BAD_PAGE ? SERVE_PAGE : f & PA_BAD_SCORE ? SERVE_SCORE : all == 0 ? SERVE_ZERO_SUM : 0;
                         if (code) atomicMax(A.status + seq, code);
-                        inv[h] = code ? 0u : inv31_chain(sum);
-                        corr[h] = SMALL ? mul31(sum, 32768u) : 0u;
+                        inv[h] = code ? 0u : inv31_chain(all);
+                        corr[h] = SMALL ? mul31(all, 32768u) : 0u;
                     }
                 }
                 __syncthreads();
-                for (u32 i = tid; i < heads * DP; i += THREADS) {
-                    const u32 h = i / DP, e = i % DP;
-                    u64 sum = 0;
-#pragma unroll 8
-                    for (u32 k = 0; k < n; k++) sum += __ldcg(slot_of(k) + h * (DP + 4) + e);
-                    if (e < d) pa_finish(A, seq, head0 + h, e, red64(sum), inv[h], corr[h]);
+#pragma unroll
+                for (int v = 0; v < PER; v++) {
+                    const u32 i = tid + v * THREADS, h = i / DP, e = i % DP;
+                    if (i < heads * DP && e < d) pa_finish(A, seq, head0 + h, e, red64(sum[v]), inv[h], corr[h]);
                 }
             }
         }
         cw.step(A, count);
+        if (cw.left) fetch_q(cw.seq, head0_of(cw), heads_of(cw));
     }
     if (gave_up) {                              // nothing of this warp may still be in flight when it ends
         for (u32 h = 0; h < NS; h++) {
@@ -601,7 +626,7 @@ inline PaChoice pa_choice(u32 d, u32 hpg) {
     const u32 most = c.dp == 256 ? 4 : 8;
     c.slices = (hpg + most - 1) / most;
     c.slice_heads = (hpg + c.slices - 1) / c.slices;
-    c.nt = c.slice_heads <= 2 ? 1 : (c.slice_heads <= 4 ? 2 : 4);
+    c.nt = c.dp == 256 ? (c.slice_heads <= 2 ? 1 : 2) : (c.slice_heads + 1) / 2;
     return c;
 }
 template <int DP, bool SMALL, int NT>

@@ -87,7 +87,7 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
 #define ZKB_PA(DP, NT)                                                                              \
     case DP | NT << 16: return pa_launch<DP, false, NT>(stream, maps, a, w, launches);                     \
     case DP | NT << 16 | 1u << 24: return pa_launch<DP, true, NT>(stream, maps, a, w, launches);
-        ZKB_PA(64, 1) ZKB_PA(64, 2) ZKB_PA(64, 4) ZKB_PA(128, 1) ZKB_PA(128, 2) ZKB_PA(128, 4) ZKB_PA(256, 1) ZKB_PA(256, 2)
+        ZKB_PA(64, 1) ZKB_PA(64, 2) ZKB_PA(64, 3) ZKB_PA(64, 4) ZKB_PA(128, 1) ZKB_PA(128, 2) ZKB_PA(128, 3) ZKB_PA(128, 4) ZKB_PA(256, 1) ZKB_PA(256, 2)
 #undef ZKB_PA
     }
     return cudaErrorInvalidValue;
