@@ -41,11 +41,11 @@ __device__ __forceinline__ u32 inv31_chain(u32 x) {
 // How the kernels are built for a head of up to DP elements: warps, and half tiles (16 keys or 16 values) in a warp's ring.  A half tile lies as the
 // tensor copies leave it: columns of 128 bytes, 16 rows of one behind the other, the 16-byte groups of a row swizzled by the row's low bits.
 // Which position becomes which row of an operand is free, and is chosen so that no two lanes of a phase meet in a bank.
-template <int DP, bool SMALL>
+template <int DP, bool SMALL, int NT>
 struct PaShape {
     static constexpr int RB = DP * (SMALL ? 2 : 4);
-    static constexpr int WARPS = RB >= 1024 ? 5 : 8;
-    static constexpr int NS = RB >= 512 ? 2 : (RB == 256 ? 4 : 6);
+    static constexpr int WARPS = RB >= 1024 ? 5 : (RB <= 256 && NT <= 2 ? 12 : 8);
+    static constexpr int NS = RB >= 512 ? 2 : (RB == 256 ? (WARPS == 12 ? 3 : 4) : 6);
     static constexpr int HALF = 16 * RB;       // bytes of a slot
     static constexpr int ED = SMALL ? 256 : 512;   // bytes of a tile's weights, as digits, per tile of columns
 };
@@ -89,9 +89,9 @@ __device__ __forceinline__ void pa_finish(const PagedAttnArgs& A, u32 seq, u32 h
 }
 
 template <int DP, bool SMALL, int NT>
-__global__ void __launch_bounds__(PaShape<DP, SMALL>::WARPS * 32, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                                    PagedAttnArgs A, PaWork P) {
-    using S = PaShape<DP, SMALL>;
+    using S = PaShape<DP, SMALL, NT>;
     constexpr int WARPS = S::WARPS, NS = S::NS, RB = S::RB, J = RB / 64, VJ = RB / 128, MT = DP / 16, HEADS = 2 * NT, THREADS = WARPS * 32;
     constexpr u32 BLOCK = WARPS * 16;
     extern __shared__ __align__(16) unsigned char pa_raw[];
@@ -631,7 +631,7 @@ inline PaChoice pa_choice(u32 d, u32 hpg) {
 }
 template <int DP, bool SMALL, int NT>
 inline cudaError_t pa_launch(cudaStream_t stream, const CUtensorMap (&maps)[2], const PagedAttnArgs& a, PaWork w, int* launches) {
-    using S = PaShape<DP, SMALL>;
+    using S = PaShape<DP, SMALL, NT>;
     constexpr size_t smem = (size_t)S::WARPS * S::NS * S::HALF + (size_t)S::RB / 64 * NT * 512 + (size_t)S::WARPS * 2 * NT * DP * 4 + (size_t)S::WARPS * NT * S::ED + 1024;
     static_assert(smem <= 226 * 1024, "with the kernel's own arrays below the 227 KB of a CTA");
     cudaError_t e = allow_smem(paged_attention_kernel<DP, SMALL, NT>, smem);
