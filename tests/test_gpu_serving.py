@@ -386,6 +386,21 @@ def test_linear_every_value_at_its_largest(ctx, t):
         check_linear(ctx, x, w)
 
 
+@pytest.mark.parametrize("t,m,n,count,rank", [(300, 5000, 40, 2, 130), (300, 5000, 33, 3, 66), (9, 70, 64, 2, 300), (5, 130, 36, 30, 65), (700, 3300, 36, 5, 20), (400, 4100, 20, 1, 64)])
+def test_linear_with_adapters_of_many_ranks_and_rows(ctx, t, m, n, count, rank):
+    """Ranks beyond one pass of the join, and joins whose CTAs take several blocks of rows."""
+    rng = np.random.default_rng(rank)
+    of = np.sort(rng.integers(-1, count, t)) if t > 50 else rng.integers(-1, count, t)
+    check_linear(ctx, field(rng, t, n), field(rng, m, n), field(rng, m), field(rng, count, rank, n), field(rng, count, m, rank), of)
+
+
+@pytest.mark.parametrize("count,rank", [(2, 4), (600, 3)])
+def test_linear_more_tokens_than_one_pass_takes(ctx, count, rank):
+    rng = np.random.default_rng(rank)
+    t, m, n = 2100, 24, 36
+    check_linear(ctx, field(rng, t, n), field(rng, m, n), field(rng, m), field(rng, count, rank, n), field(rng, count, m, rank), rng.integers(-1, count, t), x_pad=4, y_pad=4)
+
+
 @pytest.mark.parametrize("t", [1, 12, 30, 36, 48, 61, 64, 100])
 @pytest.mark.parametrize("m,n", [(6000, 2048), (5000, 2051), (300, 20000)])
 def test_linear_many_steps(ctx, t, m, n):
