@@ -92,7 +92,7 @@ struct LinWalk {                               // a CTA's stretches, the same fo
 };
 
 // Warp 0 copies W, warp 1 issues, warps 2 to 5 empty the accumulators, the others make the tokens' operand from x: 16 bytes of it a value, which would
-// be four times x to copy (that was bound by L2: 0.92 us a step of 64 KB at 256 columns).  W_COPY: W by tensor copies; otherwise (rows that start on no
+// be four times x to copy, and a kernel of its own to make (332 against 260 us for 1024 x 4096 x 4096).  W_COPY: W by tensor copies; otherwise (rows that start on no
 // 16-byte boundary) word by word, by the warps that fill.
 template <bool W_COPY>
 __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, LinPlan p, LinearArgs A, int x_vec,
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(LIN_THREADS) linear_bytes_kernel(const __grid_
     } else {
         // Each team of warps takes every third step, so that three steps' loads are under way.  There are at least as many stages as teams: a team knows that
         // the stage of its last step was empty, and from that that its next one's was emptied the time before last; with fewer stages than teams it could
-        // be two phases ahead, where a wait by parity sees the wrong one.  (Two warps a step took 0.92 us a step of 64 tokens.)
+        // be two phases ahead, where a wait by parity sees the wrong one.  (1024 x 4096 x 4096 with teams of two 253 us, of four 248.)
         constexpr u32 teams = LIN_FILL / LIN_TEAM;
         const u32 team = (warp - 6) / LIN_TEAM, member = (warp - 6) % LIN_TEAM;
         constexpr u32 GROUPS = LIN_TOKENS / (4 * LIN_TEAM);
@@ -287,6 +287,25 @@ __device__ __forceinline__ u32 lin_first(const LinPlan& p, u32 tile, u32 seg) { 
 __device__ __forceinline__ u32 lin_last(const LinPlan& p, u32 tile, u32 seg) {
     return (tile * p.steps + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps) - 1) / p.per;
 }
+// Adds the slots' sums of rows row .. row + 3 of tile mt (one tile's; `vec`: row is a multiple of 4) for a token of tile nt.
+__device__ __forceinline__ void lin_sum4(const LinPlan& p, const u32* __restrict__ slots, u32 mt, u32 nt, u32 in_tile, u32 row, bool vec, u64 (&v)[4]) {
+    const u32 tile = mt * p.ntiles + nt;
+    const u32* at = slots + (size_t)in_tile * LIN_ROWS + row;
+    for (u32 seg = 0; seg < p.segs; seg++) {
+        const u32 from = lin_first(p, tile, seg), to = lin_last(p, tile, seg);
+        const u32* s = at + ((size_t)from + (size_t)tile * p.segs + seg) * p.slot_words;
+        if (vec) {
+#pragma unroll 4
+            for (u32 c = from; c <= to; c++, s += p.slot_words) {
+                const uint4 x = *reinterpret_cast<const uint4*>(s);
+                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+            }
+        } else {
+#pragma unroll 4
+            for (u32 c = from; c <= to; c++, s += p.slot_words) { v[0] += s[0]; v[1] += s[1]; v[2] += s[2]; v[3] += s[3]; }
+        }
+    }
+}
 // Four products of field elements fit 64 bits.
 __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
     const u64 s = (u64)a[0] * b[0] + (u64)a[1] * b[1] + (u64)a[2] * b[2] + (u64)a[3] * b[3];
@@ -294,7 +313,7 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
 }
 // One CTA: `blocks` times 64 rows, up to 16 tokens of a tile of tokens.  B (A x) is a product of bytes too, on the warps' tensor cores: the rows of B are the left operand as
 // they lie in memory, read once for all tokens beside each other that have the same adapter (a run); each token's A x has four columns in the
-// right one, zero for the adapters of other tokens.  (With a multiplication a term this was 47 of 260 us for 1024 tokens of rank 32; now 17.)
+// right one, zero for the adapters of other tokens.  What bounds it is latency, slots first: 45 us for 1024 tokens of rank 32 and 4096 rows, 21 without adapters.
 constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 64;
 __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, int y_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
     __shared__ uint4 ud[LIN_JOIN_RANK / 16][LIN_JOIN_TOKENS / 2][32];              // digits of A x, 64 of the rank at a time
@@ -326,118 +345,97 @@ __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPl
     }
     // A x from column rb of the rank on, four of it a thread, and its digits
     auto make_digits = [&](u32 rb) {
-                        const u32 t = tid >> 4, r0 = rb + 4 * (tid & 15);
-                        u64 v[4] = {0, 0, 0, 0};
-                        if (t < count && of[t] >= 0 && r0 < rank) {
-                            if (!p.a_rows) {
-        #pragma unroll
-                                for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? u_own[(size_t)(t0 + t) * rank + r0 + k] : 0u;
-                            } else if (rank % 4 == 0) {  // four neighbours of one tile
-                                const u32 a_row = (u32)of[t] * rank + r0, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
-                                const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
-                                for (u32 seg = 0; seg < p.segs; seg++) {
-                                    const u32 last = lin_last(p, tile, seg);
-        #pragma unroll 4
-                                    for (u32 c = lin_first(p, tile, seg); c <= last; c++) {
-                                        const uint4 x = *reinterpret_cast<const uint4*>(from + ((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words);
-                                        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-                                    }
-                                }
-                            } else {
-                                for (u32 k = 0; k < 4 && r0 + k < rank; k++) {
-                                    const u32 a_row = (u32)of[t] * rank + r0 + k, tile = (p.wtiles + a_row / LIN_ROWS) * p.ntiles + nt;
-                                    const u32* from = slots + (size_t)(in_tile + t) * LIN_ROWS + a_row % LIN_ROWS;
-                                    u64 sum = 0;
-                                    for (u32 seg = 0; seg < p.segs; seg++) {
-                                        const u32 last = lin_last(p, tile, seg);
-        #pragma unroll 4
-                                        for (u32 c = lin_first(p, tile, seg); c <= last; c++) sum += from[((size_t)c + (size_t)tile * p.segs + seg) * p.slot_words];
-                                    }
-                                    if (k == 0) v[0] = sum; else if (k == 1) v[1] = sum; else if (k == 2) v[2] = sum; else v[3] = sum;
-                                }
-                            }
-                        }
-                        u32 w[4][4];
-        #pragma unroll
-                        for (u32 k = 0; k < 4; k++) {
-                            u32 d[4];
-                            digit_words(red64(v[k]), d);
-        #pragma unroll
-                            for (u32 c = 0; c < 4; c++) w[c][k] = d[c];
-                        }
-                        const u32 at = tid & 15;
-        #pragma unroll
-                        for (u32 c = 0; c < 4; c++) ud[at >> 2][t >> 1][((t & 1) * 4 + c) * 4 + (at & 3)] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+        const u32 t = tid >> 4, at = tid & 15, r0 = rb + 4 * at;
+        u64 v[4] = {0, 0, 0, 0};
+        if (t < count && of[t] >= 0 && r0 < rank) {
+            const u32 a_row = (u32)of[t] * rank + r0, in = a_row % LIN_ROWS;       // what lies behind the adapter's last row is not used
+            if (!p.a_rows) {
+#pragma unroll
+                for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? u_own[(size_t)(t0 + t) * rank + r0 + k] : 0u;
+            } else if (in + 4 <= LIN_ROWS) {
+                lin_sum4(p, slots, p.wtiles + a_row / LIN_ROWS, nt, in_tile + t, in, rank % 4 == 0, v);
+            } else {                             // the four lie in two tiles: each with the last four rows of its own
+                for (u32 k = 0; k < 4 && r0 + k < rank; k++) {
+                    u64 x[4] = {0, 0, 0, 0};
+                    const u32 r = (a_row + k) % LIN_ROWS, back = r < 4 ? r : 3;
+                    lin_sum4(p, slots, p.wtiles + (a_row + k) / LIN_ROWS, nt, in_tile + t, r - back, false, x);
+                    v[k] = back == 0 ? x[0] : back == 1 ? x[1] : back == 2 ? x[2] : x[3];
+                }
+            }
+        }
+        u32 w[4][4];
+#pragma unroll
+        for (u32 k = 0; k < 4; k++) {
+            u32 d[4];
+            digit_words(r0 + k < rank ? red64(v[k]) : 0u, d);
+#pragma unroll
+            for (u32 c = 0; c < 4; c++) w[c][k] = d[c];
+        }
+#pragma unroll
+        for (u32 c = 0; c < 4; c++) ud[at >> 2][t >> 1][((t & 1) * 4 + c) * 4 + (at & 3)] = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
     };
-    pdl_wait();
     const u32 g = lane >> 2, q4 = lane & 3, nt0 = (warp >> 2) * 4;
     const bool odd = q4 & 1;
     const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
+    int run_n[4];                              // the run of this lane's column in each of the warp's tiles of columns
+#pragma unroll
+    for (u32 n = 0; n < 4; n++) run_n[n] = n_runs ? run_of[2 * (nt0 + n) + (lane >> 4)] : -1;
+    // Rows row_a and row_a + 8 of B, columns 4 q4 .. + 3 of 16, for step x of a pass over the rank: its adapters' 16 columns one behind the other
+    auto load_b = [&](u32 rb, u32 x, u32 row_a, u32 (&fa)[4], u32 (&fc)[4]) {
+        const u32 chunk = x / n_runs, r = rb + 16 * chunk + 4 * q4;
+        const u32* from = A.b + ((size_t)run_adapter[x - chunk * n_runs] * A.m + row_a) * rank + r;
+        const u32* from8 = from + 8 * (size_t)rank;
+        if (b_vec) {
+            const uint4 va = r < rank && row_a < A.m ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+            const uint4 vc = r < rank && row_a + 8 < A.m ? *reinterpret_cast<const uint4*>(from8) : make_uint4(0, 0, 0, 0);
+            fa[0] = va.x; fa[1] = va.y; fa[2] = va.z; fa[3] = va.w;
+            fc[0] = vc.x; fc[1] = vc.y; fc[2] = vc.z; fc[3] = vc.w;
+        } else {
+#pragma unroll
+            for (u32 e = 0; e < 4; e++) {
+                fa[e] = r + e < rank && row_a < A.m ? from[e] : 0u;
+                fc[e] = r + e < rank && row_a + 8 < A.m ? from8[e] : 0u;
+            }
+        }
+    };
+    auto multiply = [&](u32 x, const u32 (&fa)[4], const u32 (&fc)[4], int (&acc)[4][4]) {
+        const u32 chunk = x / n_runs;
+        const int run = (int)(x - chunk * n_runs);
+#pragma unroll
+        for (u32 n = 0; n < 4; n++) {
+            if (!__any_sync(0xffffffffu, run_n[n] == run)) continue;
+            const uint4 b = run_n[n] == run ? ud[chunk][nt0 + n][lane] : make_uint4(0, 0, 0, 0);
+            mma_u8_16x8x32(acc[n], fa[0], fc[0], fa[1], fc[1], b.x, b.y);
+            mma_u8_16x8x32(acc[n], fa[2], fc[2], fa[3], fc[3], b.z, b.w);
+        }
+    };
+    pdl_wait();
     if (n_runs) make_digits(0);
     // a thread has one token and four rows of a block
     const bool has = mine < count;
-    const u32 tile = begin / LIN_ROWS * p.ntiles + nt, first = lin_first(p, tile, 0), last = lin_last(p, tile, 0);       // the rows of a CTA lie in one tile
     for (u32 i0 = begin; i0 < stop; i0 += LIN_JOIN_ROWS) {
         const u32 i = i0 + quad, row_a = i0 + (warp & 3) * 16 + g;
         u64 y[4];
 #pragma unroll
         for (u32 e = 0; e < 4; e++) y[e] = A.bias && i + e < A.m ? A.bias[i + e] : 0u;
-        if (has && i < A.m) {                  // rows of the tile that are behind the last one hold nothing of use, but are there
-            const u32* at = slots + (size_t)(in_tile + mine) * LIN_ROWS + i % LIN_ROWS;
-            for (u32 seg = 0; seg < p.segs; seg++) {
-                const u32 from = seg ? lin_first(p, tile, seg) : first, to = seg ? lin_last(p, tile, seg) : last;
-                const u32* s = at + ((size_t)from + (size_t)tile * p.segs + seg) * p.slot_words;
-#pragma unroll 4
-                for (u32 c = from; c <= to; c++, s += p.slot_words) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(s);
-                    y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
-                }
-            }
-        }
+        // rows of the tile that are behind the last one hold nothing of use, but are there
+        if (has && i < A.m) lin_sum4(p, slots, i / LIN_ROWS, nt, in_tile + mine, i % LIN_ROWS, true, y);
         if (n_runs) {
             int acc[4][4] = {};
             for (u32 rb = 0; rb < rank; rb += LIN_JOIN_RANK) {
+                const u32 steps = ((rank - rb < LIN_JOIN_RANK ? rank - rb : LIN_JOIN_RANK) + 15) / 16 * (u32)n_runs;
                 if (rb || (rank > LIN_JOIN_RANK && i0 > begin)) {
                     __syncthreads();
                     make_digits(rb);
                 }
                 __syncthreads();
-                for (u32 r0 = rb; r0 < rank && r0 < rb + LIN_JOIN_RANK; r0 += 16)
-                    for (int run0 = 0; run0 < n_runs; run0 += 2) {
-                        u32 fa[2][4], fc[2][4];     // rows row_a and row_a + 8 of up to two adapters, columns r0 + 4 q4 .. + 3
-    #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            if (run0 + k >= n_runs) break;
-                            const u32* from = A.b + ((size_t)run_adapter[run0 + k] * A.m + row_a) * rank + r0 + 4 * q4;
-                            const u32* from8 = from + 8 * (size_t)rank;
-                            if (b_vec) {
-                                const bool in = r0 + 4 * q4 < rank;
-                                const uint4 va = in && row_a < A.m ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
-                                const uint4 vc = in && row_a + 8 < A.m ? *reinterpret_cast<const uint4*>(from8) : make_uint4(0, 0, 0, 0);
-                                fa[k][0] = va.x; fa[k][1] = va.y; fa[k][2] = va.z; fa[k][3] = va.w;
-                                fc[k][0] = vc.x; fc[k][1] = vc.y; fc[k][2] = vc.z; fc[k][3] = vc.w;
-                            } else {
-    #pragma unroll
-                                for (u32 e = 0; e < 4; e++) {
-                                    const bool in = r0 + 4 * q4 + e < rank;
-                                    fa[k][e] = in && row_a < A.m ? from[e] : 0u;
-                                    fc[k][e] = in && row_a + 8 < A.m ? from8[e] : 0u;
-                                }
-                            }
-                        }
-    #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            if (run0 + k >= n_runs) break;
-    #pragma unroll
-                            for (u32 n = 0; n < 4; n++) {
-                                const u32 tok = 2 * (nt0 + n);
-                                if (run_of[tok] != run0 + k && run_of[tok + 1] != run0 + k) continue;
-                                const uint4 b = run_of[tok + (lane >> 4)] == run0 + k ? ud[(r0 - rb) / 16][nt0 + n][lane] : make_uint4(0, 0, 0, 0);
-                                mma_u8_16x8x32(acc[n], fa[k][0], fc[k][0], fa[k][1], fc[k][1], b.x, b.y);
-                                mma_u8_16x8x32(acc[n], fa[k][2], fc[k][2], fa[k][3], fc[k][3], b.z, b.w);
-                            }
-                        }
-                    }
+                for (u32 x = 0; x < steps; x += 2) {
+                    u32 f[2][2][4];
+                    load_b(rb, x, row_a, f[0][0], f[0][1]);
+                    if (x + 1 < steps) load_b(rb, x + 1, row_a, f[1][0], f[1][1]);
+                    multiply(x, f[0][0], f[0][1], acc);
+                    if (x + 1 < steps) multiply(x + 1, f[1][0], f[1][1], acc);
+                }
             }
 #pragma unroll
             for (u32 n = 0; n < 4; n++) lora[2 * (nt0 + n) + (q4 >> 1)][(warp & 3) * 16 + g + (odd ? 8 : 0)] = digit_value(acc[n], odd, weights);
