@@ -548,7 +548,7 @@ enum { ZKB_KV_FIELD = 0,          /* canonical u32 */
 #define ZKB_KV_MAX_D_HEAD 256
 /* Pages of [num_kv_heads][page_size][d_head] elements, page i at i * page_stride elements from the base (0: dense; a larger stride lets K and
  * V pages of one pool alternate).  page_size is a power of two.  d_head up to 256, any value; rows of whole 16-byte groups whose
- * base and stride are 16-byte aligned take the fast path. */
+ * base and stride are 16-byte aligned, in pages of 8 rows or more, take the fast path. */
 typedef struct {
     void* k_pages_dev;
     void* v_pages_dev;

@@ -13,12 +13,13 @@
 // positions in a 16-bit cache), so nothing is transposed on the way.  16-bit elements are made unsigned by flipping their top bit, and
 // 2^15 (sum of the other operand) is taken off at the end.
 //
-// What bounds it is reading the cache.  Every warp has a ring of half tiles of its own, filled by tensor copies (16 rows by 128 bytes each) that
-// an mbarrier a slot counts, so warps never wait for one another within a row.  (A bulk copy a row instead of a box held the 16-bit cache to
-// 3.4 TB/s.)  The work
-// of a call is one list of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences'
-// lengths are; a row that CTAs share is added up by the one that brings its last part.  Integer sums have no order, so results do not depend on
-// the split.
+// What bounds it is reading the cache.  Every warp has a ring of half tiles of its own, filled by tensor copies (16 rows a copy) that an mbarrier a slot
+// counts, so warps never wait for one another within a row.  (A bulk copy a row instead held the 16-bit cache to 3.4 TB/s.)  The work of a call
+// is one list of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences' lengths are; a
+// row that CTAs share is added up by the one that brings its last part.  Integer sums have no order, so results do not depend on the split.
+//
+// Measured, heads of 128: 48 rows of up to 6000 positions, 8 x 4 heads, field 6.3 TB/s; one row over 131071, 8 x 4 heads, 16-bit 5.3 TB/s; 64 rows of up to
+// 5000, 8 x 8 heads, 16-bit 3.9 TB/s - there 810 instructions a tile and the registers that eight heads' sums take bound it.
 #pragma once
 #include <type_traits>
 #include "m31.cuh"
@@ -40,7 +41,9 @@ __device__ __forceinline__ u32 inv31_chain(u32 x) {
 
 // How the kernels are built for a head of up to DP elements: warps, and half tiles (16 keys or 16 values) in a warp's ring.  A half tile lies as the
 // tensor copies leave it: columns of 128 bytes, 16 rows of one behind the other, the 16-byte groups of a row swizzled by the row's low bits.
-// Which position becomes which row of an operand is free, and is chosen so that no two lanes of a phase meet in a bank.
+// Which position becomes which row of an operand is free, and is chosen so that no two lanes of a phase meet in a bank.  Warps: as many as the registers of
+// dp / 16 x nt x 4 sums a lane leave (twelve against eight with four heads of 128 in 16 bits: 103 against 110 us for 131071 positions); slots: about
+// 130 to 160 KB of them.
 template <int DP, bool SMALL, int NT>
 struct PaShape {
     static constexpr int RB = DP * (SMALL ? 2 : 4);
@@ -78,8 +81,10 @@ struct PaWalk {
         slice = 0;
         if (++kvh < A.c.num_kv_heads) return;
         kvh = 0;
-        do nb = pa_blocks(A, ++seq, block, len);
-        while (nb == 0);                       // left > 0: there is one
+        do {                                   // left > 0: there is one, unless somebody changes the lengths meanwhile
+            if (++seq >= A.num_seqs) { seq = A.num_seqs - 1; left = 0; return; }
+            nb = pa_blocks(A, seq, block, len);
+        } while (nb == 0);
     }
 };
 
@@ -188,6 +193,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
     } else {
         __shared__ u32 found_seq;
         __shared__ u64 found_rest;
+        if (tid == 0) { found_seq = 0; found_rest = 0; }
         for (u32 base = 0;; base += THREADS) {
             u32 len, nb = base + tid < A.num_seqs ? pa_blocks(A, base + tid, BLOCK, len) : 0u, x = nb;
 #pragma unroll
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
             if (nb && begin <= from && from < end) { found_seq = base + tid; found_rest = from - begin; }
             before += all;
             __syncthreads();
-            if (before * grps > from) break;
+            if (before * grps > from || base + THREADS >= A.num_seqs) break;
         }
         start_seq = found_seq;
         start_rest = found_rest;
@@ -211,6 +217,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
     cw.block = BLOCK;
     cw.slices = P.slices;
     cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
+    if (cw.nb == 0) return;                     // as above
     const u32 parts = aligned ? (cw.nb + (u32)per - 1) / (u32)per : cw.nb, start_grp = start_rest >> 32 ? (u32)(start_rest / parts) : (u32)start_rest / parts;       // of an item, in what the rest is counted in
     cw.kvh = start_grp / P.slices;
     cw.slice = start_grp - cw.kvh * P.slices;

@@ -51,10 +51,13 @@ def _fn(name):
     return f
 
 
+_MAX = 0xffffffff
+
+
 def _counts(**sizes) -> None:
-    """Every size fits the C interface's unsigned 32 bits."""
+    """Every size fits the C interface's unsigned 32 bits (the calls below look at all of them at once first)."""
     for what, v in sizes.items():
-        if not 0 <= v <= 0xffffffff:
+        if not 0 <= v <= _MAX:
             raise ValueError(f"{what}: {v} is not in [0, 2^32)")
 
 
@@ -131,6 +134,9 @@ class Rotation:
 
     def __init__(self, cos_sin, positions: int, rot_dim: int, shift: int = 14, pairs: bool = False):
         self.cos_sin, self.positions, self.rot_dim, self.shift, self.pairs = cos_sin, int(positions), int(rot_dim), int(shift), bool(pairs)
+        _counts(positions=self.positions, rot_dim=self.rot_dim, shift=self.shift)
+        self._c = _Rotation(None, self.positions, self.rot_dim, self.shift, int(self.pairs))
+        self._at = C.addressof(self._c)
 
 
 class Adapters:
@@ -138,6 +144,7 @@ class Adapters:
 
     def __init__(self, a, b, count: int, rank: int):
         self.a, self.b, self.count, self.rank = a, b, int(count), int(rank)
+        _counts(adapters=self.count, rank=self.rank)
 
 
 def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int, max_blocks: int, row_start, start, status, rotation: Rotation | None = None,
@@ -146,19 +153,24 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
     from start[s] on; position p is row p % page_size of page block_table[s][p / page_size].  With a rotation K turns by its position, and so does
     q (num_tokens, num_heads, d_head) on its way to q_out (which may be q).  Rows outside every sequence are padding and left alone."""
     ctx, t, s, blocks, heads, row = cache.ctx, num_tokens, num_seqs, max_blocks, num_heads, cache.num_kv_heads * cache.d_head
-    _counts(num_tokens=t, num_seqs=s, max_blocks=blocks, num_heads=heads)
-    if (q is None) != (q_out is None):
-        raise ValueError("q and q_out: both or neither")
-    rot = None
+    if not (0 <= t <= _MAX and 0 <= s <= _MAX and 0 <= blocks <= _MAX and 0 <= heads <= _MAX):
+        _counts(num_tokens=t, num_seqs=s, max_blocks=blocks, num_heads=heads)
+    rot = q_at = q_out_at = None
     if rotation is not None:
-        table = _addr(ctx, rotation.cos_sin, rotation.positions * rotation.rot_dim, "the rotation's table") if rotation.rot_dim else 0
-        rot = _Rotation(table, rotation.positions, rotation.rot_dim, rotation.shift, int(rotation.pairs))
-    q_row = heads * cache.d_head
-    check(ctx.h, _fn("zkb_kv_append")(
-        ctx.h, cache._at, _addr(ctx, k, _rows(t, row, k_stride), "k"), k_stride, _addr(ctx, v, _rows(t, row, v_stride), "v"), v_stride, t,
-        _addr(ctx, block_table, s * blocks, "block_table"), s, blocks, _addr(ctx, row_start, s + 1, "row_start"), _addr(ctx, start, s, "start"),
-        C.addressof(rot) if rot is not None else None, _addr(ctx, q, _rows(t, q_row, q_stride), "q") if q is not None else None, q_stride, heads,
-        _addr(ctx, q_out, _rows(t, q_row, q_out_stride), "q_out") if q is not None else None, q_out_stride, _addr(ctx, status, s, "status")))
+        rot = rotation._at
+        rotation._c.cos_sin = _addr(ctx, rotation.cos_sin, rotation.positions * rotation.rot_dim, "the rotation's table") if rotation.rot_dim else None
+    if q is not None and q_out is not None:
+        q_row = heads * cache.d_head
+        q_at = _addr(ctx, q, _rows(t, q_row, q_stride) if q_stride else t * q_row, "q")
+        q_out_at = _addr(ctx, q_out, _rows(t, q_row, q_out_stride) if q_out_stride else t * q_row, "q_out")
+    elif q is not None or q_out is not None:
+        raise ValueError("q and q_out: both or neither")
+    st = _fn("zkb_kv_append")(
+        ctx.h, cache._at, _addr(ctx, k, _rows(t, row, k_stride) if k_stride else t * row, "k"), k_stride,
+        _addr(ctx, v, _rows(t, row, v_stride) if v_stride else t * row, "v"), v_stride, t, _addr(ctx, block_table, s * blocks, "block_table"), s, blocks,
+        _addr(ctx, row_start, s + 1, "row_start"), _addr(ctx, start, s, "start"), rot, q_at, q_stride, heads, q_out_at, q_out_stride, _addr(ctx, status, s, "status"))
+    if st:
+        check(ctx.h, st)
 
 
 def paged_attention_workspace(cache: KvCache, num_seqs: int, num_heads: int) -> int:
@@ -174,11 +186,15 @@ def paged_attention(cache: KvCache, q, block_table, num_seqs: int, max_blocks: i
     The score q . k_j, divided by 2^score_shift and rounded half away from zero, must be an input of the exp table; a sequence of length 0 and a
     row that is refused (status) give zeros."""
     ctx, s, blocks, heads, row = cache.ctx, num_seqs, max_blocks, num_heads, num_heads * cache.d_head
-    _counts(num_seqs=s, max_blocks=blocks, num_heads=heads, score_shift=score_shift)
-    check(ctx.h, _fn("zkb_paged_attention")(
-        ctx.h, cache._at, _addr(ctx, q, _rows(s, row, q_stride), "q"), q_stride, heads, _addr(ctx, block_table, s * blocks, "block_table"), s, blocks,
+    if not (0 <= s <= _MAX and 0 <= blocks <= _MAX and 0 <= heads <= _MAX and 0 <= score_shift <= _MAX):
+        _counts(num_seqs=s, max_blocks=blocks, num_heads=heads, score_shift=score_shift)
+    at, size = _workspace(ctx, workspace) if workspace is not None else (None, 0)
+    st = _fn("zkb_paged_attention")(
+        ctx.h, cache._at, _addr(ctx, q, _rows(s, row, q_stride) if q_stride else s * row, "q"), q_stride, heads, _addr(ctx, block_table, s * blocks, "block_table"), s, blocks,
         _addr(ctx, lens, s, "lens"), _addr(ctx, exp_table, n_table, "exp_table"), n_table, score_shift, _addr(ctx, out, s * row, "out"),
-        _addr(ctx, status, s, "status"), *_workspace(ctx, workspace)))
+        _addr(ctx, status, s, "status"), at, size)
+    if st:
+        check(ctx.h, st)
 
 
 def adapter_linear_workspace(ctx: Context, tokens: int, m: int, n: int, num_adapters: int = 0, rank: int = 0) -> int:
@@ -190,23 +206,25 @@ def adapter_linear_workspace(ctx: Context, tokens: int, m: int, n: int, num_adap
 def adapter_linear(ctx: Context, x, w, tokens: int, m: int, n: int, out, bias=None, adapters: Adapters | None = None, adapter_of=None, x_stride: int = 0,
                    out_stride: int = 0, workspace=None) -> None:
     """out[t] = W x[t] + bias + B[a] (A[a] x[t]), a = adapter_of[t] (outside the adapters: none), for `tokens` rows x of n words; W is m x n, row-major."""
-    _counts(tokens=tokens, m=m, n=n)
+    if not (0 <= tokens <= _MAX and 0 <= m <= _MAX and 0 <= n <= _MAX):
+        _counts(tokens=tokens, m=m, n=n)
     if (adapters is None) != (adapter_of is None):
         raise ValueError("adapters and adapter_of: both or neither")
+    at, size = _workspace(ctx, workspace) if workspace is not None else (None, 0)
     a = b = of = None
     count = rank = 0
     if adapters is not None:
         count, rank = adapters.count, adapters.rank
-        _counts(adapters=count, rank=rank)
         a, b, of = _addr(ctx, adapters.a, count * rank * n, "A"), _addr(ctx, adapters.b, count * m * rank, "B"), _addr(ctx, adapter_of, tokens, "adapter_of")
-    check(ctx.h, _fn("zkb_adapter_linear")(
-        ctx.h, _addr(ctx, x, _rows(tokens, n, x_stride), "x"), x_stride, _addr(ctx, w, m * n, "w"), _addr(ctx, bias, m, "bias") if bias is not None else None, tokens, m,
-        n, a, b, count, rank, of, _addr(ctx, out, _rows(tokens, m, out_stride), "out"), out_stride, *_workspace(ctx, workspace)))
+    st = _fn("zkb_adapter_linear")(
+        ctx.h, _addr(ctx, x, _rows(tokens, n, x_stride) if x_stride else tokens * n, "x"), x_stride, _addr(ctx, w, m * n, "w"),
+        _addr(ctx, bias, m, "bias") if bias is not None else None, tokens, m, n, a, b, count, rank, of,
+        _addr(ctx, out, _rows(tokens, m, out_stride) if out_stride else tokens * m, "out"), out_stride, at, size)
+    if st:
+        check(ctx.h, st)
 
 
 def _workspace(ctx, w):
-    if w is None:
-        return None, 0
     size = 4 if isinstance(w, DeviceBuffer) else w.element_size()
     at = _addr(ctx, w, 0, "workspace", size)
     return at, (4 * w.n if isinstance(w, DeviceBuffer) else w.numel() * size)
