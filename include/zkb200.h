@@ -579,6 +579,7 @@ int32_t zkb_kv_append(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint32_t* k
  * (0: dense), query head h reads key head h / (num_heads / num_kv_heads).  s_j = q . k_j as a centred integer, divided by 2^score_shift and
  * rounded half away from zero, must be an input of the exp table (65536 or 256 entries, as for zkb_row_attention_forward);
  * out[s][h] = (sum_j e_j v_j) / (sum_j e_j), e_j = table(s_j).  A row of length 0 is zero, and so is a row that is refused (status).
+ * out overlaps no input.
  * workspace: zkb_paged_attention_workspace bytes of the caller's, 256-byte aligned, for this call alone until it has run.  It is zeroed once before
  * the first call that gets it and belongs to this operator from then on: every call finds its counters zero and leaves them so.  NULL: the context's scratch, which a captured
  * call must not use (ZKB_E_ARG). */
@@ -588,7 +589,7 @@ int32_t zkb_paged_attention(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint3
                             uint32_t* out_dev, int32_t* status_dev, void* workspace_dev, size_t workspace_bytes);
 /* y[t] = W x[t] + bias + B[a] (A[a] x[t]), a = adapter_of[t]; a token whose entry is outside [0, num_adapters) has no adapter.  x: tokens rows of n
  * words, x_stride apart; W: m x n row-major; bias (m words) may be NULL; A: (num_adapters, rank, n), B: (num_adapters, m, rank); y: tokens rows of
- * m words, y_stride apart.  An adapter's scale is part of B.  The workspace as above, but with any contents. */
+ * m words, y_stride apart.  An adapter's scale is part of B.  No word of y is one of x or of another input.  The workspace as above, but with any contents. */
 size_t zkb_adapter_linear_workspace(zkb_ctx* ctx, uint32_t tokens, uint32_t m, uint32_t n, uint32_t num_adapters, uint32_t rank);
 int32_t zkb_adapter_linear(zkb_ctx* ctx, const uint32_t* x_dev, size_t x_stride, const uint32_t* w_dev, const uint32_t* bias_dev, uint32_t tokens, uint32_t m, uint32_t n,
                            const uint32_t* a_dev, const uint32_t* b_dev, uint32_t num_adapters, uint32_t rank, const int32_t* adapter_of_dev, uint32_t* y_dev,

@@ -433,6 +433,21 @@ def test_linear_matrix_on_no_16_byte_boundary(ctx):
         assert np.array_equal(out.download().reshape(t, 96), R.linear(x, w))
 
 
+@pytest.mark.parametrize("t,n,m", [(1, 128, 96), (5, 127, 95), (70, 256, 130), (2100, 64, 36)])
+def test_linear_rows_of_x_and_of_the_result_in_one_array(ctx, t, n, m):
+    """The result's words lie between the rows of x: neither is read or written as the other."""
+    rng = np.random.default_rng(t)
+    x, w, a, b, of = field(rng, t, n), field(rng, m, n), field(rng, 2, 3, n), field(rng, 2, m, 3), rng.integers(-1, 2, t)
+    both = np.full((t, n + m), 0x5a5a5a5a, np.uint32)
+    both[:, :n] = x
+    raw = ctx.upload(both)
+    zs.adapter_linear(ctx, raw, ctx.upload(w), t, m, n, zk.DeviceBuffer.wrap(ctx, buf_address(raw) + 4 * n, raw.n - n), adapters=zs.Adapters(ctx.upload(a), ctx.upload(b), 2, 3),
+                      adapter_of=ctx.upload(words(of.astype(np.int32))), x_stride=n + m, out_stride=n + m)
+    got = raw.download().reshape(t, n + m)
+    assert np.array_equal(got[:, :n], x)
+    assert np.array_equal(got[:, n:], R.linear(x, w, None, a, b, of))
+
+
 def test_linear_is_the_product_with_the_merged_matrix(ctx):
     """One row equals the framework's matrix-vector product, and an adapter the matrix W + B A, whose product the framework proves."""
     rng = np.random.default_rng(5)
@@ -476,6 +491,17 @@ def test_refused_arguments(ctx):
                    dict(adapters=zs.Adapters(z(16), z(8), 1, 1), adapter_of=z(1))):
         with pytest.raises((zk.ZkbError, ValueError)):
             zs.adapter_linear(ctx, **{**ok, **change})
+    assert ctx.launches == before
+
+
+def test_results_in_place_of_their_inputs_are_refused(ctx):
+    z = lambda n: ctx.upload(np.zeros(n, np.uint32))
+    cache, rows = zs.KvCache(ctx, 8, 2, 16, 4, False), z(64)
+    before = ctx.launches
+    with pytest.raises(zk.ZkbError, match="out is not q"):
+        zs.paged_attention(cache, rows, z(2), 1, 2, z(1), 4, z(65536), rows, z(1))
+    with pytest.raises(zk.ZkbError, match="y is not x"):
+        zs.adapter_linear(ctx, rows, z(256), 4, 16, 16, rows)
     assert ctx.launches == before
 
 

@@ -68,3 +68,15 @@ def test_both_or_neither():
         zs.kv_append(cache, Array(64), Array(64), 2, Array(2), 1, 2, Array(2), Array(1), Array(1), q=Array(64), num_heads=2)
     with pytest.raises(ValueError, match="adapters"):
         zs.adapter_linear(ctx, Array(32), Array(128), 2, 8, 16, Array(16), adapter_of=Array(2))
+
+
+def test_rotation_is_checked_at_the_size_that_is_sent():
+    ctx = Device()
+    cache = zs.KvCache(ctx, 8, 2, 16, 4, False, Array(4 * 256), Array(4 * 256))
+    rot = zs.Rotation(Array(8 * 16 - 1), 8, 16)
+    rot.positions = 1                          # the library's own copy still says 8
+    with pytest.raises(ValueError, match="rotation's table"):
+        zs.kv_append(cache, Array(64), Array(64), 2, Array(2), 1, 2, Array(2), Array(1), Array(1), rotation=rot)
+    for bad in ((-1, 16), (8, -2), (8, 16, 1 << 32)):
+        with pytest.raises(ValueError):
+            zs.Rotation(Array(8), *bad)

@@ -139,6 +139,7 @@ int32_t zkb_paged_attention(zkb_ctx* c, const zkb_kv_cache* cache, const uint32_
         if ((double)num_seqs * max_blocks * cache->page_size * num_heads >= (double)(1ull << 42)) throw ArgFail{ZKB_E_TOO_LARGE, "paged_attention: more than 2^42 scores"};
         need_words(q_dev, "q"); need_words(block_table_dev, "block_table"); need_words(lens_dev, "lens"); need_words(table_out_dev, "the exp table");
         need_words(out_dev, "out"); need_words(status_dev, "status");
+        if (out_dev == q_dev) throw ArgFail{ZKB_E_ARG, "paged_attention: out is not q"};
         a.q = q_dev; a.num_heads = num_heads; a.num_seqs = num_seqs; a.max_blocks = max_blocks;
         a.block_table = block_table_dev; a.lens = lens_dev; a.table = table_out_dev; a.n_table = (u32)n_table; a.score_shift = score_shift;
         a.out = out_dev; a.status = status_dev;
@@ -179,6 +180,7 @@ int32_t zkb_adapter_linear(zkb_ctx* c, const uint32_t* x_dev, size_t x_stride, c
         if (!tokens) return ZKB_OK;
         need_words(x_dev, "x"); need_words(w_dev, "w"); need_words(y_dev, "y");
         if (bias_dev) need_words(bias_dev, "bias");
+        if (y_dev == x_dev) throw ArgFail{ZKB_E_ARG, "adapter_linear: y is not x"};
         if (num_adapters) { need_words(a_dev, "the adapters' A"); need_words(b_dev, "the adapters' B"); need_words(adapter_of_dev, "adapter_of"); }
         a.x = x_dev; a.w = w_dev; a.bias = bias_dev; a.tokens = tokens; a.m = m; a.n = n; a.a = a_dev; a.b = b_dev;
         a.num_adapters = num_adapters; a.rank = num_adapters ? rank : 0; a.adapter_of = adapter_of_dev; a.y = y_dev;

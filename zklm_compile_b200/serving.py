@@ -136,6 +136,7 @@ class Rotation:
         self.cos_sin, self.positions, self.rot_dim, self.shift, self.pairs = cos_sin, int(positions), int(rot_dim), int(shift), bool(pairs)
         _counts(positions=self.positions, rot_dim=self.rot_dim, shift=self.shift)
         self._c = _Rotation(None, self.positions, self.rot_dim, self.shift, int(self.pairs))
+        self._words = self.positions * self.rot_dim
         self._at = C.addressof(self._c)
 
 
@@ -158,7 +159,7 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
     rot = q_at = q_out_at = None
     if rotation is not None:
         rot = rotation._at
-        rotation._c.cos_sin = _addr(ctx, rotation.cos_sin, rotation.positions * rotation.rot_dim, "the rotation's table") if rotation.rot_dim else None
+        rotation._c.cos_sin = _addr(ctx, rotation.cos_sin, rotation._words, "the rotation's table") if rotation._c.rot_dim else None
     if q is not None and q_out is not None:
         q_row = heads * cache.d_head
         q_at = _addr(ctx, q, _rows(t, q_row, q_stride) if q_stride else t * q_row, "q")
@@ -184,7 +185,7 @@ def paged_attention(cache: KvCache, q, block_table, num_seqs: int, max_blocks: i
                     q_stride: int = 0, workspace=None, n_table: int = 65536) -> None:
     """One new token per sequence: q (num_seqs, num_heads, d_head) over the first lens[s] positions of the cache, into out (num_seqs, num_heads, d_head).
     The score q . k_j, divided by 2^score_shift and rounded half away from zero, must be an input of the exp table; a sequence of length 0 and a
-    row that is refused (status) give zeros."""
+    row that is refused (status) give zeros.  `out` overlaps no input."""
     ctx, s, blocks, heads, row = cache.ctx, num_seqs, max_blocks, num_heads, num_heads * cache.d_head
     if not (0 <= s <= _MAX and 0 <= blocks <= _MAX and 0 <= heads <= _MAX and 0 <= score_shift <= _MAX):
         _counts(num_seqs=s, max_blocks=blocks, num_heads=heads, score_shift=score_shift)
@@ -205,7 +206,8 @@ def adapter_linear_workspace(ctx: Context, tokens: int, m: int, n: int, num_adap
 
 def adapter_linear(ctx: Context, x, w, tokens: int, m: int, n: int, out, bias=None, adapters: Adapters | None = None, adapter_of=None, x_stride: int = 0,
                    out_stride: int = 0, workspace=None) -> None:
-    """out[t] = W x[t] + bias + B[a] (A[a] x[t]), a = adapter_of[t] (outside the adapters: none), for `tokens` rows x of n words; W is m x n, row-major."""
+    """out[t] = W x[t] + bias + B[a] (A[a] x[t]), a = adapter_of[t] (outside the adapters: none), for `tokens` rows x of n words; W is m x n, row-major.
+    `out` overlaps no input; rows of x and of out may alternate in one array."""
     if not (0 <= tokens <= _MAX and 0 <= m <= _MAX and 0 <= n <= _MAX):
         _counts(tokens=tokens, m=m, n=n)
     if (adapters is None) != (adapter_of is None):
