@@ -38,7 +38,7 @@ enum {
     ZKB_E_NOT_QR = 5,       /* "compute_r: d/sum_sq is not a quadratic residue" (transformer/mod.rs:182) */
     ZKB_E_LENGTH = 6,       /* a length assertion of the reference failed (matmul.rs:161, 861) */
     ZKB_E_TOO_LARGE = 7,    /* request exceeds a documented fixed capacity */
-    ZKB_E_TIMEOUT = 8,      /* a peer GPU of a split sumcheck did not answer within the exchange's time limit, or a wait inside a kernel ran out (zkb_ctx_sync) */
+    ZKB_E_TIMEOUT = 8,      /* a peer GPU of a split sumcheck did not answer within the exchange's time limit, or a call of the token-by-token operators gave up (zkb_ctx_sync) */
     ZKB_E_DIV_ZERO = 9      /* batch_inverse met a zero element: p3's `.inverse()` panics there (lookup.rs:336, 358) */
 };
 
@@ -65,8 +65,8 @@ enum {
 int32_t zkb_ctx_create(int32_t device, zkb_ctx** out);
 void zkb_ctx_destroy(zkb_ctx* ctx);
 const char* zkb_last_error(const zkb_ctx* ctx);
-/* Waits for the context's stream.  ZKB_E_TIMEOUT: a bounded wait inside a kernel of the token-by-token operators ran out (which no input causes), and what the
- * context computed since its last synchronisation is not valid. */
+/* Waits for the context's stream.  ZKB_E_TIMEOUT: a bounded wait inside a kernel of the token-by-token operators ran out (which no input causes), or the lengths
+ * of an attention call changed while it ran; what the context computed since its last synchronisation is not valid. */
 int32_t zkb_ctx_sync(zkb_ctx* ctx);
 /* A context keeps a scratch arena on the device that grows to what its largest proof needed and is
  * reused from then on (nothing is allocated per proof).  zkb_ctx_scratch_bytes reports its size;
@@ -536,7 +536,8 @@ int32_t zkb_oplist_prove(zkb_oplist* list, const uint32_t* x, uint8_t* out, size
  * elements and the centred integers they stand for, so a row computed over the cache is the row that zkb_row_attention(_gqa)_forward
  * computes and zkb_prove_row_attention(_gqa) proves, and a projection with an adapter is the product with the merged matrix W + B A.
  * All pointers are device memory of the context's GPU; calls are enqueued on the context's stream and nothing is waited for, so
- * they can be captured into a graph from that stream (after a first call outside, which loads the kernels).  What only the device sees goes into the caller's status words, one per sequence:
+ * they can be captured into a graph from that stream (after a first call outside, which loads the kernels).  What a call reads - tables, lengths and adapters' numbers
+ * included - stays as it is until the call has run.  What only the device sees goes into the caller's status words, one per sequence:
  * status[s] becomes the largest code that a call found, and stays until the caller clears it. */
 enum { ZKB_SERVE_PAGE = 1,        /* a length or position outside the block table, or a page number outside the pool */
        ZKB_SERVE_ROTATION = 2,    /* a position that the rotation's table does not have */
@@ -581,7 +582,8 @@ int32_t zkb_kv_append(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint32_t* k
  * out[s][h] = (sum_j e_j v_j) / (sum_j e_j), e_j = table(s_j).  A row of length 0 is zero, and so is a row that is refused (status).
  * out overlaps no input.
  * workspace: zkb_paged_attention_workspace bytes of the caller's, 256-byte aligned, for this call alone until it has run.  It is zeroed once before
- * the first call that gets it and belongs to this operator from then on: every call finds its counters zero and leaves them so.  NULL: the context's scratch, which a captured
+ * the first call that gets it and belongs to this operator from then on: every call finds its counters zero and leaves them so (after
+ * ZKB_E_TIMEOUT zero it again; a call that finds counters left over by lengths that changed reports it).  NULL: the context's scratch, which a captured
  * call must not use (ZKB_E_ARG). */
 size_t zkb_paged_attention_workspace(zkb_ctx* ctx, const zkb_kv_cache* cache, uint32_t num_seqs, uint32_t num_heads);
 int32_t zkb_paged_attention(zkb_ctx* ctx, const zkb_kv_cache* cache, const uint32_t* q_dev, size_t q_stride, uint32_t num_heads, const int32_t* block_table_dev,

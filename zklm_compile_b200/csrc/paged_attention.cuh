@@ -56,6 +56,7 @@ struct PaWork {                                // see paged_attention_launch
     u32 slices, slice_heads, ctas;
     u32* slots;                                // [ctas][2][slice_heads][DP + 4]: sums, then the sum of weights and what went wrong
     u32* arrived;                              // [ctas], zero before and after a call: how many parts are there of the row that begins in this CTA
+    u32* begun;                                // zero before and after a call: see pa_began
     int fast;                                  // tensor copies: rows are whole 16-byte groups on 16-byte boundaries, pages have 8 rows or more
     int q_vec;                                 // q is read 16 bytes at a time
     int whole;                                 // a box has all the columns of its rows
@@ -63,30 +64,69 @@ struct PaWork {                                // see paged_attention_launch
 };
 enum : u32 { PA_BAD_PAGE = 1, PA_BAD_SCORE = 2 };
 
-// Blocks of a sequence: 0 for one without positions and one whose length the block table cannot have.
-__device__ __forceinline__ u32 pa_blocks(const PagedAttnArgs& A, u32 seq, u32 block, u32& len) {
-    const int l = A.lens[seq];
-    len = l < 0 || (u64)l > ((u64)A.max_blocks << A.c.page_bits) ? 0u : (u32)l;
+// How the blocks are shared is worked out by every CTA for itself from the lengths.  They are inputs, which nobody changes before the call has run; but
+// should somebody, no address and no barrier may depend on its luck.  So all threads of a CTA compute by what one of them read, and a share is found in the
+// lengths that it was counted by (up to PA_FEW sequences) or cut to what the arrays have.  The copies of a warp go by what the warp itself read, in bounds
+// whatever it was.  What then becomes of the rows is nothing of use: a CTA that finds blocks missing or left over sets the give-up flag, and so does the
+// next call if parts of a row are left in the counters, which it would add to.
+constexpr u32 PA_FEW = 256;
+
+// The blocks of a length: 0 for a sequence without positions and one whose length the block table cannot have.
+ZKB_HD u32 pa_blocks(u64 positions, int l, u32 block, u32& len) {
+    len = l < 0 || (u64)l > positions ? 0u : (u32)l;
     return (len + block - 1) / block;
 }
 // The stream of blocks that a CTA takes: sequences, in each its (key head, slice) items, in each its blocks.
 struct PaWalk {
-    u32 seq, kvh, slice, blk, nb, len, block, slices, left;
-    __device__ __forceinline__ void step(const PagedAttnArgs& A, u32 n) {
+    u32 seq, kvh, slice, blk, nb, len, left;
+    // Block `rest` (in shares of `per` where `aligned`) of sequence `at`, which has nb of them an item; rest < its items x its blocks.
+    ZKB_HD void start(u32 at, u64 rest, u64 count, bool aligned, u32 per, u32 slices) {
+        seq = at;
+        const u32 parts = aligned ? (nb + per - 1) / per : nb, grp = rest >> 32 ? (u32)(rest / parts) : (u32)rest / parts;      // of an item, in what the rest is counted in
+        kvh = grp / slices;
+        slice = grp - kvh * slices;
+        blk = (u32)(rest - (u64)grp * parts) * (aligned ? per : 1u);
+        left = !aligned ? (u32)count : nb - blk < per ? nb - blk : per;
+    }
+    // n blocks on, within an item or to its end; true: what comes next is another sequence (next_seq).
+    ZKB_HD bool step(u32 n, u32 slices, u32 kv_heads) {
         left -= n;
         blk += n;
-        if (blk < nb || !left) return;
+        if (blk < nb || !left) return false;
         blk = 0;
-        if (++slice < slices) return;
+        if (++slice < slices) return false;
         slice = 0;
-        if (++kvh < A.c.num_kv_heads) return;
+        if (++kvh < kv_heads) return false;
         kvh = 0;
-        do {                                   // left > 0: there is one, unless somebody changes the lengths meanwhile
-            if (++seq >= A.num_seqs) { seq = A.num_seqs - 1; left = 0; return; }
-            nb = pa_blocks(A, seq, block, len);
+        return true;
+    }
+    // The next sequence that has blocks.  There is one while blocks are left; if not (see above) none is.
+    template <class Length>
+    ZKB_HD void next_seq(u32 num_seqs, u64 positions, u32 block, const Length& length) {
+        do {
+            if (++seq >= num_seqs) { seq = num_seqs - 1; nb = len = left = 0; return; }
+            nb = pa_blocks(positions, length(seq), block, len);
         } while (nb == 0);
     }
 };
+// The CTAs that have a part of a row of nb blocks, from the first on; `at`: where in the list of blocks the row's block `first` lies, which CTA `cta` has.
+// (A row that was not counted with these blocks may seem to begin before the list or to end behind it.)
+struct PaParts { u32 first_cta, n; };
+ZKB_HD PaParts pa_parts(bool aligned, u64 per, u32 ctas, u32 cta, u64 at, u32 first, u32 nb) {
+    const u64 row0 = at - (first < at ? first : at);
+    PaParts p;
+    p.first_cta = aligned ? cta - first / (u32)per : (u32)(row0 / per);
+    p.n = aligned ? (nb + (u32)per - 1) / (u32)per : (u32)((row0 + nb - 1) / per) - p.first_cta + 1;
+    p.n = umin32(p.n, ctas - p.first_cta);
+    return p;
+}
+// What is left in the counters of a row's parts is known from one more word: its high half has the parts that were brought less those that were added up, its low
+// half the CTAs that began, the first of them as 1 - ctas, so that it is zero before a call, at its end, and in between not for a CTA that has not added itself.
+// That CTA sees whether the call began with counters at zero; nothing is waited for.  (A word for the last CTA to clear, which has to wait for its own atomic:
+// 0.4 us more in a call of 7, 0.9 in one of 19.)
+ZKB_HD u32 pa_began(u32 cta, u32 ctas) { return cta ? 1u : 1u - ctas; }
+ZKB_HD u32 pa_brought(u32 parts, u32 added) { return (parts - added) << 16; }
+ZKB_HD bool pa_stale(u32 word) { return word != 0 && (word & 0xffffu) == 0; }
 
 // One output row (or its part) in shared memory to where it belongs.
 __device__ __forceinline__ void pa_finish(const PagedAttnArgs& A, u32 seq, u32 head, u32 e, u32 acc, u32 inv, u32 correction) {
@@ -106,27 +146,40 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
     unsigned char* digits = reinterpret_cast<unsigned char*>(part + WARPS * HEADS * DP);   // [WARPS][NT][ED]
     __shared__ u32 es_part[WARPS][HEADS], flag_part[WARPS][HEADS];                 // sums of e, and what went wrong
     __shared__ u32 off_q[HEADS], corr[HEADS], inv[HEADS], scan[32];
+    __shared__ int few_lens[PA_FEW];
+    __shared__ u32 found_seq, found_len;
+    __shared__ u64 found_rest;
+    __shared__ struct { PaWalk walk; u64 per, to; bool aligned; } share;           // as thread 0 has it
     __shared__ __align__(8) u64 bars[WARPS * NS];
     __shared__ volatile int gave_up;
     __shared__ int last_part;
     const u32 tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
     const u32 grps = A.c.num_kv_heads * P.slices, hpg = A.num_heads / A.c.num_kv_heads, d = A.c.d;
+    u32 begun = 0;
     if (tid == 0) {
         gave_up = 0;
         if (P.fast) { prefetch_tensor_map(&map_k); prefetch_tensor_map(&map_v); }
+        begun = __ldcg(P.begun);
+        atomicAdd(P.begun, pa_began(blockIdx.x, P.ctas));
     }
 
     // ---- this CTA's share of the blocks ---------------------------------------------------------
     // up to 256 sequences by every warp for itself, more by the CTA
-    constexpr int K = 8;
+    constexpr int K = PA_FEW / 32;
+    const u64 positions = (u64)A.max_blocks << A.c.page_bits;
     u64 total = 0;
-    u32 own_nb[K];
-    const bool few = A.num_seqs <= 32 * K;
+    u32 own_nb[K], own_len[K];
+    const bool few = A.num_seqs <= PA_FEW;
     if (few) {
 #pragma unroll
-        for (int k = 0; k < K; k++) { u32 len; own_nb[k] = 32 * k + lane < A.num_seqs ? pa_blocks(A, 32 * k + lane, BLOCK, len) : 0u; total += own_nb[k]; }
+        for (int k = 0; k < K; k++) {
+            own_nb[k] = own_len[k] = 0;
+            if (32 * k + lane < A.num_seqs) own_nb[k] = pa_blocks(positions, A.lens[32 * k + lane], BLOCK, own_len[k]);
+            if (warp == 0) few_lens[32 * k + lane] = own_len[k];      // for the others from the first barrier on
+            total += own_nb[k];
+        }
     } else {
-        for (u32 s = tid; s < A.num_seqs; s += THREADS) { u32 len; total += pa_blocks(A, s, BLOCK, len); }
+        for (u32 s = tid; s < A.num_seqs; s += THREADS) { u32 len; total += pa_blocks(positions, A.lens[s], BLOCK, len); }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -168,14 +221,16 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
     // rows without positions are zero
     for (u32 s = blockIdx.x; s < A.num_seqs; s += P.ctas) {
         u32 len;
-        if (pa_blocks(A, s, BLOCK, len)) continue;
+        const int l = A.lens[s];
+        if (pa_blocks(positions, l, BLOCK, len)) continue;
         for (u32 i = tid; i < A.num_heads * d; i += THREADS) A.out[(size_t)s * A.num_heads * d + i] = 0;
-        if (tid == 0 && A.lens[s] != 0) atomicMax(A.status + s, (int)SERVE_PAGE);
+        if (tid == 0 && l != 0) atomicMax(A.status + s, (int)SERVE_PAGE);
     }
-    if (from >= to) return;
-    u32 start_seq = 0;                         // the sequence in which block `from` lies, and the blocks of it that lie before
+    u32 start_seq = 0, start_len = 0;          // the sequence in which block `from` lies, and the blocks of it that lie before
     u64 start_rest = 0, before = 0;
-    if (few) {
+    if (from >= to) {
+        // nothing for this CTA
+    } else if (few) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
             if (32u * k >= A.num_seqs) break;
@@ -187,15 +242,14 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
             if (here) {
                 start_seq = 32 * k + __ffs(here) - 1;
                 start_rest = from - __shfl_sync(0xffffffffu, begin, __ffs(here) - 1);
+                start_len = __shfl_sync(0xffffffffu, own_len[k], __ffs(here) - 1);
             }
             before += __shfl_sync(0xffffffffu, x, 31);
         }
     } else {
-        __shared__ u32 found_seq;
-        __shared__ u64 found_rest;
-        if (tid == 0) { found_seq = 0; found_rest = 0; }
+        if (tid == 0) { found_seq = found_len = 0; found_rest = 0; }
         for (u32 base = 0;; base += THREADS) {
-            u32 len, nb = base + tid < A.num_seqs ? pa_blocks(A, base + tid, BLOCK, len) : 0u, x = nb;
+            u32 len = 0, nb = base + tid < A.num_seqs ? pa_blocks(positions, A.lens[base + tid], BLOCK, len) : 0u, x = nb;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const u32 y = __shfl_up_sync(0xffffffffu, x, o); if ((int)lane >= o) x += y; }
             if (lane == 31) scan[warp] = x;
@@ -204,25 +258,20 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
 #pragma unroll
             for (int i = 0; i < WARPS; i++) { if (i < (int)warp) w += scan[i]; all += scan[i]; }
             const u64 end = (before + w + x) * grps, begin = end - (u64)nb * grps;
-            if (nb && begin <= from && from < end) { found_seq = base + tid; found_rest = from - begin; }
+            if (nb && begin <= from && from < end) { found_seq = base + tid; found_len = len; found_rest = from - begin; }
             before += all;
             __syncthreads();
             if (before * grps > from || base + THREADS >= A.num_seqs) break;
         }
         start_seq = found_seq;
+        start_len = found_len;
         start_rest = found_rest;
     }
     PaWalk cw{};
-    cw.seq = start_seq;
-    cw.block = BLOCK;
-    cw.slices = P.slices;
-    cw.nb = pa_blocks(A, cw.seq, BLOCK, cw.len);
-    if (cw.nb == 0) return;                     // as above
-    const u32 parts = aligned ? (cw.nb + (u32)per - 1) / (u32)per : cw.nb, start_grp = start_rest >> 32 ? (u32)(start_rest / parts) : (u32)start_rest / parts;       // of an item, in what the rest is counted in
-    cw.kvh = start_grp / P.slices;
-    cw.slice = start_grp - cw.kvh * P.slices;
-    cw.blk = (u32)(start_rest - (u64)start_grp * parts) * (aligned ? (u32)per : 1u);
-    cw.left = !aligned ? (u32)(to - from) : cw.nb - cw.blk < per ? cw.nb - cw.blk : (u32)per;
+    cw.nb = pa_blocks(positions, (int)start_len, BLOCK, cw.len);
+    if (cw.nb) cw.start(start_seq, start_rest, to - from, aligned, (u32)per, P.slices);
+    if (pa_stale(begun) || (from < to && !cw.nb)) *P.gave_up = 1;       // see above
+    if (tid == 0) { share.walk = cw; share.per = per; share.to = to; share.aligned = aligned; }
     PaWalk lw = cw;                            // the copies run ahead of the computation
 
     // ---- copies -------------------------------------------------------------------------------------
@@ -292,7 +341,13 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         }
-        if (is_v) { lw.step(A, 1); fetch_page(); }
+        if (is_v) {
+            if (lw.step(1, P.slices, A.c.num_kv_heads)) {
+                lw.next_seq(A.num_seqs, (u64)A.max_blocks << A.c.page_bits, BLOCK, [&](u32 s) { return __shfl_sync(0xffffffffu, A.lens[s], 0); });
+                if (!lw.left) gave_up = 1;     // blocks are missing: nobody waits for them
+            }
+            fetch_page();
+        }
         slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
     };
     // A thread's elements of q for a row: four words' places of one head for each of its items, fetched ahead of their use.
@@ -319,7 +374,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
     auto heads_of = [&](const PaWalk& w) { const u32 rest = hpg - w.slice * P.slice_heads; return rest < P.slice_heads ? rest : P.slice_heads; };
     auto head0_of = [&](const PaWalk& w) { return w.kvh * hpg + w.slice * P.slice_heads; };
     fetch_page();
-    fetch_q(cw.seq, head0_of(cw), heads_of(cw));
+    if (cw.left) fetch_q(cw.seq, head0_of(cw), heads_of(cw));
 #pragma unroll
     for (int h = 0; h < NS; h++) load_half(h & 1);
 
@@ -329,15 +384,17 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
     const bool odd = q4 & 1;
     const DigitWeights weights = odd ? DigitWeights{1u << 16, 1u << 24, 1u, 1u << 8} : DigitWeights{1u, 1u << 8, 1u << 16, 1u << 24};
     u32 slot_out = 0, phase = 0;
-    auto wait_half = [&] { mbar_wait(bar0 + 8 * slot_out, phase, &gave_up); };
+    auto wait_half = [&] { if (!mbar_test(bar0 + 8 * slot_out, phase) && !gave_up) mbar_wait(bar0 + 8 * slot_out, phase, &gave_up); };     // no time for more of them once one ran out
     auto next_slot = [&] { if (++slot_out == NS) { slot_out = 0; phase ^= 1; } };
 
     // ---- the stretches of items ---------------------------------------------------------------------
     u32 computed = 0;
+    __syncthreads();
+    if (cw.left != share.walk.left || (cw.left && !lw.nb)) gave_up = 1;       // copies that nobody waits for, or none where they are waited for
+    cw = share.walk;
     while (cw.left) {
         const u32 seq = cw.seq, head0 = head0_of(cw), heads = heads_of(cw);
         const u32 first = cw.blk, len = cw.len, nb = cw.nb, count = cw.left < nb - first ? cw.left : nb - first;
-        __syncthreads();                        // the row before is done with these arrays
         // The right operand of the scores: a thread takes four words' places of one head, whose digits are four lanes' 16 bytes for steps 2j and 2j + 1.
 #pragma unroll
         for (int it = 0; it < Q_ITEMS; it++) {
@@ -558,14 +615,15 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
         }
         if (!(begins && ends)) {
             // The CTA that brings a row's last part adds the parts up.  They lie in the slot of the CTA in which the row begins and those of the next ones.
-            const u64 at = to - cw.left, row0 = at - first;
-            const u32 c0 = aligned ? blockIdx.x - first / (u32)per : (u32)(row0 / per), n = aligned ? (nb + (u32)per - 1) / (u32)per : (u32)((row0 + nb - 1) / per) - c0 + 1;
+            const PaParts parts = pa_parts(share.aligned, share.per, P.ctas, blockIdx.x, share.to - cw.left, first, nb);
+            const u32 c0 = parts.first_cta, n = parts.n;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
-                const u32 before = atomicAdd(P.arrived + c0, 1u);
-                last_part = before == n - 1;
-                if (last_part) P.arrived[c0] = 0;
+                const bool all = atomicAdd(P.arrived + c0, 1u) == n - 1;
+                last_part = all;
+                if (all) atomicSub(P.arrived + c0, n);
+                atomicAdd(P.begun, pa_brought(1, all ? n : 0));
             }
             __syncthreads();
             if (last_part) {
@@ -611,8 +669,23 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
                 }
             }
         }
-        cw.step(A, count);
-        if (cw.left) fetch_q(cw.seq, head0_of(cw), heads_of(cw));
+        if (cw.step(count, P.slices, A.c.num_kv_heads)) {
+            if (few) {
+                cw.next_seq(A.num_seqs, (u64)A.max_blocks << A.c.page_bits, BLOCK, [&](u32 s) { return few_lens[s]; });
+            } else {                            // by one thread for all
+                if (tid == 0) {
+                    cw.next_seq(A.num_seqs, (u64)A.max_blocks << A.c.page_bits, BLOCK, [&](u32 s) { return A.lens[s]; });
+                    share.walk = cw;
+                }
+                __syncthreads();
+                cw = share.walk;
+            }
+            if (!cw.left) gave_up = 1;          // blocks are missing
+        }
+        if (cw.left) {
+            fetch_q(cw.seq, head0_of(cw), heads_of(cw));
+            __syncthreads();                    // all are done with this row's arrays
+        }
     }
     if (gave_up) {                              // nothing of this warp may still be in flight when it ends
         for (u32 h = 0; h < NS; h++) {

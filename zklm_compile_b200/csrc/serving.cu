@@ -48,7 +48,7 @@ static cudaError_t rows_tensor_map(CUtensorMap* map, const u32* w, u32 rows, u32
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-size_t paged_attention_counters(int sm_count) { return ((size_t)sm_count * 4 + 255) / 256 * 256; }
+size_t paged_attention_counters(int sm_count) { return ((size_t)(sm_count + 1) * 4 + 255) / 256 * 256; }
 size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs) {
     if (!num_seqs) return 0;
     const PaChoice c = pa_choice(d, num_heads / num_kv_heads);
@@ -64,6 +64,7 @@ cudaError_t paged_attention_launch(cudaStream_t stream, int sm_count, const Page
     w.gave_up = a.gave_up;
     w.q_vec = a.c.d % 4 == 0 && a.q_stride % 4 == 0 && !((uintptr_t)a.q & 15);
     w.arrived = a.counters ? (u32*)a.counters : (u32*)a.workspace;
+    w.begun = w.arrived + sm_count;
     w.slots = (u32*)((char*)a.workspace + paged_attention_counters(sm_count));
     // Tensor copies want 16-byte boundaries; a box of less than the 8 rows of the swizzle's pattern is left to plain loads.
     CUtensorMap maps[2] = {};

@@ -46,7 +46,7 @@ struct PagedAttnArgs {
     int32_t* status;
     void* workspace;
     void* counters;                                          // paged_attention_counters bytes, zero before and after every call; NULL: the first of the workspace
-    int* gave_up;                                            // set when a wait inside a kernel ran out
+    int* gave_up;                                            // set when a wait inside a kernel ran out, blocks of a row are missing or parts of one are left over
 };
 size_t paged_attention_counters(int sm_count);
 size_t paged_attention_workspace(int sm_count, uint32_t num_heads, uint32_t num_kv_heads, uint32_t d, uint32_t num_seqs);

@@ -34,6 +34,12 @@ __device__ __forceinline__ bool mbar_try(u32 bar, u32 parity) {
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+// The same without waiting at all.
+__device__ __forceinline__ bool mbar_test(u32 bar, u32 parity) {
+    u32 ok;
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 // False when the phase did not end within the limit (each try suspends the thread for a while by itself; the limit is seconds), or
 // when another role of the CTA has given up.
 __device__ __forceinline__ bool mbar_wait(u32 bar, u32 parity, volatile int* gave_up) {

@@ -111,8 +111,8 @@ int32_t zkb_ctx_sync(zkb_ctx* c) {
         ZKB_CUDA(cudaStreamSynchronize(c->stream));
         if (c->serve_gave_up && *(volatile int*)c->serve_gave_up) {
             *c->serve_gave_up = 0;
-            if (c->serve_counters) ZKB_CUDA(cudaMemset(c->serve_counters, 0, zkb::paged_attention_counters(c->sm_count)));
-            throw ArgFail{ZKB_E_TIMEOUT, "a wait inside a kernel ran out: results of this context since its last synchronisation are not valid"};
+            if (c->serve_counters) ZKB_CUDA(cudaMemsetAsync(c->serve_counters, 0, zkb::paged_attention_counters(c->sm_count), c->stream));
+            throw ArgFail{ZKB_E_TIMEOUT, "a wait inside a kernel ran out, or lengths changed while a call read them: results of this context since its last synchronisation are not valid"};
         }
     });
 }

@@ -7,8 +7,8 @@ The reference's forward pass takes a whole sequence (rust/zk_ml_prover/src/pipel
 
 Arguments on the GPU are `DeviceBuffer`s, or tensors of another library on the context's GPU (anything with data_ptr, numel,
 element_size and is_contiguous, e.g. torch's).  Calls are enqueued on the context's stream (`Context.stream`) and not waited for: a
-caller that fills its tensors on another stream orders the two.  What only the device sees (`STATUS`) is added to the caller's status
-words, one per sequence, which `check_status` reads.
+caller that fills its tensors on another stream orders the two, and changes nothing that a call reads (lengths and block tables included)
+before it has run.  What only the device sees (`STATUS`) is added to the caller's status words, one per sequence, which `check_status` reads.
 """
 from __future__ import annotations
 
@@ -176,7 +176,7 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
 
 def paged_attention_workspace(cache: KvCache, num_seqs: int, num_heads: int) -> int:
     """Bytes of workspace for calls of this size: a captured call needs one of its own, 256-byte aligned, zeroed once before its first call and used by this
-    operator alone from then on."""
+    operator alone from then on (and zeroed again if a call on it gave up, ZkbError of code 8)."""
     _counts(num_seqs=num_seqs, num_heads=num_heads)
     return int(_fn("zkb_paged_attention_workspace")(cache.ctx.h, cache._at, num_seqs, num_heads))
 
