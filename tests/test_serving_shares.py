@@ -123,6 +123,8 @@ extern "C" int walk(u32 num_seqs, u32 kv_heads, u32 slices, u32 ctas, u32 block,
     }
     return 0;
 }
+
+extern "C" u32 halves(u32 tiles, u32 slot, u32 ns) { return pa_halves(tiles, slot, ns); }
 """
 
 
@@ -184,3 +186,10 @@ def test_lengths_that_change_meanwhile(lib):
         seen[rng.random((ctas, 3)) < rng.choice([0.05, 0.5])] = other
         told.append(call(lib, seqs, kv, slices, ctas, block, positions, seen, 3, False))
     assert {1, 2} <= set(told) and 0 in told
+
+
+@pytest.mark.parametrize("ns", [2, 3, 4, 6])
+def test_half_tiles_under_way(lib, ns):
+    """A warp that gives up waits for the last ns of its copies; keys and values are copied in turn, and it may be between the two."""
+    for n in range(3 * ns + 5):
+        assert lib.halves((n + 1) // 2, n % ns, ns) == n

@@ -128,6 +128,9 @@ ZKB_HD u32 pa_began(u32 cta, u32 ctas) { return cta ? 1u : 1u - ctas; }
 ZKB_HD u32 pa_brought(u32 parts, u32 added) { return (parts - added) << 16; }
 ZKB_HD bool pa_stale(u32 word) { return word != 0 && (word & 0xffffu) == 0; }
 
+// Half tiles that a warp has copied into a ring of ns slots, `slot` being the next one's: the last of its tiles with its values or without.
+ZKB_HD u32 pa_halves(u32 tiles, u32 slot, u32 ns) { return 2 * tiles % ns == slot ? 2 * tiles : 2 * tiles - 1; }
+
 // One output row (or its part) in shared memory to where it belongs.
 __device__ __forceinline__ void pa_finish(const PagedAttnArgs& A, u32 seq, u32 head, u32 e, u32 acc, u32 inv, u32 correction) {
     A.out[((size_t)seq * A.num_heads + head) * A.c.d + e] = mul31(sub31(acc, correction), inv);
@@ -688,9 +691,10 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
         }
     }
     if (gave_up) {                              // nothing of this warp may still be in flight when it ends
+        const u32 halves = pa_halves(loaded, slot_in, NS);
         for (u32 h = 0; h < NS; h++) {
-            const u32 last = 2 * loaded - 1 - h, use = last / NS;
-            if (h < 2 * loaded)
+            const u32 last = halves - 1 - h, use = last / NS;
+            if (h < halves)
                 for (u32 n = 0; n < (1u << 16) && !mbar_try(bar0 + 8 * (last % NS), use & 1); n++) {}
         }
         if (lane == 0) *P.gave_up = 1;
