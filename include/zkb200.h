@@ -38,7 +38,7 @@ enum {
     ZKB_E_NOT_QR = 5,       /* "compute_r: d/sum_sq is not a quadratic residue" (transformer/mod.rs:182) */
     ZKB_E_LENGTH = 6,       /* a length assertion of the reference failed (matmul.rs:161, 861) */
     ZKB_E_TOO_LARGE = 7,    /* request exceeds a documented fixed capacity */
-    ZKB_E_TIMEOUT = 8,      /* a peer GPU of a split sumcheck did not answer within the exchange's time limit, or a call of the token-by-token operators gave up (zkb_ctx_sync) */
+    ZKB_E_TIMEOUT = 8,      /* a peer GPU of a split sumcheck did not answer within the exchange's time limit, or a call of the token-by-token operators gave up (zkb_ctx_sync, zkb_buf_download_u32) */
     ZKB_E_DIV_ZERO = 9      /* batch_inverse met a zero element: p3's `.inverse()` panics there (lookup.rs:336, 358) */
 };
 
@@ -66,7 +66,8 @@ int32_t zkb_ctx_create(int32_t device, zkb_ctx** out);
 void zkb_ctx_destroy(zkb_ctx* ctx);
 const char* zkb_last_error(const zkb_ctx* ctx);
 /* Waits for the context's stream.  ZKB_E_TIMEOUT: a bounded wait inside a kernel of the token-by-token operators ran out (which no input causes), or the lengths
- * of an attention call changed while it ran; what the context computed since its last synchronisation is not valid. */
+ * of an attention call changed while it ran; what the context computed since its last synchronisation is not valid.  Reported once, by this call or by
+ * zkb_buf_download_u32, whichever comes first. */
 int32_t zkb_ctx_sync(zkb_ctx* ctx);
 /* A context keeps a scratch arena on the device that grows to what its largest proof needed and is
  * reused from then on (nothing is allocated per proof).  zkb_ctx_scratch_bytes reports its size;

@@ -179,6 +179,7 @@ struct zkb_ctx {
     }
     // Counters of the paged attention, zero between its calls (which are in order on `stream`); made at the first of them.
     void* serve_counters = nullptr;
+    size_t serve_counter_bytes = 0;
     void* serve_counts(size_t bytes) {
         if (!serve_counters) {
             void* p = nullptr;
@@ -186,8 +187,17 @@ struct zkb_ctx {
             const cudaError_t e = cudaMemsetAsync(p, 0, bytes, stream);
             if (e != cudaSuccess) { cudaFree(p); ZKB_CUDA(e); }
             serve_counters = p;
+            serve_counter_bytes = bytes;
         }
         return serve_counters;
+    }
+    // Once `stream` has been waited for, by the calls that hand results to the host: a call that gave up is reported, once, and its counters are cleared in
+    // front of the next one.
+    void serve_check() {
+        if (!serve_gave_up || !*(volatile int*)serve_gave_up) return;
+        *serve_gave_up = 0;
+        if (serve_counters) ZKB_CUDA(cudaMemsetAsync(serve_counters, 0, serve_counter_bytes, stream));
+        throw zkb::ArgFail{ZKB_E_TIMEOUT, "a wait inside a kernel ran out, or lengths changed while a call read them: results of this context since its last synchronisation are not valid"};
     }
     // Second stream for work that does not depend on the transcript (the fold / tree chain of a Basefold
     // opening), joined to `stream` through events; created on first use.

@@ -109,11 +109,7 @@ int32_t zkb_ctx_sync(zkb_ctx* c) {
     ZKB_TRY(c, {
         c->use();
         ZKB_CUDA(cudaStreamSynchronize(c->stream));
-        if (c->serve_gave_up && *(volatile int*)c->serve_gave_up) {
-            *c->serve_gave_up = 0;
-            if (c->serve_counters) ZKB_CUDA(cudaMemsetAsync(c->serve_counters, 0, zkb::paged_attention_counters(c->sm_count), c->stream));
-            throw ArgFail{ZKB_E_TIMEOUT, "a wait inside a kernel ran out, or lengths changed while a call read them: results of this context since its last synchronisation are not valid"};
-        }
+        c->serve_check();
     });
 }
 int32_t zkb_timer_start(zkb_ctx* c) {
@@ -229,6 +225,7 @@ int32_t zkb_buf_download_u32(zkb_ctx* c, const uint32_t* src, size_t n, uint32_t
         c->use();
         ZKB_CUDA(cudaMemcpyAsync(host, src, n * sizeof(u32), cudaMemcpyDeviceToHost, c->stream));
         ZKB_CUDA(cudaStreamSynchronize(c->stream));
+        c->serve_check();
     });
 }
 int32_t zkb_buf_free(zkb_ctx* c, uint32_t* dev) {
