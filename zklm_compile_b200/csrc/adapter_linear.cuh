@@ -287,8 +287,9 @@ __device__ __forceinline__ u32 lin_first(const LinPlan& p, u32 tile, u32 seg) { 
 __device__ __forceinline__ u32 lin_last(const LinPlan& p, u32 tile, u32 seg) {
     return (tile * p.steps + ((seg + 1) * LIN_SEG < p.steps ? (seg + 1) * LIN_SEG : p.steps) - 1) / p.per;
 }
-// Adds the slots' sums of rows row .. row + 3 of tile mt (one tile's; `vec`: row is a multiple of 4) for a token of tile nt.
-__device__ __forceinline__ void lin_sum4(const LinPlan& p, const u32* __restrict__ slots, u32 mt, u32 nt, u32 in_tile, u32 row, bool vec, u64 (&v)[4]) {
+// Adds the slots' sums of rows row .. row + 3 of tile mt (one tile's; `vec`: row is a multiple of 4) for a token of tile nt.  The slots are written while the join
+// is already there: they are no read-only memory to the compiler, and read from L2.
+__device__ __forceinline__ void lin_sum4(const LinPlan& p, const u32* slots, u32 mt, u32 nt, u32 in_tile, u32 row, bool vec, u64 (&v)[4]) {
     const u32 tile = mt * p.ntiles + nt;
     const u32* at = slots + (size_t)in_tile * LIN_ROWS + row;
     for (u32 seg = 0; seg < p.segs; seg++) {
@@ -297,12 +298,12 @@ __device__ __forceinline__ void lin_sum4(const LinPlan& p, const u32* __restrict
         if (vec) {
 #pragma unroll 4
             for (u32 c = from; c <= to; c++, s += p.slot_words) {
-                const uint4 x = *reinterpret_cast<const uint4*>(s);
+                const uint4 x = __ldcg(reinterpret_cast<const uint4*>(s));
                 v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
             }
         } else {
 #pragma unroll 4
-            for (u32 c = from; c <= to; c++, s += p.slot_words) { v[0] += s[0]; v[1] += s[1]; v[2] += s[2]; v[3] += s[3]; }
+            for (u32 c = from; c <= to; c++, s += p.slot_words) { v[0] += __ldcg(s); v[1] += __ldcg(s + 1); v[2] += __ldcg(s + 2); v[3] += __ldcg(s + 3); }
         }
     }
 }
@@ -315,7 +316,7 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
 // they lie in memory, read once for all tokens beside each other that have the same adapter (a run); each token's A x has four columns in the
 // right one, zero for the adapters of other tokens.  What bounds it is latency, slots first: 45 us for 1024 tokens of rank 32 and 4096 rows, 21 without adapters.
 constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 64;
-__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, int y_vec, const u32* __restrict__ slots, const u32* __restrict__ u_own) {
+__global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, int y_vec, const u32* slots, const u32* u_own) {
     __shared__ uint4 ud[LIN_JOIN_RANK / 16][LIN_JOIN_TOKENS / 2][32];              // digits of A x, 64 of the rank at a time
     __shared__ __align__(16) u32 lora[LIN_JOIN_TOKENS][LIN_JOIN_ROWS + 4];
     __shared__ int of[LIN_JOIN_TOKENS], run_of[LIN_JOIN_TOKENS], run_adapter[LIN_JOIN_TOKENS], runs;
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPl
             const u32 a_row = (u32)of[t] * rank + r0, in = a_row % LIN_ROWS;       // what lies behind the adapter's last row is not used
             if (!p.a_rows) {
 #pragma unroll
-                for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? u_own[(size_t)(t0 + t) * rank + r0 + k] : 0u;
+                for (u32 k = 0; k < 4; k++) v[k] = r0 + k < rank ? __ldcg(u_own + (size_t)(t0 + t) * rank + r0 + k) : 0u;
             } else if (in + 4 <= LIN_ROWS) {
                 lin_sum4(p, slots, p.wtiles + a_row / LIN_ROWS, nt, in_tile + t, in, rank % 4 == 0, v);
             } else {                             // the four lie in two tiles: each with the last four rows of its own
