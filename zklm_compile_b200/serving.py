@@ -106,26 +106,31 @@ def _rows(count: int, row: int, stride: int) -> int:
 class KvCache:
     """Pages of [num_kv_heads][page_size][d_head] elements for K and for V: field elements, or with `small` 16-bit centred integers.
     `k_pages` and `v_pages` are the caller's arrays; without them the cache allocates its own, zeroed.  `page_stride` (elements, 0: dense)
-    is the distance between pages, so that one array can hold both in turn."""
+    is the distance between pages, so that one array can hold both in turn.  What a cache is made with is fixed: the library holds its addresses and sizes."""
 
     def __init__(self, ctx: Context, page_size: int, num_kv_heads: int, d_head: int, num_pages: int, small: bool = False, k_pages=None, v_pages=None,
                  page_stride: int = 0):
-        self.ctx, self.page_size, self.num_kv_heads, self.d_head = ctx, int(page_size), int(num_kv_heads), int(d_head)
-        self.num_pages, self.small, self.page_stride = int(num_pages), bool(small), int(page_stride)
-        size, page = (2 if small else 4), self.num_kv_heads * self.page_size * self.d_head
+        page_size, num_kv_heads, d_head, num_pages, page_stride = int(page_size), int(num_kv_heads), int(d_head), int(num_pages), int(page_stride)
+        _counts(page_size=page_size, num_kv_heads=num_kv_heads, d_head=d_head, num_pages=num_pages)
+        size, page = (2 if small else 4), num_kv_heads * page_size * d_head
         if (k_pages is None) != (v_pages is None):
             raise ValueError("k_pages and v_pages: both or neither")
-        if min(page, self.num_pages) <= 0:
+        if min(page, num_pages) <= 0:
             raise ValueError("a cache has at least one page, key head and element")
-        reach = _rows(self.num_pages, page, self.page_stride)
+        reach = _rows(num_pages, page, page_stride)
         if k_pages is None:
             import numpy as np
             words = (reach * size + 3) // 4
             k_pages, v_pages = (ctx.upload(np.zeros(words, np.uint32)) for _ in range(2))
-        self.k_pages, self.v_pages = k_pages, v_pages
-        self._c = _Cache(_addr(ctx, k_pages, reach, "k_pages", size), _addr(ctx, v_pages, reach, "v_pages", size), self.page_stride, self.num_pages,
-                         self.page_size, self.num_kv_heads, self.d_head, int(self.small))
+        self._pages, self._ctx, self._row, self._d = (k_pages, v_pages), ctx, num_kv_heads * d_head, d_head
+        self._c = _Cache(_addr(ctx, k_pages, reach, "k_pages", size), _addr(ctx, v_pages, reach, "v_pages", size), page_stride, num_pages, page_size, num_kv_heads, d_head,
+                         int(bool(small)))
         self._at = C.addressof(self._c)
+
+    ctx = property(lambda self: self._ctx)
+    k_pages, v_pages = property(lambda self: self._pages[0]), property(lambda self: self._pages[1])
+    page_size, num_kv_heads, d_head = property(lambda self: self._c.page_size), property(lambda self: self._c.num_kv_heads), property(lambda self: self._c.d_head)
+    num_pages, page_stride, small = property(lambda self: self._c.num_pages), property(lambda self: self._c.page_stride), property(lambda self: bool(self._c.elem))
 
 
 class Rotation:
@@ -153,7 +158,7 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
     """Put k, v (num_tokens, num_kv_heads, d_head) into the cache: sequence s brings tokens row_start[s] .. row_start[s + 1] - 1, which get the positions
     from start[s] on; position p is row p % page_size of page block_table[s][p / page_size].  With a rotation K turns by its position, and so does
     q (num_tokens, num_heads, d_head) on its way to q_out (which may be q).  Rows outside every sequence are padding and left alone."""
-    ctx, t, s, blocks, heads, row = cache.ctx, num_tokens, num_seqs, max_blocks, num_heads, cache.num_kv_heads * cache.d_head
+    ctx, t, s, blocks, heads, row = cache._ctx, num_tokens, num_seqs, max_blocks, num_heads, cache._row
     if not (0 <= t <= _MAX and 0 <= s <= _MAX and 0 <= blocks <= _MAX and 0 <= heads <= _MAX):
         _counts(num_tokens=t, num_seqs=s, max_blocks=blocks, num_heads=heads)
     rot = q_at = q_out_at = None
@@ -161,7 +166,7 @@ def kv_append(cache: KvCache, k, v, num_tokens: int, block_table, num_seqs: int,
         rot = rotation._at
         rotation._c.cos_sin = _addr(ctx, rotation.cos_sin, rotation._words, "the rotation's table") if rotation._c.rot_dim else None
     if q is not None and q_out is not None:
-        q_row = heads * cache.d_head
+        q_row = heads * cache._d
         q_at = _addr(ctx, q, _rows(t, q_row, q_stride) if q_stride else t * q_row, "q")
         q_out_at = _addr(ctx, q_out, _rows(t, q_row, q_out_stride) if q_out_stride else t * q_row, "q_out")
     elif q is not None or q_out is not None:
@@ -186,7 +191,7 @@ def paged_attention(cache: KvCache, q, block_table, num_seqs: int, max_blocks: i
     """One new token per sequence: q (num_seqs, num_heads, d_head) over the first lens[s] positions of the cache, into out (num_seqs, num_heads, d_head).
     The score q . k_j, divided by 2^score_shift and rounded half away from zero, must be an input of the exp table; a sequence of length 0 and a
     row that is refused (status) give zeros.  `out` overlaps no input."""
-    ctx, s, blocks, heads, row = cache.ctx, num_seqs, max_blocks, num_heads, num_heads * cache.d_head
+    ctx, s, blocks, heads, row = cache._ctx, num_seqs, max_blocks, num_heads, num_heads * cache._d
     if not (0 <= s <= _MAX and 0 <= blocks <= _MAX and 0 <= heads <= _MAX and 0 <= score_shift <= _MAX):
         _counts(num_seqs=s, max_blocks=blocks, num_heads=heads, score_shift=score_shift)
     at, size = _workspace(ctx, workspace) if workspace is not None else (None, 0)
