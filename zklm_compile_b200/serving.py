@@ -79,6 +79,8 @@ def _addr_or_why(ctx: Context, x, least: int, what: str, size: int) -> int:
             raise ValueError(f"{what} lies on another GPU than the context")
         have = 4 * x.n
         at = C.cast(x.ptr, C.c_void_p).value or 0
+        if not at:
+            raise ValueError(f"{what} has been freed")
     else:
         try:
             at, unit, dense, on = x.data_ptr(), x.element_size(), x.is_contiguous(), x.get_device()
@@ -232,7 +234,8 @@ def adapter_linear(ctx: Context, x, w, tokens: int, m: int, n: int, out, bias=No
 
 
 def _workspace(ctx, w):
-    size = 4 if isinstance(w, DeviceBuffer) else w.element_size()
+    """A workspace may have elements of any size."""
+    size = 4 if isinstance(w, DeviceBuffer) else getattr(w, "itemsize", 1)
     at = _addr(ctx, w, 0, "workspace", size)
     return at, (4 * w.n if isinstance(w, DeviceBuffer) else w.numel() * size)
 
