@@ -534,11 +534,12 @@ int32_t zkb_oplist_prove(zkb_oplist* list, const uint32_t* x, uint8_t* out, size
 
 /* ---- token-by-token forward passes: a paged key-value cache, the attention that reads it, projections with adapters ----
  * No counterpart in the reference, whose forward pass takes whole sequences or one vector.  The arithmetic is its own, though: field
- * elements and the centred integers they stand for, so a row computed over the cache is the row that zkb_row_attention(_gqa)_forward
- * computes and zkb_prove_row_attention(_gqa) proves, and a projection with an adapter is the product with the merged matrix W + B A.
+ * elements and the centred integers they stand for, so a row computed over the cache with score_shift 0 is the row that
+ * zkb_row_attention(_gqa)_forward computes and zkb_prove_row_attention(_gqa) proves (those have neither a shift nor a mask: scores that need a shift to be inputs of
+ * the table have no proof there, and every row is one over the whole sequence), and a projection with an adapter is the product with the merged matrix W + B A.
  * All pointers are device memory of the context's GPU; calls are enqueued on the context's stream and nothing is waited for, so
  * they can be captured into a graph from that stream (after a first call outside, which loads the kernels).  What a call reads - tables, lengths and adapters' numbers
- * included - stays as it is until the call has run.  What only the device sees goes into the caller's status words, one per sequence:
+ * included - stays allocated and as it is until the call has run.  What only the device sees goes into the caller's status words, one per sequence:
  * status[s] becomes the largest code that a call found, and stays until the caller clears it. */
 enum { ZKB_SERVE_PAGE = 1,        /* a length or position outside the block table, or a page number outside the pool */
        ZKB_SERVE_ROTATION = 2,    /* a position that the rotation's table does not have */

@@ -63,7 +63,9 @@ inline bool lin_fits(u32 tokens, u32 m, u32 n, u32 a_rows) {
     return ((u64)((m + LIN_ROWS - 1) / LIN_ROWS) + (a_rows + LIN_ROWS - 1) / LIN_ROWS) * ((tokens + LIN_TOKENS - 1) / LIN_TOKENS) * ((n + LIN_STEP - 1) / LIN_STEP) < (1ull << 31);
 }
 // Rows of A that the product takes along with W's (all adapters for all tokens), or 0: then each token's own rank products are made apart.
-// Along, an adapter's rows are read once however many tokens use it and no launch is added; apart, no adapter that no token has is read.
+// Along, an adapter's rows are read once however many tokens use it and no launch is added; apart, no adapter that no token has is read.  2560 x 2560 and twelve adapters of
+// 16 for 1 / 64 / 1024 tokens: along 10.0 / 25 / 96 us, apart 10.3 / 25 / 112; 256 adapters: 16.7 / 35 / 212 and 12.3 / 29 / 140 (where the rule's second clause, which counts
+// bytes, takes the slower side at 1024).
 inline u32 lin_a_rows(u32 tokens, u32 m, u32 num_adapters, u32 rank) {
     const u64 rows = (u64)num_adapters * rank, tiles = (rows + LIN_ROWS - 1) / LIN_ROWS, wtiles = (m + LIN_ROWS - 1) / LIN_ROWS;
     return rows && (tiles <= (wtiles < 8 ? 1 : wtiles / 8) || tiles * LIN_ROWS <= (u64)tokens * rank / 2) && rows < (1u << 30) ? (u32)rows : 0u;
@@ -314,7 +316,8 @@ __device__ __forceinline__ u64 lin_dot4(const u32* a, const u32* b) {
 }
 // One CTA: `blocks` times 64 rows, up to 16 tokens of a tile of tokens.  B (A x) is a product of bytes too, on the warps' tensor cores: the rows of B are the left operand as
 // they lie in memory, read once for all tokens beside each other that have the same adapter (a run); each token's A x has four columns in the
-// right one, zero for the adapters of other tokens.  What bounds it is latency, slots first: 45 us for 1024 tokens of rank 32 and 4096 rows, 21 without adapters.
+// right one, zero for the adapters of other tokens; tokens of one adapter apart from each other are two runs, which read B twice (48 tokens of 9728 rows and twelve
+// adapters: 45 us in any order, 36 sorted by adapter, the whole call).  What bounds it is latency, slots first: 45 us for 1024 tokens of rank 32 and 4096 rows, 21 without adapters.
 constexpr u32 LIN_JOIN_ROWS = 64, LIN_JOIN_TOKENS = 16, LIN_JOIN_RANK = 64;
 __global__ void __launch_bounds__(256, 3) linear_join_kernel(LinearArgs A, LinPlan p, u32 blocks, int b_vec, int y_vec, const u32* slots, const u32* u_own) {
     __shared__ uint4 ud[LIN_JOIN_RANK / 16][LIN_JOIN_TOKENS / 2][32];              // digits of A x, 64 of the rank at a time

@@ -50,7 +50,7 @@ __device__ __forceinline__ void rotate_pair(u32& a, u32& b, int c, int s, u32 sh
 // 16 bytes at a time, for rows, rotations and addresses that are whole groups of 16 bytes (see kv_append_launch).  What bounds it is the copy: K, V and
 // Q in, the cache and Q out.  A row has `items` items: four neighbours, or where halves turn four elements and their four partners; a thread has the same item in
 // every row that it takes, so its cosines and sines stay in registers.  The first rows are read before the place is looked up.
-// 8111 tokens of 32 + 2 x 8 heads of 128 into a field cache (400 MB): 69 us, 5.8 TB/s.
+// 8111 tokens of 32 + 2 x 8 heads of 128, a quarter of each turned, into a field cache (400 MB): 69 us, 5.8 TB/s; into a 16-bit one (367 MB) 68 us.
 template <bool SMALL, bool PAIRS>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) kv_append_vec_kernel(AppendArgs A, u32 items, u32 rot_items) {
     constexpr u32 BATCH = PAIRS ? 6 : 3;                       // rows under way, 16 bytes or 32 of each

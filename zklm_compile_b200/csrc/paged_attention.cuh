@@ -18,8 +18,8 @@
 // is one list of blocks (positions of one sequence and key head) that the CTAs share evenly by its length, whatever the sequences' lengths are; a
 // row that CTAs share is added up by the one that brings its last part.  Integer sums have no order, so results do not depend on the split.
 //
-// Measured, heads of 128: 48 rows of up to 6000 positions, 8 x 4 heads, field 6.3 TB/s; one row over 131071, 8 x 4 heads, 16-bit 5.3 TB/s; 64 rows of up to
-// 5000, 8 x 8 heads, 16-bit 3.9 TB/s - there 810 instructions a tile and the registers that eight heads' sums take bound it.
+// Measured, heads of 128: 48 rows of up to 6000 positions, 8 x 4 heads, field 5.8 TB/s (190 us); one row over 131071, 8 x 4 heads, 16-bit 5.4 TB/s (99 us); 64 rows
+// of up to 5000, 8 x 8 heads, 16-bit 3.9 TB/s (230 us) - there 810 instructions a tile and the registers that eight heads' sums take bound it.
 #pragma once
 #include <type_traits>
 #include "m31.cuh"
@@ -42,8 +42,9 @@ __device__ __forceinline__ u32 inv31_chain(u32 x) {
 // How the kernels are built for a head of up to DP elements: warps, and half tiles (16 keys or 16 values) in a warp's ring.  A half tile lies as the
 // tensor copies leave it: columns of 128 bytes, 16 rows of one behind the other, the 16-byte groups of a row swizzled by the row's low bits.
 // Which position becomes which row of an operand is free, and is chosen so that no two lanes of a phase meet in a bank.  Warps: as many as the registers of
-// dp / 16 x nt x 4 sums a lane leave (twelve against eight with four heads of 128 in 16 bits: 103 against 110 us for 131071 positions); slots: about
-// 130 to 160 KB of them.
+// dp / 16 x nt x 4 sums a lane leave.  Twelve against eight, 131071 positions, 8 key heads with one / four heads each: 128 in 16 bits 90 / 94 against 94 / 105 us, 64 in 16 bits
+// 66 / 74 against 84 / 92, 64 in the field 89 / 91 against 91 / 103; a few rows of 77 positions lose what the set-up of four more warps takes, 7.5 to 9.5 us against 7.0 to 8.5.
+// Slots: about 130 to 160 KB of them.
 template <int DP, bool SMALL, int NT>
 struct PaShape {
     static constexpr int RB = DP * (SMALL ? 2 : 4);
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(PaShape<DP, SMALL, NT>::WARPS * 32, 1) paged_a
                 if (page0 >= 0) tensor_load_4d_one(dst + c * 2048, map, (int)(c * (128 / E)), (int)(kv_row + (pos0 & mask)), 0, page0, bar);
                 if (page1 >= 0) tensor_load_4d_one(dst + c * 2048 + 1024, map, (int)(c * (128 / E)), (int)(kv_row + ((pos0 + 8) & mask)), 0, page1, bar);
             }
-        } else {
+        } else {                               // a word at a time, nothing under way: 3.9 ms for the 48 rows in pages of four, against 0.2 by copies
             const u32 pos = pos0 + lane;
             const bool there = lane < 16 && pos < lw.len;
             const int page = there ? page_of(pos) : 0;

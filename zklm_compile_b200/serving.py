@@ -2,13 +2,16 @@
 
 The reference's forward pass takes a whole sequence (rust/zk_ml_prover/src/pipeline/forward.rs:233-276, 594-640) or one vector
 (transformer/mod.rs:140-163); these calls compute the same rows for one new token at a time, in the same exact arithmetic: what
-`paged_attention` returns over a cache is the row that `attention.row_attention_forward` returns over the whole sequence, and what
-`adapter_linear` returns is the product with the merged matrix W + B A.
+`paged_attention` returns over a cache with score_shift 0 is the row that `attention.row_attention_forward` returns over the whole sequence
+(which has neither a shift nor a mask: scores that need a shift to be inputs of the table have no proof there, and a row of a prompt is one
+over all of its positions), and what `adapter_linear` returns is the product with the merged matrix W + B A.
 
 Arguments on the GPU are `DeviceBuffer`s, or tensors of another library on the context's GPU (anything with data_ptr, numel,
 element_size and is_contiguous, e.g. torch's).  Calls are enqueued on the context's stream (`Context.stream`) and not waited for: a
 caller that fills its tensors on another stream orders the two, and changes nothing that a call reads (lengths and block tables included)
-before it has run.  What only the device sees (`STATUS`) is added to the caller's status words, one per sequence, which `check_status` reads.
+before it has run.  Memory is kept until then, too: a DeviceBuffer that is dropped waits for the stream, but torch's allocator hands a dropped
+tensor's memory out in the order of its own streams unless it is told, `x.record_stream(torch.cuda.ExternalStream(ctx.stream))`.  What only the
+device sees (`STATUS`) is added to the caller's status words, one per sequence, which `check_status` reads.
 """
 from __future__ import annotations
 
