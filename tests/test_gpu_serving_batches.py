@@ -202,3 +202,54 @@ def test_counters_that_somebody_left_are_reported(ctx):
 def sm_count():
     import torch
     return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def test_tokens_one_after_the_other_in_a_16_bit_cache(ctx):
+    """Append with rotation and attention for token after token, the values requantised by the caller in between: step by step, then captured once and replayed."""
+    import torch
+    rng = np.random.default_rng(8)
+    h, kv, d, page, room = 8, 2, 64, 16, 7
+    lens = [0, 15, 40, 131, 16]
+    b = len(lens)
+    paged = Paged(ctx, rng, [n + room for n in lens], kv, d, page, True)
+    angle = rng.uniform(0, 6.3, (max(lens) + room, d // 2))
+    cs = np.round(np.stack([np.cos(angle), np.sin(angle)], -1) * (1 << 14)).astype(np.int32)
+    exp, shift = tables.build_exp_table(1000), shift_for(d) + 1         # a turned vector's elements may be the square root of two larger
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    k, v, q, turned, out, status, start, after = z(b, kv, d), z(b, kv, d), z(b, h, d), z(b, h, d), z(b, h, d), z(b), z(b), z(b)
+    rows, cs_dev, exp_dev = (torch.from_numpy(a.astype(np.int32)).cuda() for a in (np.arange(b + 1), cs, exp))
+    rotation = zs.Rotation(cs_dev, len(cs), d, 14)
+    ws = torch.zeros(zs.paged_attention_workspace(paged.cache, b, h), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+
+    def step():
+        zs.kv_append(paged.cache, k, v, b, paged.table_dev, b, paged.max_blocks, rows, start, status, rotation=rotation, q=q, q_out=turned, num_heads=h)
+        zs.paged_attention(paged.cache, turned, paged.table_dev, b, paged.max_blocks, after, h, exp_dev, out, status, score_shift=shift, workspace=ws)
+
+    graph = None
+    for i in range(room):
+        new = [small(rng, 127, b, kv, d), small(rng, 32767, b, kv, d), small(rng, 127, b, h, d)]
+        with torch.cuda.stream(stream):
+            for to, a in zip((k, v, q), new):
+                to.copy_(torch.from_numpy(a.view(np.int32)))
+            start.copy_(torch.tensor(lens, dtype=torch.int32))
+            after.copy_(torch.tensor([n + 1 for n in lens], dtype=torch.int32))
+        if i == 3:
+            ctx.sync()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+                step()
+        if graph:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        else:
+            step()
+        zs.check_status(ctx, status)
+        want_q = np.zeros((b, h, d), np.int64)
+        assert not R.append(paged.k, paged.v, new[0], new[1], paged.table, list(range(b + 1)), lens, cs, 14, False, new[2], want_q, True).any()
+        lens = [n + 1 for n in lens]
+        want, codes = R.attend(paged.k, paged.v, want_q, paged.table, lens, exp, shift)
+        assert not codes.any() and np.array_equal(turned.cpu().numpy(), want_q) and np.array_equal(out.cpu().numpy(), want)
+        got_k, got_v = paged.fetch()
+        assert np.array_equal(got_k, paged.k) and np.array_equal(got_v, paged.v)
