@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(LinearArgs A, int v
     pdl_launch_dependents();
     const u32 r = blockIdx.x, t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int of = A.adapter_of[t];
-    if (of < 0 || (u32)of >= A.num_adapters) return;      // nobody reads this token's
+    if (__syncthreads_or(of < 0 || (u32)of >= A.num_adapters)) return;      // nobody reads this token's; all of the CTA or none (a number that changes meanwhile)
     const u32* a = A.a + ((size_t)of * A.rank + r) * A.n;
     const u32* x = A.x + t * A.x_stride;
     u64 acc = 0;
